@@ -39,6 +39,16 @@ extern "C" {
 #define LQ_KIND_INT4 4    /* weights: uint8 [rows, cols/2], two's-complement nibbles,
                              even column in the low nibble (quantize_int4.py:47-50) */
 #define LQ_KIND_ACT8 1    /* activations: int8 [rows, cols] signed (runq.c:133) */
+#define LQ_KIND_ROW8 2    /* int8 signed, one fp32 scale per row (group_size = cols): rows of
+                             LQ_ROW8_PITCH(cols) bytes, zeros past cols; activations (a scale
+                             per token) and weights (a scale per output channel) alike */
+#define LQ_ROW8_PITCH(cols) (((cols) + 15) / 16 * 16)
+
+/* element types of the activations that the calls below "token-scaled
+ * products" and "paged cache" take and give */
+#define LQ_F32 0
+#define LQ_F16 1
+#define LQ_BF16 2
 
 /* Group-quantized tensor (replaces QWeight, v1-int8-vnni/runq.c:43-49, and
  * DQWeight, v5-cuda-fused/run.cu:61-65; the activation form replaces the
@@ -79,7 +89,9 @@ void* lq_get_stream(void);
  * words of the operator calls on the current device: the context's, and the
  * fixed scratch's when matmul_f32_noalloc has been used there.  A bounded
  * device wait that gave up in any earlier call makes this return
- * LQ_ETIMEOUT. */
+ * LQ_ETIMEOUT, and a page number, position or row count that a paged-cache call
+ * found outside its bounds on the device (that part of the call was left out)
+ * LQ_EINVAL. */
 int lq_sync(void);
 
 /* Launch flags for the operator entry points.  LQ_LAUNCH_PDL lets each
@@ -153,6 +165,108 @@ int matmul_f32(float* xout, const float* x, const QuantizedTensor* w, int n, int
  * of these calls (a bounded wait that gave up) is kept in the array until
  * the next lq_sync() reports it. */
 int matmul_f32_noalloc(float* xout, const float* x, const QuantizedTensor* w, int n, int d);
+
+/* ---- token-scaled products ----------------------------------------------
+ * The int8 product with one scale per token and one per output channel, next
+ * to the group-scaled one above (no counterpart in the reference, whose
+ * scales are per group of 32).  Any cols from 1 to 131072 (an int32 holds the
+ * dot of that many codes), any row counts.  All device memory. */
+
+/* Quantize out->rows rows of x (type LQ_F32 / LQ_F16 / LQ_BF16, row r at
+ * element r * ld, ld >= n): s = max|x|/127 over the row (0 -> 1e-8), q =
+ * rint(x/s).  out->q: int8 [rows][LQ_ROW8_PITCH(n)], 16-byte aligned, padding
+ * written as zeros; out->s: fp32 [rows].  Sets cols = group_size = n and kind =
+ * LQ_KIND_ROW8.  A row that holds a NaN or an infinity gets the scale NaN and
+ * zero codes, so that its products are NaN.  Quantizes weights the same way. */
+int quantize_rows(QuantizedTensor* out, const void* x, int type, int64_t ld, int n);
+
+/* xout[b, i] = (sum_k x.q[b, k] * w.q[i, k]) * (x.s[b] * w.s[i]): the sum
+ * exact in int32, rounded once to fp32, then two fp32 products and the
+ * rounding to `type`.  x, w: LQ_KIND_ROW8, [B, n] and [d, n], x->rows >= 0; row b
+ * of xout starts at element b * ld (ld >= d).  x->q and w->q 16-byte aligned. */
+int matmul_rows(void* xout, int type, int64_t ld, const QuantizedTensor* x, const QuantizedTensor* w, int n, int d);
+
+/* ---- paged cache ----------------------------------------------------------
+ * A KV cache of int8 pages shared by many sequences, one scale per (page, kv
+ * head, K or V), with the append that fills it and the attention that reads
+ * it.  The model's own cache is fp32 and contiguous per sequence; the
+ * reference's int8 cache (v5-cuda-fused/run.cu:46-48, off by default) has one
+ * scale per token and head. */
+
+/* The cache: page_size tokens a page.  codes: int8
+ * [n_pages][n_kv_heads][K, V][head_size * page_size], where K of a page is
+ * [head_size / 16][page_size][16] (16 dims of one token together) and V is
+ * [page_size / 16][head_size][16] (16 tokens of one dim together): both are
+ * K-major tensor-core operands as they lie.  A token's value is code * scale.
+ * scales: fp32 [n_pages][n_kv_heads][K, V].  Fresh memory needs no clearing: a
+ * page's scale is set when its first token arrives. */
+typedef struct PagedKV {
+    void* codes;        /* device, 16-byte aligned */
+    float* scales;      /* device, 8-byte aligned */
+    int64_t n_pages;
+    int32_t page_size;  /* 16, 32, 64 or 128 */
+    int32_t n_kv_heads;
+    int32_t head_size;  /* multiple of 16, 16 to 256 */
+    int32_t reserved;   /* 0 */
+} PagedKV;
+
+/* The sequences of one call.  Rows row_start[s] .. row_start[s + 1] - 1 of the
+ * call's tensors are the newest tokens of sequence s: its last row is at
+ * position context[s] - 1.  Rows whose position would be negative (more rows
+ * than context) are no tokens: kv_append leaves them alone and they attend
+ * to nothing.  The token at position p is in page pages[s][p / page_size].
+ * No page is shared by two sequences of a kv_append call. */
+typedef struct KVBatch {
+    const int32_t* row_start; /* device [n_seqs + 1], ascending from 0 to n_rows */
+    const int32_t* context;   /* device [n_seqs]: tokens with this call's */
+    const int32_t* pages;     /* device [n_seqs][max_pages] */
+    int32_t n_seqs;
+    int32_t n_rows;
+    int32_t max_pages;
+    int32_t max_rows;         /* at least the rows of any one sequence */
+    int32_t max_context;      /* at least every context[s] */
+} KVBatch;
+
+/* The rows that kv_append takes and gives; head h of row r of a tensor is at
+ * element r * ld + h * head_size. */
+#define LQ_ROPE_PAIRS 0  /* dims 2i and 2i + 1 turn together (runq.c:352-367) */
+#define LQ_ROPE_HALVES 1 /* dims i and i + head_size / 2 turn together */
+typedef struct KVRows {
+    const void* q;      /* may be null: no queries */
+    const void* k;
+    const void* v;
+    void* q_out;        /* rotated queries; may be q itself */
+    void* k_out;        /* code * scale of the new rows as the cache now holds them; may be null */
+    void* v_out;
+    int64_t ld_q, ld_k, ld_v, ld_q_out;
+    int64_t ld_kv_out;  /* of k_out and v_out */
+    int32_t n_heads;    /* query heads */
+    int32_t type;       /* LQ_F32, LQ_F16 or LQ_BF16, of all six */
+    const float* rope;  /* [rope_rows][head_size / 2] of (cos, sin); null: no rotation */
+    int32_t rope_rows;
+    int32_t rope_mode;  /* LQ_ROPE_* */
+} KVRows;
+
+/* Fill a rotation table in host memory: (cos, sin) of p * base^(-2i/head_size)
+ * for p < positions, i < head_size / 2 (runq.c:352-367 with base 10000). */
+int lq_rope_table(float* table, int positions, int head_size, float base);
+
+/* Append the call's keys (rotated by their positions) and values to the cache,
+ * and rotate its queries.  A page's scale is max|x|/127 over the tokens it has
+ * ever held since its first one arrived (0 -> 1e-8); when new tokens raise it
+ * from s to s', the codes of the earlier ones become rint(code * (s / s')).
+ * A NaN or an infinity makes the scale of its page and head NaN (codes zero)
+ * until the page is begun again. */
+int kv_append(const PagedKV* cache, const KVBatch* batch, const KVRows* rows);
+
+/* Causal attention of every row over its sequence's cache, its own position
+ * included: out = softmax(scale * q . K) V per head, n_heads a multiple of
+ * n_kv_heads (query head h reads kv head h / (n_heads / n_kv_heads)).  out and q
+ * of `type`, head h of row r at element r * ld + h * head_size.  lse (may be
+ * null): fp32 [n_rows][n_heads], log of the sum of exp(scale * q . K).  A row that
+ * attends to nothing gives zeros and lse -inf. */
+int paged_attention(void* out, int64_t ld_out, const void* q, int64_t ld_q, int type, int n_heads,
+                    const PagedKV* cache, const KVBatch* batch, float scale, float* lse);
 
 /* ---- model ------------------------------------------------------------- */
 

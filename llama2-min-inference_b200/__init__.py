@@ -28,6 +28,11 @@ RUNNER_PATH = os.path.join(_HERE, "bin", "run")
 KIND_INT8 = 8
 KIND_INT4 = 4
 KIND_ACT8 = 1
+KIND_ROW8 = 2
+
+# element types of the token-scaled products and the paged cache
+F32, F16, BF16 = range(3)
+ROPE_PAIRS, ROPE_HALVES = range(2)
 
 OK, EINVAL, ECUDA, ENOMEM, EIO, EFORMAT, ETIMEOUT, EUNSUPPORTED = range(8)
 
@@ -79,11 +84,64 @@ class Config(C.Structure):
                 self.vocab_size, self.seq_len)
 
 
+class PagedKV(C.Structure):
+    """PagedKV of include/llama2q.h: the int8 cache of pages."""
+
+    _fields_ = [
+        ("codes", C.c_void_p),
+        ("scales", C.c_void_p),
+        ("n_pages", C.c_int64),
+        ("page_size", C.c_int32),
+        ("n_kv_heads", C.c_int32),
+        ("head_size", C.c_int32),
+        ("reserved", C.c_int32),
+    ]
+
+
+class KVBatch(C.Structure):
+    """KVBatch of include/llama2q.h: the sequences of one call."""
+
+    _fields_ = [
+        ("row_start", C.c_void_p),
+        ("context", C.c_void_p),
+        ("pages", C.c_void_p),
+        ("n_seqs", C.c_int32),
+        ("n_rows", C.c_int32),
+        ("max_pages", C.c_int32),
+        ("max_rows", C.c_int32),
+        ("max_context", C.c_int32),
+    ]
+
+
+class KVRows(C.Structure):
+    """KVRows of include/llama2q.h: the rows kv_append takes and gives."""
+
+    _fields_ = [
+        ("q", C.c_void_p),
+        ("k", C.c_void_p),
+        ("v", C.c_void_p),
+        ("q_out", C.c_void_p),
+        ("k_out", C.c_void_p),
+        ("v_out", C.c_void_p),
+        ("ld_q", C.c_int64),
+        ("ld_k", C.c_int64),
+        ("ld_v", C.c_int64),
+        ("ld_q_out", C.c_int64),
+        ("ld_kv_out", C.c_int64),
+        ("n_heads", C.c_int32),
+        ("type", C.c_int32),
+        ("rope", C.c_void_p),
+        ("rope_rows", C.c_int32),
+        ("rope_mode", C.c_int32),
+    ]
+
+
 # names the C ABI exports (checked by the CPU test suite against the header)
 EXPORTS = (
     "lq_last_error", "lq_select_device", "lq_set_stream", "lq_get_stream", "lq_sync",
     "lq_set_launch_flags", "lq_set_trace", "lq_graph_begin", "lq_graph_end", "lq_graph_launch", "lq_graph_destroy",
     "lq_synth_tensor", "quantize", "matmul", "matmul_f32", "matmul_f32_noalloc",
+    "quantize_rows", "matmul_rows", "lq_rope_table", "kv_append", "paged_attention",
     "build_transformer", "build_transformer_random", "forward", "forward_argmax", "forward_prompt",
     "transformer_reserve_batch", "forward_batch", "forward_batch_argmax",
     "lq_tp_unique_id", "build_transformer_tp", "build_transformer_random_tp", "lq_tp_wait_selftest",
@@ -123,6 +181,11 @@ def lib() -> C.CDLL:
         "matmul": (I, [P, QT, QT, I, I]),
         "matmul_f32": (I, [P, P, QT, I, I]),
         "matmul_f32_noalloc": (I, [P, P, QT, I, I]),
+        "quantize_rows": (I, [QT, P, I, I64, I]),
+        "matmul_rows": (I, [P, I, I64, QT, QT, I, I]),
+        "lq_rope_table": (I, [P, I, I, F]),
+        "kv_append": (I, [C.POINTER(PagedKV), C.POINTER(KVBatch), C.POINTER(KVRows)]),
+        "paged_attention": (I, [P, I64, P, I64, I, I, C.POINTER(PagedKV), C.POINTER(KVBatch), F, P]),
         "build_transformer": (I, [C.POINTER(P), C.c_char_p, I]),
         "build_transformer_random": (I, [C.POINTER(P), CFG, I, I, U64, I]),
         "forward": (C.POINTER(F), [P, I, I]),
@@ -227,6 +290,54 @@ def matmul_f32(xout_ptr: int, x_ptr: int, w: QuantizedTensor, n: int, d: int) ->
 def matmul_f32_noalloc(xout_ptr: int, x_ptr: int, w: QuantizedTensor, n: int, d: int) -> None:
     """matmul_f32 without any device allocation (fixed library scratch, n <= 32768, device pointers)."""
     check(lib().matmul_f32_noalloc(C.c_void_p(xout_ptr), C.c_void_p(x_ptr), C.byref(w), n, d))
+
+
+def quantize_rows(out: QuantizedTensor, x_ptr: int, n: int, dtype: int = F32, ld: int | None = None) -> None:
+    """One scale per row of x [out.rows, n] (rows ld elements apart) into out, kind ROW8."""
+    rc = lib().quantize_rows(out, x_ptr, dtype, n if ld is None else ld, n)
+    if rc != OK:
+        raise LlamaQError(rc, last_error())
+
+
+def matmul_rows(xout_ptr: int, x: QuantizedTensor, w: QuantizedTensor, n: int, d: int, dtype: int = F32,
+                ld: int | None = None) -> None:
+    """xout[B, d] = W[d, n] . x[B, n], both of kind ROW8 (a scale per channel, a scale per token)."""
+    rc = lib().matmul_rows(xout_ptr, dtype, d if ld is None else ld, x, w, n, d)
+    if rc != OK:
+        raise LlamaQError(rc, last_error())
+
+
+def row8_pitch(cols: int) -> int:
+    """Bytes of a ROW8 row."""
+    return (cols + 15) // 16 * 16
+
+
+def rope_table(positions: int, head_size: int, base: float = 10000.0):
+    """numpy [positions, head_size / 2, 2] of (cos, sin) for kv_append."""
+    import numpy as np
+
+    t = np.empty((max(positions, 0), head_size // 2, 2), np.float32)
+    check(lib().lq_rope_table(t.ctypes.data, positions, head_size, base))
+    return t
+
+
+def kv_append(cache: PagedKV, batch: KVBatch, rows: KVRows) -> None:
+    """Append the batch's keys (rotated) and values to the paged cache, rotate its queries."""
+    rc = lib().kv_append(cache, batch, rows)
+    if rc != OK:
+        raise LlamaQError(rc, last_error())
+
+
+def paged_attention(out_ptr: int, q_ptr: int, n_heads: int, cache: PagedKV, batch: KVBatch, dtype: int = F32,
+                    scale: float | None = None, ld_out: int | None = None, ld_q: int | None = None,
+                    lse_ptr: int | None = None) -> None:
+    """Causal attention of the batch's rows over the paged cache (scale: 1 / sqrt(head_size) when None)."""
+    row = n_heads * cache.head_size
+    rc = lib().paged_attention(out_ptr, row if ld_out is None else ld_out, q_ptr, row if ld_q is None else ld_q,
+                               dtype, n_heads, cache, batch,
+                               cache.head_size ** -0.5 if scale is None else scale, lse_ptr)
+    if rc != OK:
+        raise LlamaQError(rc, last_error())
 
 
 # ---- model -------------------------------------------------------------------

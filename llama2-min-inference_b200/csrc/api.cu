@@ -101,6 +101,8 @@ int check_device_error(int* err_dev, cudaStream_t st) {
     if (h != 0) {
         cudaMemsetAsync(err_dev, 0, sizeof(int), st);
         cudaStreamSynchronize(st);
+        if (h >= 0x202)  // the paged cache's checks (lq_paged.cuh)
+            return lq_fail(LQ_EINVAL, "a page, position or row count was out of bounds on the device (code 0x%x)", h);
         return lq_fail(LQ_ETIMEOUT, "device-side wait gave up (code 0x%x)", h);
     }
     return LQ_OK;

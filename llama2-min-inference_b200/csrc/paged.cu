@@ -1,0 +1,340 @@
+// kv_append: rotation by position, int8 quantization into the paged cache, and
+// the host checks that the paged-cache entry points share.
+#include <cmath>
+
+#include "lq_ctx.h"
+#include "lq_paged.cuh"
+#include "lq_paged_host.h"
+#include "lq_types.cuh"
+
+namespace lq {
+namespace {
+
+constexpr int kAppendThreads = 128;
+
+struct AppendArgs {
+    PagedKV c;
+    KVBatch b;
+    KVRows r;
+    int* err;
+    int jobs;      // page jobs (per kv head)
+    int q_blocks;  // query blocks per row
+};
+
+// dims d .. d + 3 of a row, rotated as its position asks.  d is a multiple of
+// 4.  The products and sums are separate fp32 operations (no fused multiply-add).
+template <typename T, bool VEC>
+__device__ __forceinline__ void rotated4(const T* x, const float* tab, int hs, int mode, int d, float (&v)[4]) {
+    load_n<4, VEC>(x + d, v);
+    if (!tab) return;
+    if (mode == LQ_ROPE_PAIRS) {
+        const float2 t0 = reinterpret_cast<const float2*>(tab)[d / 2], t1 = reinterpret_cast<const float2*>(tab)[d / 2 + 1];
+        const float a0 = v[0], b0 = v[1], a1 = v[2], b1 = v[3];
+        v[0] = a0 * t0.x - b0 * t0.y;
+        v[1] = a0 * t0.y + b0 * t0.x;
+        v[2] = a1 * t1.x - b1 * t1.y;
+        v[3] = a1 * t1.y + b1 * t1.x;
+    } else {
+        const int half = hs / 2;  // a multiple of 8: the four dims lie in one half
+        const bool up = d >= half;
+        float o[4];
+        load_n<4, VEC>(x + (up ? d - half : d + half), o);
+        const float2* t = reinterpret_cast<const float2*>(tab) + (up ? d - half : d);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = up ? o[e] * t[e].y + v[e] * t[e].x : v[e] * t[e].x - o[e] * t[e].y;
+    }
+}
+
+__device__ __forceinline__ float append_scale(uint32_t amax_bits, float old) {
+    const float s = __uint_as_float(amax_bits) / 127.0f;
+    float m = s > old ? s : old;
+    if (m == 0.0f) m = 1e-8f;
+    if (amax_bits >= kInfBits || !(old < __uint_as_float(kInfBits))) m = __uint_as_float(0x7FC00000u);
+    return m;
+}
+
+// Blocks [0, jobs * n_kv_heads): one (page, kv head) that receives tokens.
+// Sequence s owns the jobs from row_start[s] / page + 2 s on, which are at
+// least as many as the pages that its rows touch.
+// The other blocks: rotated queries, one row and a slice of its heads each.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_constant__ AppendArgs a) {
+    pdl_trigger();
+    pdl_wait();
+    const int tid = threadIdx.x;
+    const int hs = a.c.head_size, P = a.c.page_size, H = a.c.n_kv_heads;
+    const int64_t kv_blocks = (int64_t)a.jobs * H;
+    if (blockIdx.x >= kv_blocks) {
+        const int64_t qb = blockIdx.x - kv_blocks;
+        const int row = (int)(qb / a.q_blocks), part = (int)(qb % a.q_blocks);
+        int s = -1;  // the last sequence whose rows begin at or before `row`
+        for (int i0 = 0; i0 < a.b.n_seqs; i0 += kAppendThreads) {
+            const int c = __syncthreads_count(i0 + tid < a.b.n_seqs && __ldg(a.b.row_start + i0 + tid) <= row);
+            s += c;
+            if (c < kAppendThreads) break;
+        }
+        if (s < 0) return;
+        const SeqRows q = seq_rows(a.b, s, tid == 0 ? a.err : nullptr);
+        if (row < q.r0 || row >= q.r0 + q.n) return;
+        const int pos = q.begin + (row - q.r0);
+        const float* tab = nullptr;
+        if (a.r.rope) {
+            if (pos >= a.r.rope_rows) {
+                if (tid == 0) set_err(a.err, DEV_BAD_POS);
+                return;
+            }
+            tab = a.r.rope + (int64_t)pos * hs;
+        }
+        const int i = (part * kAppendThreads + tid) * 8;  // 8 dims of a head
+        if (i >= a.r.n_heads * hs) return;
+        const int h = i / hs, d = i - h * hs;
+        const T* x = static_cast<const T*>(a.r.q) + (int64_t)row * a.r.ld_q + (int64_t)h * hs;
+        T* y = static_cast<T*>(a.r.q_out) + (int64_t)row * a.r.ld_q_out + (int64_t)h * hs;
+        // in place, both halves of a pair have to be read before either is written
+        if (a.r.rope_mode == LQ_ROPE_HALVES && tab) {
+            const int half = hs / 2, p0 = d / 2;  // pairs p0 .. p0 + 3
+            float lo[4], hi[4];
+            rotated4<T, VEC>(x, tab, hs, LQ_ROPE_HALVES, p0, lo);
+            rotated4<T, VEC>(x, tab, hs, LQ_ROPE_HALVES, p0 + half, hi);
+            store_n<4, VEC>(y + p0, lo);
+            store_n<4, VEC>(y + p0 + half, hi);
+        } else {
+            float v0[4], v1[4];
+            rotated4<T, VEC>(x, tab, hs, LQ_ROPE_PAIRS, d, v0);
+            rotated4<T, VEC>(x, tab, hs, LQ_ROPE_PAIRS, d + 4, v1);
+            store_n<4, VEC>(y + d, v0);
+            store_n<4, VEC>(y + d + 4, v1);
+        }
+        return;
+    }
+
+    const int job = blockIdx.x / H, h = blockIdx.x % H;
+    int s = -1;
+    for (int i0 = 0; i0 < a.b.n_seqs; i0 += kAppendThreads) {
+        const int i = i0 + tid;
+        const int c = __syncthreads_count(i < a.b.n_seqs && __ldg(a.b.row_start + i) / P + 2 * i <= job);
+        s += c;
+        if (c < kAppendThreads) break;
+    }
+    if (s < 0) return;
+    const SeqRows q = seq_rows(a.b, s, tid == 0 ? a.err : nullptr);
+    if (q.n <= 0) return;
+    const int lp = q.begin / P + (job - (__ldg(a.b.row_start + s) / P + 2 * s));
+    const int t0 = max(q.begin, lp * P), t1 = min(q.ctx, lp * P + P);  // the page's new tokens
+    if (t0 >= t1) return;
+    if (a.r.rope && t1 > a.r.rope_rows) {
+        if (tid == 0) set_err(a.err, DEV_BAD_POS);
+        return;
+    }
+    const int64_t page = page_of(a.c, a.b, s, lp, tid == 0 ? a.err : nullptr);
+    if (page < 0) return;
+    const int64_t cell = page * H + h;
+    int8_t* kc = static_cast<int8_t*>(a.c.codes) + cell * 2 * hs * P;
+    int8_t* vc = kc + (int64_t)hs * P;
+    const int row0 = q.r0 + (t0 - q.begin), nt = t1 - t0, off = t0 - lp * P;
+    const T* kr = static_cast<const T*>(a.r.k) + (int64_t)row0 * a.r.ld_k + (int64_t)h * hs;
+    const T* vr = static_cast<const T*>(a.r.v) + (int64_t)row0 * a.r.ld_v + (int64_t)h * hs;
+    const float* tab0 = a.r.rope ? a.r.rope + (int64_t)t0 * hs : nullptr;
+
+    // the maxima of the new tokens
+    uint32_t mk = 0, mv = 0;
+    for (int i = tid; i < nt * (hs / 4); i += kAppendThreads) {
+        const int t = i / (hs / 4), d = 4 * (i - t * (hs / 4));
+        float k[4], v[4];
+        rotated4<T, VEC>(kr + t * a.r.ld_k, tab0 ? tab0 + (int64_t)t * hs : nullptr, hs, a.r.rope_mode, d, k);
+        load_n<4, VEC>(vr + t * a.r.ld_v + d, v);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            mk = max(mk, abs_bits(k[e]));
+            mv = max(mv, abs_bits(v[e]));
+        }
+    }
+    __shared__ uint32_t wk[kAppendThreads / 32], wv[kAppendThreads / 32];
+    mk = __reduce_max_sync(0xffffffffu, mk);
+    mv = __reduce_max_sync(0xffffffffu, mv);
+    if ((tid & 31) == 0) {
+        wk[tid >> 5] = mk;
+        wv[tid >> 5] = mv;
+    }
+    float old_k = 0.0f, old_v = 0.0f;  // a page whose first token arrives now starts afresh
+    if (off > 0) {
+        old_k = a.c.scales[cell * 2];
+        old_v = a.c.scales[cell * 2 + 1];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kAppendThreads / 32; ++w) {
+        mk = max(mk, wk[w]);
+        mv = max(mv, wv[w]);
+    }
+    const float sk = append_scale(mk, old_k), sv = append_scale(mv, old_v);
+    const bool bad_k = sk != sk, bad_v = sv != sv;
+    if (tid == 0) {
+        a.c.scales[cell * 2] = sk;
+        a.c.scales[cell * 2 + 1] = sv;
+    }
+    // earlier tokens at the grown scale (a NaN scale leaves nothing to keep)
+    const bool grow_k = off > 0 && sk != old_k, grow_v = off > 0 && sv != old_v;
+    auto again = [](uint32_t word, float ratio) {
+        int o[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = __float2int_rn((float)(int8_t)(word >> (8 * e)) * ratio);
+        return pack8(o[0], o[1], o[2], o[3]);
+    };
+    if (grow_k) {
+        const float ratio = bad_k ? 0.0f : old_k / sk;
+        for (int i = tid; i < off * (hs / 4); i += kAppendThreads) {
+            const int t = i % off, w = i / off;  // word w (4 dims) of token t
+            uint32_t* p = reinterpret_cast<uint32_t*>(kc + ((int64_t)(w / 4) * P + t) * 16) + (w & 3);
+            *p = again(*p, ratio);
+        }
+    }
+    // new keys: 4 dims of a token are one word
+    for (int i = tid; i < nt * (hs / 4); i += kAppendThreads) {
+        const int t = i / (hs / 4), d = 4 * (i - t * (hs / 4));
+        float k[4];
+        rotated4<T, VEC>(kr + t * a.r.ld_k, tab0 ? tab0 + (int64_t)t * hs : nullptr, hs, a.r.rope_mode, d, k);
+        int c[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) c[e] = bad_k ? 0 : quant8(k[e], sk);
+        *reinterpret_cast<uint32_t*>(kc + ((int64_t)(d / 16) * P + off + t) * 16 + d % 16) = pack8(c[0], c[1], c[2], c[3]);
+        if (a.r.k_out) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) k[e] = (float)c[e] * sk;
+            store_n<4, VEC>(static_cast<T*>(a.r.k_out) + (int64_t)(row0 + t) * a.r.ld_kv_out + (int64_t)h * hs + d, k);
+        }
+    }
+    // values: a word is 4 tokens of a dim; the words that hold tokens up to the
+    // last new one, earlier tokens in them kept or rescaled, later bytes kept
+    const float ratio_v = bad_v ? 0.0f : old_v / sv;
+    const int w0 = grow_v ? 0 : off / 4, w1 = (off + nt + 3) / 4;
+    for (int i = tid; i < (w1 - w0) * hs; i += kAppendThreads) {
+        const int w = w0 + i / hs, d = i % hs;
+        uint32_t* p = reinterpret_cast<uint32_t*>(vc + ((int64_t)(w / 4) * hs + d) * 16) + (w & 3);
+        const bool whole = 4 * w >= off && 4 * w + 4 <= off + nt;
+        uint32_t word = whole ? 0u : *p;
+        if (grow_v && 4 * w < off) {
+            const int keep = off - 4 * w;  // bytes of earlier tokens
+            const uint32_t mask = keep >= 4 ? 0xFFFFFFFFu : (1u << (8 * keep)) - 1u;
+            word = (again(word, ratio_v) & mask) | (word & ~mask);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int t = 4 * w + e - off;
+            if (t < 0 || t >= nt) continue;
+            const float x = to_f32(vr[t * a.r.ld_v + d]);
+            const int c = bad_v ? 0 : quant8(x, sv);
+            word = (word & ~(0xFFu << (8 * e))) | ((uint32_t)(c & 255) << (8 * e));
+            if (a.r.v_out)
+                static_cast<T*>(a.r.v_out)[(int64_t)(row0 + t) * a.r.ld_kv_out + (int64_t)h * hs + d] =
+                    from_f32<T>((float)c * sv);
+        }
+        *p = word;
+    }
+}
+
+template <typename T>
+cudaError_t append_t(const AppendArgs& a, cudaStream_t st) {
+    const KVRows& r = a.r;
+    const uintptr_t bytes = 4 * sizeof(T);
+    auto fits = [&](const void* p, int64_t ld) { return !p || (reinterpret_cast<uintptr_t>(p) % bytes == 0 && ld % 4 == 0); };
+    const bool vec = fits(r.q, r.ld_q) && fits(r.k, r.ld_k) && fits(r.v, r.ld_v) && fits(r.q_out, r.ld_q_out) &&
+                     fits(r.k_out, r.ld_kv_out) && fits(r.v_out, r.ld_kv_out);
+    const int64_t blocks = (int64_t)a.jobs * a.c.n_kv_heads + (r.q ? (int64_t)a.b.n_rows * a.q_blocks : 0);
+    if (blocks > INT32_MAX) return cudaErrorInvalidConfiguration;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)blocks);
+    cfg.blockDim = dim3(kAppendThreads);
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return vec ? cudaLaunchKernelEx(&cfg, append_kernel<T, true>, a) : cudaLaunchKernelEx(&cfg, append_kernel<T, false>, a);
+}
+
+}  // namespace
+
+int check_paged(const PagedKV* c, const KVBatch* b, int n_heads, int type, const char* fn) {
+    if (!c || !b) return lq_fail(LQ_EINVAL, "%s: null argument", fn);
+    if (type != LQ_F32 && type != LQ_F16 && type != LQ_BF16) return lq_fail(LQ_EINVAL, "%s: type %d", fn, type);
+    if (c->page_size != 16 && c->page_size != 32 && c->page_size != 64 && c->page_size != 128)
+        return lq_fail(LQ_EINVAL, "%s: page size %d (16, 32, 64 or 128)", fn, c->page_size);
+    if (c->head_size < 16 || c->head_size > 256 || c->head_size % 16)
+        return lq_fail(LQ_EINVAL, "%s: head size %d (a multiple of 16, 16 to 256)", fn, c->head_size);
+    if (c->n_kv_heads <= 0 || c->n_kv_heads > 65535 || n_heads < 0 || n_heads % c->n_kv_heads)
+        return lq_fail(LQ_EINVAL, "%s: %d query heads over %d kv heads", fn, n_heads, c->n_kv_heads);
+    if (c->n_pages < 0 || c->n_pages > INT32_MAX || b->n_seqs < 0 || b->n_rows < 0 || b->max_pages < 0 ||
+        b->max_rows < 0 || b->max_context < 0)
+        return lq_fail(LQ_EINVAL, "%s: a count is negative or too large", fn);
+    if (b->n_seqs > 65535 || b->n_rows > (1 << 24) || b->max_context > (1 << 28))
+        return lq_fail(LQ_EUNSUPPORTED, "%s: at most 65535 sequences, 2^24 rows and contexts of 2^28", fn);
+    if (b->n_seqs == 0 || b->n_rows == 0) return LQ_OK;
+    if (!c->codes || !c->scales || !b->row_start || !b->context || (b->max_pages > 0 && !b->pages))
+        return lq_fail(LQ_EINVAL, "%s: the cache's or the batch's memory is not set", fn);
+    if ((reinterpret_cast<uintptr_t>(c->codes) & 15u) || (reinterpret_cast<uintptr_t>(c->scales) & 7u) ||
+        ((reinterpret_cast<uintptr_t>(b->row_start) | reinterpret_cast<uintptr_t>(b->context) |
+          reinterpret_cast<uintptr_t>(b->pages)) & 3u))
+        return lq_fail(LQ_EINVAL, "%s: codes must be 16-byte, scales 8-byte and the batch's arrays 4-byte aligned", fn);
+    return LQ_OK;
+}
+
+}  // namespace lq
+
+using namespace lq;
+
+extern "C" {
+
+int lq_rope_table(float* table, int positions, int head_size, float base) {
+    if (!table || positions < 0 || head_size <= 0 || head_size % 2 || !(base > 0.0f))
+        return lq_fail(LQ_EINVAL, "lq_rope_table: null table, odd head size or base <= 0");
+    for (int pos = 0; pos < positions; ++pos)
+        for (int i = 0; i < head_size / 2; ++i) {
+            const float freq = 1.0f / powf(base, (2 * i) / (float)head_size);
+            const float val = pos * freq;
+            float* t = table + ((size_t)pos * (head_size / 2) + i) * 2;
+            t[0] = cosf(val);
+            t[1] = sinf(val);
+        }
+    return LQ_OK;
+}
+
+int kv_append(const PagedKV* cache, const KVBatch* batch, const KVRows* rows) {
+    if (!rows) return lq_fail(LQ_EINVAL, "kv_append: null argument");
+    int rc = check_paged(cache, batch, rows->q ? rows->n_heads : 0, rows->type, "kv_append");
+    if (rc) return rc;
+    if (rows->rope && (rows->rope_rows < 0 || (rows->rope_mode != LQ_ROPE_PAIRS && rows->rope_mode != LQ_ROPE_HALVES) ||
+                       (reinterpret_cast<uintptr_t>(rows->rope) & 15u)))
+        return lq_fail(LQ_EINVAL, "kv_append: rope mode %d, or a table that is not 16-byte aligned", rows->rope_mode);
+    if (batch->n_seqs == 0 || batch->n_rows == 0) return LQ_OK;
+    const int64_t kv = (int64_t)cache->n_kv_heads * cache->head_size;
+    if (!rows->k || !rows->v || rows->ld_k < kv || rows->ld_v < kv)
+        return lq_fail(LQ_EINVAL, "kv_append: k or v not set, or rows closer than %lld elements", (long long)kv);
+    if ((rows->k_out || rows->v_out) && rows->ld_kv_out < kv)
+        return lq_fail(LQ_EINVAL, "kv_append: ld_kv_out=%lld is less than %lld", (long long)rows->ld_kv_out, (long long)kv);
+    const int64_t qd = (int64_t)rows->n_heads * cache->head_size;
+    if (rows->q && (!rows->q_out || rows->ld_q < qd || rows->ld_q_out < qd))
+        return lq_fail(LQ_EINVAL, "kv_append: q_out not set, or rows closer than %lld elements", (long long)qd);
+    const uintptr_t size = rows->type == LQ_F32 ? 4 : 2;
+    const void* all[] = {rows->q, rows->k, rows->v, rows->q ? rows->q_out : nullptr, rows->k_out, rows->v_out};
+    for (const void* p : all)
+        if (reinterpret_cast<uintptr_t>(p) % size)
+            return lq_fail(LQ_EINVAL, "kv_append: a tensor is not aligned to its elements");
+    DevCtx* c = ctx();
+    if (!c) return lq_fail(LQ_ECUDA, "no CUDA device context (no device, or first use inside a graph capture)");
+    AppendArgs a;
+    a.c = *cache;
+    a.b = *batch;
+    a.r = *rows;
+    a.err = c->err;
+    a.jobs = batch->n_rows / cache->page_size + 2 * batch->n_seqs;
+    a.q_blocks = (int)((qd + kAppendThreads * 8 - 1) / (kAppendThreads * 8));
+    if (rows->q && rows->n_heads == 0) a.r.q = nullptr;
+    cudaError_t e = rows->type == LQ_F32   ? append_t<float>(a, stream())
+                    : rows->type == LQ_F16 ? append_t<__half>(a, stream())
+                                           : append_t<__nv_bfloat16>(a, stream());
+    return e == cudaSuccess ? LQ_OK : cuda_fail(e, "kv_append launch");
+}
+
+}  // extern "C"
