@@ -93,6 +93,50 @@ int ensure_scratch(DevCtx* c, size_t bytes) {
     return LQ_OK;
 }
 
+// the workspace of the library's stream, with room for partial_bytes
+int stream_workspace(DevCtx* c, size_t partial_bytes, int** counters, void** partials) {
+    constexpr size_t kHead = kWsCounters * sizeof(int);
+    DevCtx::Workspace* w = nullptr;
+    for (int i = 0; i < c->n_ws; ++i)
+        if (c->ws[i].stream == g_stream) w = &c->ws[i];
+    if (!w || w->bytes < kHead + partial_bytes) {
+        cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
+        if (cudaStreamIsCapturing(g_stream, &cs) == cudaSuccess && cs != cudaStreamCaptureStatusNone)
+            return lq_fail(LQ_EINVAL,
+                           "workspace of %zu bytes needed inside a graph capture: make one call of this size on this "
+                           "stream before capturing",
+                           partial_bytes);
+        if (!w && c->n_ws == c->cap_ws) {
+            const int cap = c->cap_ws ? 2 * c->cap_ws : 16;
+            void* m = realloc(c->ws, cap * sizeof(DevCtx::Workspace));
+            if (!m) return lq_fail(LQ_ENOMEM, "workspace table");
+            c->ws = static_cast<DevCtx::Workspace*>(m);
+            c->cap_ws = cap;
+        }
+        // at least twice the old size: what growth leaves behind adds up to one workspace
+        size_t bytes = kHead + partial_bytes;
+        if (w && bytes < 2 * w->bytes) bytes = 2 * w->bytes;
+        if (bytes < (size_t)1 << 22) bytes = (size_t)1 << 22;
+        void* p = nullptr;
+        cudaError_t e = cudaMalloc(&p, bytes);
+        if (e == cudaSuccess) e = cudaMemset(p, 0, kHead);
+        if (e == cudaSuccess) e = cudaStreamSynchronize(nullptr);
+        if (e != cudaSuccess) {
+            if (p) cudaFree(p);
+            return cuda_fail(e, "workspace allocation");
+        }
+        if (!w) {
+            w = &c->ws[c->n_ws++];
+            w->stream = g_stream;
+        }
+        w->p = p;
+        w->bytes = bytes;
+    }
+    *counters = static_cast<int*>(w->p);
+    *partials = static_cast<char*>(w->p) + kHead;
+    return LQ_OK;
+}
+
 int check_device_error(int* err_dev, cudaStream_t st) {
     int h = 0;
     cudaError_t e = cudaMemcpyAsync(&h, err_dev, sizeof(int), cudaMemcpyDeviceToHost, st);
@@ -193,6 +237,10 @@ int lq_sync(void) {
     DevCtx* c = ctx();
     if (!c) return lq_fail(LQ_ECUDA, "no CUDA device context (no device, or first use inside a graph capture)");
     const int a = check_device_error(c->err, g_stream);
+    if (a) {  // a call that gave up may have left its arrival counters
+        for (int i = 0; i < c->n_ws; ++i)
+            if (c->ws[i].stream == g_stream) cudaMemsetAsync(c->ws[i].p, 0, kWsCounters * sizeof(int), g_stream);
+    }
     const int b = noalloc_check_error(g_stream);  // always read (and clear) both words
     return a ? a : b;
 }

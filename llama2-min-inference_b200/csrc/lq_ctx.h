@@ -36,12 +36,25 @@ struct DevCtx {
         uint64_t used;
     };
     std::vector<CallGraph> graphs;
+    // workspaces of the token-scaled products and the paged attention, one per
+    // stream: kWsCounters arrival counters (zero between launches), then
+    // partial results.  One that grows leaves the old one allocated: captured
+    // graphs may hold it.
+    struct Workspace {
+        cudaStream_t stream;
+        void* p;
+        size_t bytes;
+    };
+    Workspace* ws = nullptr;
+    int n_ws = 0, cap_ws = 0;
     cudaStream_t capture = nullptr;  // private stream the graphs are captured on
     uint64_t tick = 0;
 };
 
 DevCtx* ctx();  // context of the current device (created on first use)
 int ensure_scratch(DevCtx* c, size_t bytes);
+constexpr int kWsCounters = 16384;
+int stream_workspace(DevCtx* c, size_t partial_bytes, int** counters, void** partials);
 int cuda_fail(cudaError_t e, const char* what);
 int check_device_error(int* err_dev, cudaStream_t st);
 int noalloc_check_error(cudaStream_t st);  // matmul_f32_noalloc's error word (noalloc.cu)

@@ -33,6 +33,10 @@ cudaError_t quantize_act_launch(const float* x, int64_t rows, int64_t n, int gs,
 size_t attention_smem_bytes(int head_size, int kv_mul);
 // the attention kernel's K-cache map over `rows` cached positions of head_size floats
 bool kv_tensor_map(CUtensorMap* m, const float* kcache, int head_size, uint64_t rows);
+// 2-D map over a row-major byte matrix: `rows` rows of `inner` bytes, `pitch`
+// apart (a multiple of 16), copied as boxes; what lies outside reads as zeros
+bool byte_map_2d(CUtensorMap* m, const void* base, uint64_t inner, uint64_t rows, uint64_t pitch, uint32_t box_inner,
+                 uint32_t box_rows, bool swizzle128);
 cudaError_t attention_launch(const AttnArgs& a, int batch, cudaStream_t st, bool pdl);
 cudaError_t argmax_launch(const float* logits, int n, int batch, int stride, int* out, cudaStream_t st,
                           bool pdl, uint64_t* kt = nullptr);

@@ -47,6 +47,7 @@
 #include "lq_epilogue.cuh"
 #include "lq_kernels.h"
 #include "lq_ops.h"
+#include "lq_tc.cuh"
 
 namespace lq {
 
@@ -64,13 +65,6 @@ constexpr int kEpiWarps = 16;
 constexpr int kEpiWarp0 = kConvWarp0 + kConvWarps;
 constexpr int kXsStages = 8;     // activation-scale ring: one entry (the stage's groups) per stage
 
-enum : int {
-    DEV_TIMEOUT_CONV = 0x111,   // MMA waited too long for a converted stage
-    DEV_TIMEOUT_TFULL = 0x112,  // epilogue waited too long for a group's dots
-    DEV_TIMEOUT_TEMPTY = 0x113, // MMA waited too long for a free TMEM buffer
-    DEV_TIMEOUT_MMA = 0x114,    // final MMA completion wait gave up
-};
-
 struct QgemmArgs {
     CUtensorMap wmap[kMaxSegs][2];  // weight tiles (second: the paired w3 tensor)
     CUtensorMap xmap;               // activation [rows][cols] int8, boxes of npad rows (zero fill)
@@ -83,110 +77,6 @@ struct QgemmArgs {
     int tiles, kst, stages;         // tiles, K stages per row, smem ring depth
 };
 
-// ---- PTX wrappers (public PTX ISA: tcgen05, cp.async.bulk.tensor) --------
-
-__device__ __forceinline__ uint64_t l2_evict_last_policy() {
-    uint64_t p;
-    asm volatile("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(p));
-    return p;
-}
-
-__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-
-// Shared-memory matrix descriptor: K-major, 128-byte swizzle, 8-row core
-// groups 1024 bytes apart (stride byte offset), version 1 (sm_100).
-__device__ __forceinline__ uint64_t smem_desc_sw128(uint32_t addr) {
-    return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) |
-           ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
-}
-
-__device__ __forceinline__ void mma_i8(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
-                                       uint32_t accumulate) {
-    asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-        " tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n}\n" ::"r"(d_tmem),
-        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
-        : "memory");
-}
-
-__device__ __forceinline__ void mma_commit(uint64_t* bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
-                     smem_addr(bar))
-                 : "memory");
-}
-
-template <int NC>
-__device__ __forceinline__ void tmem_ld(uint32_t taddr, int (&d)[NC]);
-
-template <>
-__device__ __forceinline__ void tmem_ld<4>(uint32_t taddr, int (&d)[4]) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
-                 : "r"(taddr));
-}
-
-template <>
-__device__ __forceinline__ void tmem_ld<8>(uint32_t taddr, int (&d)[8]) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-                 : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3]), "=r"(d[4]), "=r"(d[5]), "=r"(d[6]),
-                   "=r"(d[7])
-                 : "r"(taddr));
-}
-
-template <>
-__device__ __forceinline__ void tmem_ld<16>(uint32_t taddr, int (&d)[16]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-        : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3]), "=r"(d[4]), "=r"(d[5]), "=r"(d[6]), "=r"(d[7]),
-          "=r"(d[8]), "=r"(d[9]), "=r"(d[10]), "=r"(d[11]), "=r"(d[12]), "=r"(d[13]), "=r"(d[14]), "=r"(d[15])
-        : "r"(taddr));
-}
-
-template <>
-__device__ __forceinline__ void tmem_ld<32>(uint32_t taddr, int (&d)[32]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-        : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3]), "=r"(d[4]), "=r"(d[5]), "=r"(d[6]), "=r"(d[7]),
-          "=r"(d[8]), "=r"(d[9]), "=r"(d[10]), "=r"(d[11]), "=r"(d[12]), "=r"(d[13]), "=r"(d[14]), "=r"(d[15]),
-          "=r"(d[16]), "=r"(d[17]), "=r"(d[18]), "=r"(d[19]), "=r"(d[20]), "=r"(d[21]), "=r"(d[22]), "=r"(d[23]),
-          "=r"(d[24]), "=r"(d[25]), "=r"(d[26]), "=r"(d[27]), "=r"(d[28]), "=r"(d[29]), "=r"(d[30]), "=r"(d[31])
-        : "r"(taddr));
-}
-
-__device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-
-// packed fp32x2 arithmetic (sm_100): two IEEE round-to-nearest results
-__device__ __forceinline__ uint64_t f2_pack(float lo, float hi) {
-    return (uint64_t)__float_as_uint(lo) | ((uint64_t)__float_as_uint(hi) << 32);
-}
-__device__ __forceinline__ float f2_lo(uint64_t v) { return __uint_as_float((uint32_t)v); }
-__device__ __forceinline__ float f2_hi(uint64_t v) { return __uint_as_float((uint32_t)(v >> 32)); }
-__device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
-    uint64_t d;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-    return d;
-}
-__device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
-    uint64_t d;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-    return d;
-}
-__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-    return d;
-}
-
-// ---- stream-K partition ---------------------------------------------------
-
-__device__ __host__ __forceinline__ int64_t sk_start(int i, int64_t W, int G) { return (int64_t)i * W / G; }
-// the CTA whose stage range holds stage s
-__device__ __host__ __forceinline__ int sk_owner(int64_t s, int64_t W, int G) {
-    return (int)(((s + 1) * G + W - 1) / W - 1);
-}
-
 struct Bars {
     uint64_t full[16], conv[16], empty[16], tfull[kMaxBuf], tempty[kMaxBuf], done[kMmaWarps];
     uint64_t xfull[kXsStages], xempty[kXsStages];
@@ -194,36 +84,6 @@ struct Bars {
     int abort_flag;
     int last_flag;
 };
-
-// wait that returns at once when the CTA has given up; records `code` on timeout
-__device__ __forceinline__ bool mbar_test_wait(uint64_t* bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n"
-        " selp.u32 %0, 1, 0, p;\n}\n"
-        : "=r"(ok)
-        : "r"(smem_addr(bar)), "r"(parity)
-        : "memory");
-    return ok != 0;
-}
-
-__device__ __forceinline__ bool qwait(uint64_t* bar, uint32_t parity, int* err, int code, volatile int* abort_flag) {
-    if (mbar_test_wait(bar, parity)) return true;  // already complete: no blocking probe
-    if (*abort_flag) return false;
-    if (mbar_try_wait(bar, parity)) return true;
-    const uint64_t t0 = globaltimer();
-    for (uint32_t i = 1;; ++i) {
-        if (mbar_try_wait(bar, parity)) return true;
-        if ((i & 63u) == 0) {
-            if (*abort_flag) return false;
-            if (globaltimer() - t0 > kWaitLimitNs) {
-                set_err(err, code);
-                *abort_flag = 1;
-                return false;
-            }
-        }
-    }
-}
 
 template <int KIND, int N, int MULT>
 struct Layout {
@@ -659,6 +519,16 @@ bool make_map(CUtensorMap* m, const void* base, uint64_t inner, uint64_t rows, u
                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS;
 }
+
+}  // namespace
+
+bool byte_map_2d(CUtensorMap* m, const void* base, uint64_t inner, uint64_t rows, uint64_t pitch, uint32_t box_inner,
+                 uint32_t box_rows, bool swizzle128) {
+    return get_encoder() && make_map(m, base, inner, rows, pitch, box_inner, box_rows,
+                                     swizzle128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE);
+}
+
+namespace {
 
 int npad_for(int rows) { return rows <= 16 ? 16 : (rows <= 32 ? 32 : 64); }
 
