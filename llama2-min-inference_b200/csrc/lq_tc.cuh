@@ -44,6 +44,15 @@ __device__ __forceinline__ void mma_commit(uint64_t* bar) {
                  : "memory");
 }
 
+// One lane of the (converged) warp.  Single-thread instructions are issued
+// under this rather than under lane == 0: a loop of wait, four MMAs and commit
+// takes 361 cycles so and 500 with a divergent branch (128 x 128 x 32).
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(p));
+    return p != 0;
+}
+
 // the forms below with CTAS = 2 are a pair's (cta_group::2): CTA 0 of the
 // cluster issues MMAs and commits for both
 template <int CTAS>
@@ -73,25 +82,26 @@ __device__ __forceinline__ void mma_commit_n(uint64_t* bar) {
             : "memory");
 }
 
-template <int CTAS>
-__device__ __forceinline__ void tmem_alloc(uint32_t* base, int cols) {
+// COLS columns of tensor memory; a constant, so that the compiler records how much the kernel holds
+template <int CTAS, int COLS>
+__device__ __forceinline__ void tmem_alloc(uint32_t* base) {
     if constexpr (CTAS == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(base)), "r"(cols)
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(base)), "n"(COLS)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     } else {
-        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(base)), "r"(cols)
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(base)), "n"(COLS)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
     }
 }
 
-template <int CTAS>
-__device__ __forceinline__ void tmem_free(uint32_t tmem, int cols) {
+template <int CTAS, int COLS>
+__device__ __forceinline__ void tmem_free(uint32_t tmem) {
     if constexpr (CTAS == 1)
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cols) : "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(COLS) : "memory");
     else
-        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cols) : "memory");
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(COLS) : "memory");
 }
 
 __device__ __forceinline__ void cluster_sync() {

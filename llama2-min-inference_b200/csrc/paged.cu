@@ -168,7 +168,7 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
         mv = max(mv, wv[w]);
     }
     const float sk = append_scale(mk, old_k), sv = append_scale(mv, old_v);
-    const bool bad_k = sk != sk, bad_v = sv != sv;
+    const Quant8 qk(sk), qv(sv);
     if (tid == 0) {
         a.c.scales[cell * 2] = sk;
         a.c.scales[cell * 2 + 1] = sv;
@@ -176,13 +176,13 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
     // earlier tokens at the grown scale (a NaN scale leaves nothing to keep)
     const bool grow_k = off > 0 && sk != old_k, grow_v = off > 0 && sv != old_v;
     auto again = [](uint32_t word, float ratio) {
-        int o[4];
+        uint32_t o[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = __float2int_rn((float)(int8_t)(word >> (8 * e)) * ratio);
+        for (int e = 0; e < 4; ++e) o[e] = (uint32_t)__float2int_rn((float)code_of(word >> (8 * e)) * ratio);
         return pack8(o[0], o[1], o[2], o[3]);
     };
     if (grow_k) {
-        const float ratio = bad_k ? 0.0f : old_k / sk;
+        const float ratio = qk.bad ? 0.0f : old_k / sk;
         for (int i = tid; i < off * (hs / 4); i += kAppendThreads) {
             const int t = i % off, w = i / off;  // word w (4 dims) of token t
             uint32_t* p = reinterpret_cast<uint32_t*>(kc + ((int64_t)(w / 4) * P + t) * 16) + (w & 3);
@@ -194,19 +194,17 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
         const int t = i / (hs / 4), d = 4 * (i - t * (hs / 4));
         float k[4];
         rotated4<T, VEC>(kr + t * a.r.ld_k, tab0 ? tab0 + (int64_t)t * hs : nullptr, hs, a.r.rope_mode, d, k);
-        int c[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) c[e] = bad_k ? 0 : quant8(k[e], sk);
-        *reinterpret_cast<uint32_t*>(kc + ((int64_t)(d / 16) * P + off + t) * 16 + d % 16) = pack8(c[0], c[1], c[2], c[3]);
+        const uint32_t c = qk(k[0], k[1], k[2], k[3]);
+        *reinterpret_cast<uint32_t*>(kc + ((int64_t)(d / 16) * P + off + t) * 16 + d % 16) = c;
         if (a.r.k_out) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) k[e] = (float)c[e] * sk;
+            for (int e = 0; e < 4; ++e) k[e] = (float)code_of(c >> (8 * e)) * sk;
             store_n<4, VEC>(static_cast<T*>(a.r.k_out) + (int64_t)(row0 + t) * a.r.ld_kv_out + (int64_t)h * hs + d, k);
         }
     }
     // values: a word is 4 tokens of a dim; the words that hold tokens up to the
     // last new one, earlier tokens in them kept or rescaled, later bytes kept
-    const float ratio_v = bad_v ? 0.0f : old_v / sv;
+    const float ratio_v = qv.bad ? 0.0f : old_v / sv;
     const int w0 = grow_v ? 0 : off / 4, w1 = (off + nt + 3) / 4;
     for (int i = tid; i < (w1 - w0) * hs; i += kAppendThreads) {
         const int w = w0 + i / hs, d = i % hs;
@@ -218,16 +216,21 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
             const uint32_t mask = keep >= 4 ? 0xFFFFFFFFu : (1u << (8 * keep)) - 1u;
             word = (again(word, ratio_v) & mask) | (word & ~mask);
         }
+        float x[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int t = 4 * w + e - off;
+            x[e] = t >= 0 && t < nt ? to_f32(vr[t * a.r.ld_v + d]) : 0.0f;
+        }
+        const uint32_t c = qv(x[0], x[1], x[2], x[3]);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const int t = 4 * w + e - off;
             if (t < 0 || t >= nt) continue;
-            const float x = to_f32(vr[t * a.r.ld_v + d]);
-            const int c = bad_v ? 0 : quant8(x, sv);
-            word = (word & ~(0xFFu << (8 * e))) | ((uint32_t)(c & 255) << (8 * e));
+            word = (word & ~(0xFFu << (8 * e))) | (c & (0xFFu << (8 * e)));
             if (a.r.v_out)
                 static_cast<T*>(a.r.v_out)[(int64_t)(row0 + t) * a.r.ld_kv_out + (int64_t)h * hs + d] =
-                    from_f32<T>((float)c * sv);
+                    from_f32<T>((float)code_of(c >> (8 * e)) * sv);
         }
         *p = word;
     }

@@ -11,90 +11,110 @@ namespace {
 
 // ---------------------------------------------------------------------------
 // quantize_rows: s = max|x| / 127 (0 -> 1e-8), q = rint(x / s), one CTA per row.
-// The row is read once: each thread keeps up to kKeep quads of it between the
-// maximum and the rounding; longer rows are read again (from L2).
+// Bound by memory (each element read once, one byte written).  A thread keeps
+// up to KEEP 16-byte pieces of the row, as they lie in memory, in registers
+// between the maximum and the rounding, all loaded at once; rows longer than
+// that are read again.
 
-constexpr int kQuantThreads = 256;
-constexpr int kKeep = 16;  // quads per thread: rows of up to 16384 stay in registers
-
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(kQuantThreads) quantize_rows_kernel(const T* __restrict__ x, int64_t ld, int n,
-                                                                      int8_t* __restrict__ q, int pitch,
-                                                                      float* __restrict__ s) {
+template <typename T, bool VEC, int KEEP>
+__global__ void __maxnreg__(40) quantize_rows_kernel(const T* __restrict__ x, int64_t ld, int n, int8_t* __restrict__ q, int pitch,
+                                     float* __restrict__ s) {
+    constexpr int E = 16 / sizeof(T);  // elements of a piece; their codes are E bytes
+    constexpr int W = E / 4;           // elements of a word
     pdl_trigger();
     pdl_wait();
     const T* xr = x + (int64_t)blockIdx.x * ld;
-    const int quads = pitch / 4;
-    float keep[kKeep][4];
+    const int pieces = pitch / E, step = blockDim.x;
+    uint4 keep[KEEP];
     uint32_t m = 0;
-    auto load = [&](int i, float (&v)[4]) {
-        if (4 * i + 4 <= n) {
-            load_n<4, VEC>(xr + 4 * i, v);
-        } else {
+    auto load = [&](int i) {
+        if (VEC && E * i + E <= n) return *reinterpret_cast<const uint4*>(xr + E * i);
+        uint32_t w[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = 4 * i + e < n ? to_f32(xr[4 * i + e]) : 0.0f;
+        for (int k = 0; k < 4; ++k) {
+            float v[W];
+#pragma unroll
+            for (int e = 0; e < W; ++e) v[e] = E * i + W * k + e < n ? to_f32(xr[E * i + W * k + e]) : 0.0f;
+            w[k] = pack_word<T>(v);
+        }
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    };
+    auto peak = [&](uint4 p) {
+        const uint32_t w[4] = {p.x, p.y, p.z, p.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            float v[W];
+            unpack_word<T>(w[k], v);
+#pragma unroll
+            for (int e = 0; e < W; ++e) m = max(m, abs_bits(v[e]));
         }
     };
 #pragma unroll
-    for (int j = 0; j < kKeep; ++j) {
-        const int i = threadIdx.x + j * kQuantThreads;
-        if (i < quads) load(i, keep[j]);
+    for (int j = 0; j < KEEP; ++j) {
+        const int i = threadIdx.x + j * step;
+        if (i < pieces) keep[j] = load(i);
     }
 #pragma unroll
-    for (int j = 0; j < kKeep; ++j) {
-        if (threadIdx.x + j * kQuantThreads < quads) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) m = max(m, abs_bits(keep[j][e]));
-        }
-    }
-    for (int i = threadIdx.x + kKeep * kQuantThreads; i < quads; i += kQuantThreads) {
-        float v[4];
-        load(i, v);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) m = max(m, abs_bits(v[e]));
-    }
-    __shared__ uint32_t wm[kQuantThreads / 32];
+    for (int j = 0; j < KEEP; ++j)
+        if (threadIdx.x + j * step < pieces) peak(keep[j]);
+    for (int i = threadIdx.x + KEEP * step; i < pieces; i += step) peak(load(i));
+    __shared__ uint32_t wm[32];
     m = __reduce_max_sync(0xffffffffu, m);
     if ((threadIdx.x & 31) == 0) wm[threadIdx.x >> 5] = m;
     __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kQuantThreads / 32; ++w) m = max(m, wm[w]);
-    const bool bad = m >= kInfBits;  // a NaN or an infinity: scale NaN, codes 0
+    m = __reduce_max_sync(0xffffffffu, (threadIdx.x & 31) < (step >> 5) ? wm[threadIdx.x & 31] : 0u);
     float sc = __uint_as_float(m) / 127.0f;
     if (sc == 0.0f) sc = 1e-8f;
-    uint32_t* qr = reinterpret_cast<uint32_t*>(q + (int64_t)blockIdx.x * pitch);
-    auto store = [&](int i, const float (&v)[4]) {
-        qr[i] = bad ? 0u : pack8(quant8(v[0], sc), quant8(v[1], sc), quant8(v[2], sc), quant8(v[3], sc));
+    if (m >= kInfBits) sc = __uint_as_float(0x7FC00000u);  // a NaN or an infinity: scale NaN, codes 0
+    const Quant8 code(sc);
+    int8_t* qr = q + (int64_t)blockIdx.x * pitch;
+    auto store = [&](int i, uint4 p) {
+        float v[E];
+        unpack_word<T>(p.x, v);
+        unpack_word<T>(p.y, v + W);
+        unpack_word<T>(p.z, v + 2 * W);
+        unpack_word<T>(p.w, v + 3 * W);
+        if constexpr (E == 4)
+            reinterpret_cast<uint32_t*>(qr)[i] = code(v[0], v[1], v[2], v[3]);
+        else
+            reinterpret_cast<uint2*>(qr)[i] = make_uint2(code(v[0], v[1], v[2], v[3]), code(v[4], v[5], v[6], v[7]));
     };
 #pragma unroll
-    for (int j = 0; j < kKeep; ++j) {
-        const int i = threadIdx.x + j * kQuantThreads;
-        if (i < quads) store(i, keep[j]);
+    for (int j = 0; j < KEEP; ++j) {
+        const int i = threadIdx.x + j * step;
+        if (i < pieces) store(i, keep[j]);
     }
-    for (int i = threadIdx.x + kKeep * kQuantThreads; i < quads; i += kQuantThreads) {
-        float v[4];
-        load(i, v);
-        store(i, v);
-    }
-    if (threadIdx.x == 0) s[blockIdx.x] = bad ? __uint_as_float(0x7FC00000u) : sc;
+    for (int i = threadIdx.x + KEEP * step; i < pieces; i += step) store(i, load(i));
+    if (threadIdx.x == 0) s[blockIdx.x] = sc;
 }
 
 template <typename T>
-cudaError_t quantize_rows_t(const void* x, int64_t ld, int64_t rows, int n, int8_t* q, float* s, cudaStream_t st) {
+cudaError_t quantize_rows_t(const void* x, int64_t ld, int64_t rows, int n, int8_t* q, float* s, int sms,
+                            cudaStream_t st) {
+    constexpr int E = 16 / sizeof(T);
     const T* xt = static_cast<const T*>(x);
-    const int pitch = LQ_ROW8_PITCH(n);
-    const bool vec = reinterpret_cast<uintptr_t>(x) % (4 * sizeof(T)) == 0 && ld % 4 == 0;
+    const int pitch = LQ_ROW8_PITCH(n), pieces = pitch / E;
+    const bool vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && ld % E == 0;
+    // Few rows: the time of one, so two pieces a thread.  Many: four, so that
+    // more rows are in flight on an SM.
+    const int want = rows <= 4 * sms ? 2 : 4;
+    int threads = 64;
+    while (threads < 1024 && threads * want < pieces) threads *= 2;
+    const int keep = (pieces + threads - 1) / threads;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)rows);
-    cfg.blockDim = dim3(kQuantThreads);
+    cfg.blockDim = dim3(threads);
     cfg.stream = st;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return vec ? cudaLaunchKernelEx(&cfg, quantize_rows_kernel<T, true>, xt, ld, n, q, pitch, s)
-               : cudaLaunchKernelEx(&cfg, quantize_rows_kernel<T, false>, xt, ld, n, q, pitch, s);
+    auto kern = !vec      ? quantize_rows_kernel<T, false, 4>
+                : keep <= 1 ? quantize_rows_kernel<T, true, 1>
+                : keep <= 2 ? quantize_rows_kernel<T, true, 2>
+                            : quantize_rows_kernel<T, true, 4>;
+    return cudaLaunchKernelEx(&cfg, kern, xt, ld, n, q, pitch, s);
 }
 
 // ---------------------------------------------------------------------------
@@ -104,17 +124,26 @@ cudaError_t quantize_rows_t(const void* x, int64_t ld, int64_t rows, int n, int8
 // the weights then stream at memory speed, and a thread of the epilogue holds
 // one channel of all tokens, so that a warp's store is 32 neighbouring channels.
 //
-// One CTA per SM: warp 0 issues the TMA copies (128-byte K stages, 128-byte
-// swizzle; bytes past the row or the tensor read as zeros), warp 1 the MMAs,
-// warps 2-5 turn a finished accumulator into outputs while the MMAs fill the
-// other.  Tiles that fill whole rounds of the grid are done by one CTA each;
-// the stages of the remaining ones are cut into equal runs over all CTAs
-// (stream-K).  A tile cut so leaves int32 partials, which the last of its CTAs
-// to arrive adds: integer sums, the same whatever the order.
+// One persistent CTA (or half a pair) per SM: warps 0 and 6 issue the TMA
+// copies (128-byte swizzle; bytes past the row or the tensor read as zeros), warp 1 the MMAs, warps 2-5 turn a finished accumulator into
+// outputs while the MMAs fill the other.  A tile may hold fewer than 128
+// channels, so that the tiles fill whole rounds of the grid: the copies, which
+// bound every size here (HBM for few tokens, L2 to SM for many), then are only
+// those of its channels, and the MMA's other rows, which compute with whatever
+// follows in shared memory, are not read out.
 
-constexpr int kRowsThreads = 192;
-constexpr int kStageBytes = 128;  // K bytes per stage
+constexpr int kRowsThreads = 224;
 constexpr int kMaxStages = 12;
+
+// K bytes per stage, in 128-byte halves (the swizzle's width): two halves for
+// up to 64 tokens, whose MMAs are short (64 cycles each, 128 x N x 32 for any
+// N up to 128), so that waiting and committing once per stage (about 250
+// cycles of the issuing thread) is spread over eight of them; one beyond, for
+// a deeper ring.
+template <int N>
+constexpr int rows_halves() {
+    return N <= 64 ? 2 : 1;
+}
 
 struct RowsArgs {
     CUtensorMap wmap, xmap;
@@ -122,59 +151,23 @@ struct RowsArgs {
     void* y;
     int64_t ld;
     int rows, d, type;
-    int kst;                // K stages
-    int ttiles;             // tiles along the tokens
-    int whole, shared;      // tiles done by one CTA group each; tiles cut by stages
-    int sk_grid;            // CTA groups that share them
-    int stages;
-    int early;              // the weights may be read before the previous kernel ends
-    int *part, *cnt, *err;
+    int pitch, kst;  // bytes of a row, K stages
+    int ttiles;  // tiles along the tokens
+    int tiles;
+    int m;       // channels per tile and CTA: a multiple of 8, at most 128
+    int xbox;    // tokens of an activation copy: no more than there are (an MMA
+                 // column past them holds anything and is not read out)
+    int stages, rot;
+    int* err;
 };
 
 struct RowsBars {
     uint64_t full[kMaxStages], empty[kMaxStages], tfull[2], tempty[2], done;
     uint32_t tmem_base;
-    int abort_flag, last_flag;
+    int abort_flag;
 };
 
-// the (tile, K range) pieces of one CTA group: first its run of shared stages, then whole tiles
-struct Pieces {
-    int64_t s, s1;
-    int t, whole, groups, kst;
-    __device__ Pieces(const RowsArgs& a, int group, int groups_) {
-        const int64_t w = (int64_t)a.shared * a.kst;
-        s = group < a.sk_grid ? sk_start(group, w, a.sk_grid) : 0;
-        s1 = group < a.sk_grid ? sk_start(group + 1, w, a.sk_grid) : 0;
-        t = group;
-        whole = a.whole;
-        groups = groups_;
-        kst = a.kst;
-    }
-    __device__ bool next(int& tile, int& k0, int& k1) {
-        if (s < s1) {
-            const int q = (int)(s / kst);
-            tile = whole + q;
-            k0 = (int)(s - (int64_t)q * kst);
-            k1 = (int)min((int64_t)kst, k0 + (s1 - s));
-            s += k1 - k0;
-            return true;
-        }
-        if (t < whole) {
-            tile = t;
-            k0 = 0;
-            k1 = kst;
-            t += groups;
-            return true;
-        }
-        return false;
-    }
-};
-
-template <int N, int CTAS>
-constexpr int rows_stage_bytes() {
-    return 128 * kStageBytes + N / CTAS * kStageBytes;
-}
-
+// one channel of CH tokens: fl(fl(sum) * fl(sx * sw)), rounded to the type
 template <int CH, typename T>
 __device__ __forceinline__ void store_columns(T* y, int64_t ld, const int (&acc)[CH], float xsv, float wsv, int n,
                                               bool ok) {
@@ -185,22 +178,48 @@ __device__ __forceinline__ void store_columns(T* y, int64_t ld, const int (&acc)
     }
 }
 
+template <int CH>
+__device__ __forceinline__ void store_columns(const RowsArgs& a, int tok, int ch, const int (&v)[CH], int lane) {
+    const int n = min(CH, a.rows - tok);
+    const float xsv = lane < n ? __ldg(a.xs + tok + lane) : 0.0f;
+    const float wsv = ch < a.d ? __ldg(a.ws + ch) : 0.0f;
+    const int64_t at = (int64_t)tok * a.ld + ch;
+    if (a.type == LQ_F32)
+        store_columns<CH>(static_cast<float*>(a.y) + at, a.ld, v, xsv, wsv, n, ch < a.d);
+    else if (a.type == LQ_F16)
+        store_columns<CH>(static_cast<__half*>(a.y) + at, a.ld, v, xsv, wsv, n, ch < a.d);
+    else
+        store_columns<CH>(static_cast<__nv_bfloat16*>(a.y) + at, a.ld, v, xsv, wsv, n, ch < a.d);
+}
+
+// s32 += s8 x s8, both K-major
+template <int N, int CTAS>
+constexpr uint32_t rows_idesc() {
+    return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(8 * CTAS) << 24);
+}
+
 template <int N, int CTAS>
 __global__ void __launch_bounds__(kRowsThreads, 1) matmul_rows_kernel(const __grid_constant__ RowsArgs a) {
-    constexpr int kA = 128 * kStageBytes, kB = N / CTAS * kStageBytes, kStage = kA + kB;
-    constexpr int kCols = 2 * N < 32 ? 32 : 2 * N;
+    constexpr int kCols = 2 * N;
     constexpr int CH = N < 32 ? N : 32;
+    constexpr int kHalves = rows_halves<N>(), kB = N / CTAS * 128;
+    const int kA = a.m * 128, kHalf = kA + kB, kStage = kHalves * kHalf;
     extern __shared__ __align__(1024) unsigned char raw[];
     unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
-    RowsBars* bars = reinterpret_cast<RowsBars*>(sm + (size_t)a.stages * kStage);
+    RowsBars* bars = reinterpret_cast<RowsBars*>(sm);
+    sm += 1024;
     volatile int* abort_flag = &bars->abort_flag;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int group = blockIdx.x / CTAS, groups = gridDim.x / CTAS, rank = CTAS == 2 ? blockIdx.x & 1 : 0;
     const int S = a.stages;
+    // Where the weights of a CTA are its own, the CTAs begin at different K
+    // stages (an integer sum has no order): together they would all ask L2
+    // for the same few lines of the activations.
+    const int k0 = a.rot ? (int)((int64_t)group * a.kst / groups) : 0;
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < S; ++i) {
-            mbar_init(&bars->full[i], 1);
+            mbar_init(&bars->full[i], 2);  // both producers
             mbar_init(&bars->empty[i], 1);
         }
         for (int i = 0; i < 2; ++i) {
@@ -211,172 +230,126 @@ __global__ void __launch_bounds__(kRowsThreads, 1) matmul_rows_kernel(const __gr
         bars->abort_flag = 0;
         fence_mbar_init();
     }
-    if (warp == 1) tmem_alloc<CTAS>(&bars->tmem_base, kCols);
+    if (warp == 1) tmem_alloc<CTAS, kCols>(&bars->tmem_base);
     tc_fence_before();
     __syncthreads();
     if (CTAS == 2) cluster_sync();
     tc_fence_after();
     const uint32_t tmem = bars->tmem_base;
     pdl_trigger();
-    if (!(warp == 0 && a.early)) pdl_wait();
+    if (threadIdx.x == 0) {
+        prefetch_map(&a.wmap);
+        prefetch_map(&a.xmap);
+        if (group < a.tiles)  // no read: what the previous kernel still writes is seen by the copies below
+            for (int i = 0; i < S * kHalves && 128 * i < a.pitch; ++i)
+                tma_prefetch_2d(&a.wmap, (k0 * kHalves * 128 + i * 128) % (a.kst * kHalves * 128), (group / a.ttiles * CTAS + rank) * a.m);
+    }
+    pdl_wait();
 
-    if (warp == 0) {
-        if (lane == 0) {
-            const uint64_t pw = l2_evict_first_policy(), px = l2_evict_last_policy();
-            const uint64_t pol_w = a.ttiles > 1 ? px : pw;  // weights that several token tiles read stay in L2
-            Pieces p(a, group, groups);
-            int tile, k0, k1, slot = 0, issued = 0;
-            uint32_t ph = 0;
-            bool ok = true;
-            uint64_t* full0 = bars->full;
-            const uint32_t lead = CTAS == 2 ? cluster_addr(full0, 0) : smem_addr(full0);
-            if (CTAS == 1 && a.early) {
-                // the ring's first weight tiles, then the previous kernel's end, then the activations
-                Pieces e(a, group, groups);
-                int n = 0;
-                while (n < S && e.next(tile, k0, k1))
-                    for (int k = k0; k < k1 && n < S; ++k, ++n) {
-                        mbar_arrive_expect_tx(&bars->full[n], kStage);
-                        tma_load_2d(sm + n * kStage, &a.wmap, k * kStageBytes, tile / a.ttiles * 128, &bars->full[n], pol_w);
-                    }
-                pdl_wait();
-            }
-            while (ok && p.next(tile, k0, k1)) {
-                const int ch = tile / a.ttiles * (128 * CTAS) + rank * 128, tok = tile % a.ttiles * N + rank * (N / CTAS);
-                for (int k = k0; k < k1; ++k) {
-                    if (!qwait(&bars->empty[slot], ph ^ 1u, a.err, DEV_TIMEOUT_EMPTY, abort_flag)) {
-                        ok = false;
-                        break;
-                    }
-                    unsigned char* at = sm + slot * kStage;
-                    if (CTAS == 1) {
-                        if (!(a.early && issued < S)) {
-                            mbar_arrive_expect_tx(&bars->full[slot], kStage);
-                            tma_load_2d(at, &a.wmap, k * kStageBytes, ch, &bars->full[slot], pol_w);
+    if (warp == 0 || warp == 6) {
+        // warp 0 copies weights, warp 6 activations
+        const CUtensorMap* map = warp == 0 ? &a.wmap : &a.xmap;
+        const int bytes = warp == 0 ? kA : a.xbox * 128, off = warp == 0 ? 0 : kA;
+        const uint64_t pol = l2_normal_policy();
+        const uint32_t lead = CTAS == 2 ? cluster_addr(bars->full, 0) : 0;
+        int slot = 0, issued = 0;
+        uint32_t ph = 0;
+        bool ok = true;
+        for (int tile = group; ok && tile < a.tiles; tile += groups) {
+            const int y = warp == 0 ? (tile / a.ttiles * CTAS + rank) * a.m : tile % a.ttiles * N + rank * (N / CTAS);
+            for (int i = 0; i < a.kst; ++i) {
+                const int k = i + k0 < a.kst ? i + k0 : i + k0 - a.kst;
+                ok = __all_sync(0xffffffffu, qwait(&bars->empty[slot], ph ^ 1u, a.err, DEV_TIMEOUT_EMPTY, abort_flag));
+                if (!ok) break;
+                if (elect_one()) {
+                    const int halves = kHalves == 2 && k * 256 + 128 < a.pitch ? 2 : 1;
+                    // a pair's copies are all counted on CTA 0's barrier
+                    if (rank == 0) mbar_arrive_expect_tx(&bars->full[slot], CTAS * halves * bytes);
+#pragma unroll
+                    for (int j = 0; j < kHalves; ++j) {
+                        unsigned char* at = sm + slot * kStage + j * kHalf + off;
+                        const int x = (k * kHalves + j) * 128;
+                        if (j < halves) {
+                            if (CTAS == 1)
+                                tma_load_2d(at, map, x, y, &bars->full[slot], pol);
+                            else
+                                tma_load_2d_pair(at, map, x, y, lead + slot * 8, pol);
                         }
-                        tma_load_2d(at + kA, &a.xmap, k * kStageBytes, tok, &bars->full[slot], px);
-                    } else {
-                        if (rank == 0) mbar_arrive_expect_tx(&bars->full[slot], 2 * kStage);
-                        tma_load_2d_pair(at, &a.wmap, k * kStageBytes, ch, lead + slot * 8, pol_w);
-                        tma_load_2d_pair(at + kA, &a.xmap, k * kStageBytes, tok, lead + slot * 8, px);
-                    }
-                    ++issued;
-                    if (++slot == S) {
-                        slot = 0;
-                        ph ^= 1u;
                     }
                 }
-            }
-            if (*abort_flag && rank == 0) {  // confirm the copies still in flight
-                for (int j = max(0, issued - S); j < issued; ++j)
-                    if (!mbar_wait(&bars->full[j % S], (uint32_t)((j / S) & 1), a.err, DEV_TIMEOUT_DRAIN)) break;
+                __syncwarp();
+                ++issued;
+                if (++slot == S) {
+                    slot = 0;
+                    ph ^= 1u;
+                }
             }
         }
+        if (*abort_flag && rank == 0 && warp == 0)  // confirm the copies still in flight
+            for (int j = max(0, issued - S); j < issued; ++j)
+                if (!__all_sync(0xffffffffu, mbar_wait(&bars->full[j % S], (uint32_t)((j / S) & 1), a.err, DEV_TIMEOUT_DRAIN)))
+                    break;
+        __syncwarp();
     } else if (warp == 1) {
-        if (lane == 0 && rank == 0) {
-            // s32 += s8 x s8, both K-major
-            const uint32_t idesc =
-                (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(8 * CTAS) << 24);
-            Pieces p(a, group, groups);
-            int tile, k0, k1, slot = 0, buf = 0;
+        if (rank == 0) {
+            const uint64_t desc0 = smem_desc_sw128(smem_addr(sm));
+            constexpr uint32_t idesc = rows_idesc<N, CTAS>();
+            int slot = 0, buf = 0;
             uint32_t ph = 0, bph = 0;
-            bool ok = true, issued = false;
-            while (ok && p.next(tile, k0, k1)) {
-                if (!qwait(&bars->tempty[buf], bph ^ 1u, a.err, DEV_TIMEOUT_TEMPTY, abort_flag)) break;
+            bool ok = true;
+            for (int tile = group; ok && tile < a.tiles; tile += groups) {
+                ok = __all_sync(0xffffffffu, qwait(&bars->tempty[buf], bph ^ 1u, a.err, DEV_TIMEOUT_TEMPTY, abort_flag));
+                if (!ok) break;
                 tc_fence_after();
                 const uint32_t dst = tmem + (uint32_t)(buf * N);
-                for (int k = k0; k < k1; ++k) {
-                    if (!qwait(&bars->full[slot], ph, a.err, DEV_TIMEOUT_FULL, abort_flag)) {
-                        ok = false;
-                        break;
-                    }
+                for (int i = 0; i < a.kst; ++i) {
+                    const int k = i + k0 < a.kst ? i + k0 : i + k0 - a.kst;
+                    ok = __all_sync(0xffffffffu, qwait(&bars->full[slot], ph, a.err, DEV_TIMEOUT_FULL, abort_flag));
+                    if (!ok) break;
                     tc_fence_after();
-                    const uint64_t ad = smem_desc_sw128(smem_addr(sm + slot * kStage));
-                    const uint64_t bd = smem_desc_sw128(smem_addr(sm + slot * kStage + kA));
+                    if (elect_one()) {
+                        const uint64_t ad = desc0 + (uint32_t)(slot * kStage >> 4), bd = ad + (uint32_t)(kA >> 4);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)  // 32 bytes of K each: 2 descriptor units
-                        mma_i8_n<CTAS>(dst, ad + 2 * j, bd + 2 * j, idesc, k > k0 || j > 0);
-                    issued = true;
-                    mma_commit_n<CTAS>(&bars->empty[slot]);
+                        for (int j = 0; j < 4; ++j)  // 32 bytes of K each: 2 descriptor units
+                            mma_i8_n<CTAS>(dst, ad + 2 * j, bd + 2 * j, idesc, i > 0 || j > 0);
+                        if (kHalves == 2 && k * 256 + 128 < a.pitch) {
+#pragma unroll
+                            for (int j = 0; j < 4; ++j)
+                                mma_i8_n<CTAS>(dst, ad + (uint32_t)(kHalf >> 4) + 2 * j, bd + (uint32_t)(kHalf >> 4) + 2 * j,
+                                               idesc, 1);
+                        }
+                        mma_commit_n<CTAS>(&bars->empty[slot]);
+                        if (i == a.kst - 1) mma_commit_n<CTAS>(&bars->tfull[buf]);
+                    }
+                    __syncwarp();
                     if (++slot == S) {
                         slot = 0;
                         ph ^= 1u;
                     }
                 }
-                if (ok) mma_commit_n<CTAS>(&bars->tfull[buf]);
                 buf ^= 1;
                 if (buf == 0) bph ^= 1u;
             }
-            if (issued) {  // every MMA has completed before the tensor memory is freed
-                mma_commit_n<CTAS>(&bars->done);
-                mbar_wait(&bars->done, 0, a.err, DEV_TIMEOUT_MMA);
-            }
+            if (elect_one()) mma_commit_n<CTAS>(&bars->done);
+            __syncwarp();
+            mbar_wait(&bars->done, 0, a.err, DEV_TIMEOUT_MMA);  // every MMA is done before the memory is freed
         }
+        __syncwarp();
     } else {
         const int q = warp & 3, rr = 32 * q + lane;  // channel within the CTA's 128 = TMEM lane
-        const uint32_t tl = tmem + ((uint32_t)(32 * q) << 16);
-        const int64_t w = (int64_t)a.shared * a.kst;
-        const int64_t my0 = group < a.sk_grid ? sk_start(group, w, a.sk_grid) : 0;
-        Pieces p(a, group, groups);
-        int tile, k0, k1, buf = 0;
+        int buf = 0;
         uint32_t bph = 0;
-        while (p.next(tile, k0, k1)) {
+        for (int tile = group; tile < a.tiles; tile += groups) {
             if (!__all_sync(0xffffffffu, qwait(&bars->tfull[buf], bph, a.err, DEV_TIMEOUT_TFULL, abort_flag))) break;
             tc_fence_after();
-            const uint32_t src = tl + (uint32_t)(buf * N);
-            const int ch = tile / a.ttiles * (128 * CTAS) + rank * 128 + rr, tok0 = tile % a.ttiles * N;
-            int first = 0, pieces = 1;
-            const int64_t tk0 = (int64_t)(tile - a.whole) * a.kst;
-            if (k1 - k0 < a.kst) {
-                first = sk_owner(tk0, w, a.sk_grid);
-                pieces = sk_owner(tk0 + a.kst - 1, w, a.sk_grid) - first + 1;
-            }
-            bool finish = true;
-            if (pieces > 1) {
-                int* pb = a.part + ((size_t)blockIdx.x * 2 + (my0 >= tk0 ? 0 : 1)) * (N * 128) + rr;
-                for (int c = 0; c < N && tok0 + c < a.rows; c += CH) {
-                    int v[CH];
-                    tmem_ld<CH>(src + c, v);
-                    tmem_ld_wait();
-#pragma unroll
-                    for (int j = 0; j < CH; ++j) __stcg(pb + (c + j) * 128, v[j]);
-                }
-                __threadfence();
-                named_bar_sync(1, 128);
-                if (threadIdx.x == 64) {
-                    int* cnt = a.cnt + (tile - a.whole) * CTAS + rank;
-                    const int last = atomicAdd(cnt, 1) == pieces - 1;
-                    if (last) *cnt = 0;  // as the next launch expects it
-                    bars->last_flag = last;
-                }
-                named_bar_sync(1, 128);
-                finish = bars->last_flag != 0;
-                named_bar_sync(1, 128);  // the next piece writes last_flag again
-                if (finish) __threadfence();
-            }
-            if (finish) {
-                const float wsv = ch < a.d ? __ldg(a.ws + ch) : 0.0f;
-                for (int c = 0; c < N && tok0 + c < a.rows; c += CH) {
-                    int v[CH];
-                    tmem_ld<CH>(src + c, v);
-                    tmem_ld_wait();
-                    for (int o = 0; o < pieces; ++o) {
-                        if (first + o == group || pieces == 1) continue;
-                        const int64_t o0 = sk_start(first + o, w, a.sk_grid);
-                        const int* pb = a.part + ((size_t)((first + o) * CTAS + rank) * 2 + (o0 >= tk0 ? 0 : 1)) * (N * 128) + rr;
-#pragma unroll
-                        for (int j = 0; j < CH; ++j) v[j] += __ldcg(pb + (c + j) * 128);
-                    }
-                    const int n = min(CH, a.rows - tok0 - c);
-                    const float xsv = lane < n ? __ldg(a.xs + tok0 + c + lane) : 0.0f;
-                    const int64_t at = (int64_t)(tok0 + c) * a.ld + ch;
-                    if (a.type == LQ_F32)
-                        store_columns<CH>(static_cast<float*>(a.y) + at, a.ld, v, xsv, wsv, n, ch < a.d);
-                    else if (a.type == LQ_F16)
-                        store_columns<CH>(static_cast<__half*>(a.y) + at, a.ld, v, xsv, wsv, n, ch < a.d);
-                    else
-                        store_columns<CH>(static_cast<__nv_bfloat16*>(a.y) + at, a.ld, v, xsv, wsv, n, ch < a.d);
-                }
+            const uint32_t src = tmem + ((uint32_t)(32 * q) << 16) + (uint32_t)(buf * N);
+            const int tok0 = tile % a.ttiles * N;
+            const int ch = rr < a.m ? (tile / a.ttiles * CTAS + rank) * a.m + rr : a.d;
+            for (int c = 0; 32 * q < a.m && c < N && tok0 + c < a.rows; c += CH) {
+                int v[CH];
+                tmem_ld<CH>(src + c, v);
+                tmem_ld_wait();
+                store_columns<CH>(a, tok0 + c, ch, v, lane);
             }
             tc_fence_before();
             __syncwarp();
@@ -396,25 +369,23 @@ __global__ void __launch_bounds__(kRowsThreads, 1) matmul_rows_kernel(const __gr
     if (CTAS == 2) cluster_sync();
     if (warp == 1) {
         tc_fence_after();
-        tmem_free<CTAS>(tmem, kCols);
+        tmem_free<CTAS, kCols>(tmem);
     }
 }
 
+constexpr int kRowsSmem = 227 * 1024;
+
 template <int N, int CTAS>
-cudaError_t rows_launch(RowsArgs a, int grid, cudaStream_t st) {
-    constexpr int kStage = rows_stage_bytes<N, CTAS>();
-    const int most = (227 * 1024 - 1024 - (int)sizeof(RowsBars)) / kStage;
+cudaError_t rows_launch(RowsArgs& a, int sms, cudaStream_t st) {
+    // barriers (1 KB), the ring, and what an MMA reads past the last stage's channels
+    const int stage = rows_halves<N>() * (a.m + N / CTAS) * 128, slack = (128 - a.m) * 128;
+    a.kst = (a.pitch + rows_halves<N>() * 128 - 1) / (rows_halves<N>() * 128);
+    const int most = (kRowsSmem - 2048 - slack) / stage;
     a.stages = most < kMaxStages ? most : kMaxStages;
-    const int smem = a.stages * kStage + 1024 + (int)sizeof(RowsBars);
+    const int smem = 2048 + a.stages * stage + slack;
     auto kern = matmul_rows_kernel<N, CTAS>;
-    static bool set[64] = {};
-    int dev = 0;
-    cudaGetDevice(&dev);
-    if (dev < 0 || dev >= 64 || !set[dev]) {
-        cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-        if (e != cudaSuccess) return e;
-        if (dev >= 0 && dev < 64) set[dev] = true;
-    }
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kRowsSmem);
+    if (e != cudaSuccess) return e;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -422,13 +393,30 @@ cudaError_t rows_launch(RowsArgs a, int grid, cudaStream_t st) {
     attr[1].val.clusterDim.x = CTAS;
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(grid);
+    const int groups = sms / CTAS;
+    cfg.gridDim = dim3((a.tiles < groups ? a.tiles : groups) * CTAS);
     cfg.blockDim = dim3(kRowsThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cfg.attrs = attr;
     cfg.numAttrs = CTAS == 2 ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, kern, a);
+}
+
+struct RowsPlan {
+    int n, ctas, m;  // tokens per tile, CTAs per tile, channels per CTA
+    int64_t rounds;
+};
+
+// The narrowest channels per tile with which all tiles of n tokens fit the
+// fewest rounds that 128 channels need.
+RowsPlan rows_plan(int n, int ctas, int rows, int d, int sms) {
+    const int64_t groups = sms / ctas, tt = (rows + n - 1) / n, ct = (d + 128 * ctas - 1) / (128 * ctas);
+    const int64_t rounds = (tt * ct + groups - 1) / groups;
+    int64_t most = rounds * groups / tt;  // channel tiles that fit
+    if (most < ct) most = ct;
+    const int64_t m = ((d + most - 1) / most + ctas - 1) / ctas;
+    return {n, ctas, (int)((m + 7) / 8 * 8), rounds};
 }
 
 }  // namespace
@@ -449,11 +437,12 @@ int quantize_rows(QuantizedTensor* out, const void* x, int type, int64_t ld, int
         if ((reinterpret_cast<uintptr_t>(out->q) & 15u) || (reinterpret_cast<uintptr_t>(out->s) & 3u) ||
             reinterpret_cast<uintptr_t>(x) % size)
             return lq_fail(LQ_EINVAL, "quantize_rows: out->q must be 16-byte aligned, x and out->s to their elements");
-        if (!ctx()) return lq_fail(LQ_ECUDA, "no CUDA device context (no device, or first use inside a graph capture)");
+        DevCtx* c = ctx();
+        if (!c) return lq_fail(LQ_ECUDA, "no CUDA device context (no device, or first use inside a graph capture)");
         int8_t* q = static_cast<int8_t*>(out->q);
-        cudaError_t e = type == LQ_F32   ? quantize_rows_t<float>(x, ld, out->rows, n, q, out->s, stream())
-                        : type == LQ_F16 ? quantize_rows_t<__half>(x, ld, out->rows, n, q, out->s, stream())
-                                         : quantize_rows_t<__nv_bfloat16>(x, ld, out->rows, n, q, out->s, stream());
+        cudaError_t e = type == LQ_F32   ? quantize_rows_t<float>(x, ld, out->rows, n, q, out->s, c->num_sms, stream())
+                        : type == LQ_F16 ? quantize_rows_t<__half>(x, ld, out->rows, n, q, out->s, c->num_sms, stream())
+                                         : quantize_rows_t<__nv_bfloat16>(x, ld, out->rows, n, q, out->s, c->num_sms, stream());
         if (e != cudaSuccess) return cuda_fail(e, "quantize_rows launch");
     }
     out->cols = out->group_size = n;
@@ -490,47 +479,49 @@ int matmul_rows(void* xout, int type, int64_t ld, const QuantizedTensor* x, cons
     a.rows = rows;
     a.d = d;
     a.type = type;
-    a.kst = (pitch + kStageBytes - 1) / kStageBytes;
-    a.early = (launch_flags() & LQ_LAUNCH_PDL) != 0;
+    a.pitch = pitch;
+    a.rot = 0;
     a.err = c->err;
-    // Tokens per tile: the fewest that hold them all up to 128; beyond, 256
-    // wherever that leaves a tile per SM, else 128.  (Pairs of CTAs: below.)
-    const int64_t ct = (d + 127) / 128;
-    int N = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256;
-    if (N == 256 && ct * ((rows + 255) / 256) < c->num_sms) N = 128;
-    const int ctas = 1;
-    const int64_t ctiles = (d + 128 * ctas - 1) / (128 * ctas);
-    a.ttiles = (rows + N - 1) / N;
-    const int64_t tiles = ctiles * a.ttiles;
-    if (tiles > INT32_MAX) return lq_fail(LQ_EUNSUPPORTED, "matmul_rows: %lld tiles", (long long)tiles);
-    const int groups = c->num_sms / ctas;
-    // whole rounds of tiles, the rest cut by stages so that every CTA gets an
-    // equal run of at least kMinRun (a cut costs a partial tile's round trip)
-    constexpr int kMinRun = 4;
-    int64_t shared = tiles % groups;
-    int64_t sk = shared * a.kst / kMinRun;
-    if (sk > groups) sk = groups;
-    if (sk <= shared) shared = sk = 0;  // nothing gained
-    a.shared = (int)shared;
-    a.whole = (int)(tiles - shared);
-    a.sk_grid = (int)sk;
-    const int64_t most = tiles - shared > sk ? tiles - shared : sk;
-    const int grid = (int)(most < groups ? most : groups) * ctas;
-    void* part = nullptr;
-    a.cnt = nullptr;
-    if (a.shared) {
-        int rc = stream_workspace(c, (size_t)grid * 2 * N * 128 * sizeof(int), &a.cnt, &part);
-        if (rc) return rc;
+    // The plan with the least time by rounds * K * time per K + start.
+    // Measured, per 128 bytes of K: the copies, about 90 bytes per ns and SM
+    // (128 channels x 128 tokens: 0.34 us, x 256: 0.48 us; a pair's 256 x 256:
+    // 0.50 us), and at least the MMAs with their waits, 0.17 us (0.19 us
+    // beyond 64 tokens); starting and ending take about 6 us, the last tile's
+    // outputs 1 us per 64 tokens.
+    RowsPlan best = {};
+    double least = 0;
+    for (int i = 0; i < 6; ++i) {
+        const int n = i < 5 ? 16 << i : 256, ctas = i < 5 ? 1 : 2;
+        if (n > 16 && n / 2 >= rows) break;  // half of it would do
+        const RowsPlan p = rows_plan(n, ctas, rows, d, c->num_sms);
+        double stage = ctas == 2 ? 0.50 * (p.m + 128) / 256 : (p.m + n) * 128 / 90e3;
+        const double mma = n <= 64 ? 0.17 : 0.19;
+        if (stage < mma) stage = mma;
+        const double us = 6 + n / 64.0 + p.rounds * (pitch / 128.0) * stage;
+        if (!best.n || us < least) {
+            best = p;
+            least = us;
+        }
     }
-    a.part = static_cast<int*>(part);
-    if (!byte_map_2d(&a.wmap, w->q, pitch, d, pitch, kStageBytes, 128, true) ||
-        !byte_map_2d(&a.xmap, x->q, pitch, rows, pitch, kStageBytes, N / ctas, true))
+    const int N = best.n;
+    a.m = best.m;
+    a.ttiles = (rows + N - 1) / N;
+    const int64_t tiles = (int64_t)((d + a.m * best.ctas - 1) / (a.m * best.ctas)) * a.ttiles;
+    if (tiles > INT32_MAX / 2) return lq_fail(LQ_EUNSUPPORTED, "matmul_rows: %d x %d outputs", rows, d);
+    a.tiles = (int)tiles;
+    a.rot = a.ttiles == 1;
+    a.xbox = N / best.ctas < rows ? N / best.ctas : rows;
+    if (!byte_map_2d(&a.wmap, w->q, pitch, d, pitch, 128, a.m, true) ||
+        !byte_map_2d(&a.xmap, x->q, pitch, rows, pitch, 128, a.xbox, true))
         return lq_fail(LQ_ECUDA, "matmul_rows: tensor map of %d x %d or %d x %d", d, pitch, rows, pitch);
-    cudaError_t e = N == 16   ? rows_launch<16, 1>(a, grid, stream())
-                    : N == 32 ? rows_launch<32, 1>(a, grid, stream())
-                    : N == 64 ? rows_launch<64, 1>(a, grid, stream())
-                    : N == 128 ? rows_launch<128, 1>(a, grid, stream())
-                               : rows_launch<256, 1>(a, grid, stream());
+    cudaStream_t st = stream();
+    const int sms = c->num_sms;
+    cudaError_t e = best.ctas == 2 ? rows_launch<256, 2>(a, sms, st)
+                    : N == 16      ? rows_launch<16, 1>(a, sms, st)
+                    : N == 32      ? rows_launch<32, 1>(a, sms, st)
+                    : N == 64      ? rows_launch<64, 1>(a, sms, st)
+                    : N == 128     ? rows_launch<128, 1>(a, sms, st)
+                                   : rows_launch<256, 1>(a, sms, st);
     if (e != cudaSuccess) return cuda_fail(e, "matmul_rows launch");
     return LQ_OK;
 }
