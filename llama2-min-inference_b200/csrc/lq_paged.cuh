@@ -15,16 +15,16 @@ enum : int {
 };
 
 // rows [r0, r0 + n) of the call are positions [begin, ctx) of the sequence;
-// rows at negative positions are dropped (r0 moves up)
+// rows [first, r0) would be at negative positions and are no tokens
 struct SeqRows {
-    int r0, n, begin, ctx;
+    int first, r0, n, begin, ctx;
 };
 
 __device__ __forceinline__ SeqRows seq_rows(const KVBatch& b, int s, int* err) {
     const int a = __ldg(b.row_start + s), e = __ldg(b.row_start + s + 1);
     SeqRows q;
     q.ctx = __ldg(b.context + s);
-    q.r0 = a;
+    q.first = q.r0 = a;
     q.n = e - a;
     if (a < 0 || e < a || e > b.n_rows || e - a > b.max_rows) {
         set_err(err, DEV_BAD_ROWS);

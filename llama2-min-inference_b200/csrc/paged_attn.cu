@@ -1,5 +1,19 @@
 // paged_attention: causal attention of ragged rows over the paged int8 cache.
-#include <cfloat>
+//
+// Both products run on integer tensor-core instructions over the cache's
+// codes as they lie, so that no code is ever converted.  The other operand is
+// written in fixed point, as int8 digits:
+//
+//   q . K:  a row of q is qs * (65536 d1 + 256 d2 + d3), qs = max|q| / (127 *
+//           65536), the digits signed bytes (fp32; two digits for the 16-bit
+//           types).  The digits' dots with the codes are exact; the score is
+//           (65536 D1 + 256 D2 + D3) * qs * scale * s_K[page].
+//   p . V:  p * s_V[page] / max s_V of the 32 tokens is in [0, 1] and becomes 24
+//           (or 16) bits, whose bytes are unsigned digits.
+//
+// A product's error so is 2^-25 of the row's largest term (2^-17 for the
+// 16-bit types, whose results carry 2^-9 or 2^-12), less than the rounding of
+// an fp32 sum.  Softmax statistics and the output's accumulator are fp32.
 #include <cmath>
 
 #include "lq_ctx.h"
@@ -10,6 +24,12 @@
 namespace lq {
 namespace {
 
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+// Adding an integer below 2^22 to these bits gives the float 1.5 * 2^23 plus it:
+// accumulators that start here are read as floats without a conversion.
+constexpr int kBiasBits = 0x4B400000;
+constexpr float kBias = 12582912.0f;
+
 struct AttArgs {
     PagedKV c;
     KVBatch b;
@@ -17,14 +37,499 @@ struct AttArgs {
     void* out;
     float* lse;
     int64_t ld_q, ld_out;
-    int n_heads;
-    float scale;
+    int n_heads, group, type;
+    float scale;      // log2(e) times the caller's
+    int row_tiles;    // tiles of 8 (token, head) rows of a sequence and kv head
+    int chunk;        // tokens per split
+    float* part;      // [job][split][8][head_size + 2]: out, max, sum
+    int* cnt;         // [job] arrivals
     int* err;
 };
 
-// one warp per (row, head); the cache is walked token by token
-template <typename T>
-__global__ void __launch_bounds__(128) attend_kernel(const __grid_constant__ AttArgs a) {
+__device__ __forceinline__ float load_q(const AttArgs& a, int64_t i) {
+    if (a.type == LQ_F32) return static_cast<const float*>(a.q)[i];
+    if (a.type == LQ_F16) return to_f32(static_cast<const __half*>(a.q)[i]);
+    return to_f32(static_cast<const __nv_bfloat16*>(a.q)[i]);
+}
+
+__device__ __forceinline__ void store_out(const AttArgs& a, int64_t i, float v) {
+    if (a.type == LQ_F32)
+        static_cast<float*>(a.out)[i] = v;
+    else if (a.type == LQ_F16)
+        static_cast<__half*>(a.out)[i] = from_f32<__half>(v);
+    else
+        static_cast<__nv_bfloat16*>(a.out)[i] = from_f32<__nv_bfloat16>(v);
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr));
+}
+
+// d += a (16 x 32 signed bytes) * b (32 x 8 signed bytes)
+__device__ __forceinline__ void mma_s8(int (&d)[4], uint4 a, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+        : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+}
+
+// d += a (16 x 32 unsigned bytes) * b (32 x 8 signed bytes)
+__device__ __forceinline__ void mma_u8(int (&d)[4], uint4 a, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+        : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ float unbias(int d) { return __int_as_float(d) - kBias; }
+
+// ---------------------------------------------------------------------------
+// Few rows per kv head (decode): bound by the cache's bytes from HBM.
+//
+// One CTA per (sequence, kv head, tile of 8 rows, split of the context); its
+// four warps take 32 tokens each in turn, each through a ring of its own of
+// bulk copies, and are joined at the end; the splits of a row are joined by
+// the last CTA to arrive, in split order.  An MMA's 16 rows are the 8 (token,
+// head) rows twice: rows 0-7 hold their first digit, rows 8-15 the second, so
+// a thread finds both digits' dots of its row in its own registers.  A third
+// digit takes a second MMA.
+//
+// Tokens and MMA columns: the two 8-column tiles over 16 tokens are dealt so
+// that a thread's four scores are four neighbouring tokens (the A operand of
+// p . V) and that the eight rows an ldmatrix reads lie in different banks:
+// column 2j + e of the even tile is token 4j + 2x + e with x = j / 2, of the odd
+// tile with x = 1 - j / 2.
+
+constexpr int kFewWarps = 4;
+constexpr int kFewThreads = 32 * kFewWarps;
+constexpr int kItem = 32;   // tokens of one step of a warp
+constexpr int kSlots = 2;   // its ring
+constexpr int kFewRows = 32;  // (token, head) rows of a sequence up to which it is taken
+
+template <int HS>
+constexpr int few_smem() {
+    return kFewWarps * kSlots * kItem * HS * 2;
+}
+
+template <int ND, int HS, bool EXACT>
+__global__ void __launch_bounds__(kFewThreads) attend_few_kernel(const __grid_constant__ AttArgs a) {
+    constexpr int KS = HS / 32;       // k steps of q . K
+    constexpr int NP = ND == 3 ? 2 : 1;  // MMAs per tile
+    constexpr int NT = HS / 8;        // column tiles of p . V
+    extern __shared__ __align__(128) unsigned char ring_all[];
+    __shared__ uint4 qfrag[KS * NP * 32];
+    __shared__ float qscale[8];
+    __shared__ uint64_t bars[kFewWarps * kSlots];
+    __shared__ int last_flag;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int hs = EXACT ? HS : a.c.head_size;
+    const int P = a.c.page_size, H = a.c.n_kv_heads, g = a.group;
+    const int rt = blockIdx.x % a.row_tiles, sh = blockIdx.x / a.row_tiles, h = sh % H, s = sh / H;
+    const int split = blockIdx.y;
+
+    if (tid < kFewWarps * kSlots) mbar_init(&bars[tid], 1);
+    fence_mbar_init();
+    pdl_trigger();
+    pdl_wait();
+    const SeqRows q = seq_rows(a.b, s, split == 0 && rt == 0 && h == 0 && tid == 0 ? a.err : nullptr);
+    if (split == 0 && rt == 0) {  // rows that attend to nothing
+        for (int i = tid; i < (q.r0 - q.first) * g * hs; i += kFewThreads) {
+            const int row = q.first + i / (g * hs), d = i % (g * hs);
+            store_out(a, (int64_t)row * a.ld_out + (int64_t)h * g * hs + d, 0.0f);
+            if (a.lse && d % hs == 0) a.lse[(int64_t)row * a.n_heads + h * g + d / hs] = -INFINITY;
+        }
+    }
+    const int rows = q.n * g;
+    if (rows > kFewRows || rt * 8 >= rows) return;
+    const int top = min(rows, rt * 8 + 8) - 1;            // the tile's last row
+    const int seen = q.begin + top / g + 1;               // tokens that it sees
+    const int splits = (seen + a.chunk - 1) / a.chunk;
+    if (split >= splits) return;
+    const int ta = split * a.chunk, tb = min(ta + a.chunk, seen);
+    int* const err = lane == 0 ? a.err : nullptr;
+
+    // the warp's items are kItem tokens at ta + (warp + kFewWarps * j) * kItem; lane L
+    // keeps the pages of item j0 + L
+    const int items = max(0, ((tb - ta + kItem - 1) / kItem - warp + kFewWarps - 1) / kFewWarps);
+    unsigned char* ring = ring_all + warp * kSlots * kItem * HS * 2;
+    int held = -1;  // the block of 32 items whose pages are held
+    int64_t pg0 = -1, pg1 = -1;
+    float2 sc_slot[kSlots];
+    const uint64_t policy = l2_evict_first_policy();
+    auto issue = [&](int j) {
+        if ((j >> 5) != held) {
+            held = j >> 5;
+            const int t = ta + (warp + kFewWarps * (held * 32 + lane)) * kItem;
+            pg0 = t < tb ? page_of(a.c, a.b, s, t / P, a.err) : -1;
+            pg1 = P < kItem && t + 16 < tb ? page_of(a.c, a.b, s, t / P + 1, a.err) : -1;
+        }
+        const int64_t p0 = __shfl_sync(0xffffffffu, pg0, j & 31), p1 = __shfl_sync(0xffffffffu, pg1, j & 31);
+        const int slot = j % kSlots;
+        uint64_t* bar = &bars[warp * kSlots + slot];
+        unsigned char* dst = ring + slot * kItem * HS * 2;
+        const int64_t cell = (int64_t)hs * P * 2;
+        const int8_t* codes = static_cast<const int8_t*>(a.c.codes);
+        const int8_t *c0 = codes + (p0 * H + h) * cell, *c1 = codes + (p1 * H + h) * cell;
+        const int bytes = P < kItem ? ((p0 >= 0) + (p1 >= 0)) * (int)cell : p0 >= 0 ? kItem * hs * 2 : 0;
+        __syncwarp();  // every lane has read the slot's last item
+        if (lane == 0) mbar_arrive_expect_tx(bar, bytes);
+        __syncwarp();
+        if (P <= kItem) {
+            // whole pages, K and V together
+            if (lane == 0 && p0 >= 0) bulk_g2s(dst, c0, (uint32_t)cell, bar, policy);
+            if (lane == 1 && p1 >= 0) bulk_g2s(dst + cell, c1, (uint32_t)cell, bar, policy);
+        } else if (p0 >= 0) {
+            const int off = (ta + (warp + kFewWarps * j) * kItem) % P;
+            if (lane < hs / 16)  // 16 dims of the item's tokens
+                bulk_g2s(dst + lane * kItem * 16, c0 + ((int64_t)lane * P + off) * 16, kItem * 16, bar, policy);
+            else if (lane == hs / 16)
+                bulk_g2s(dst + kItem * hs, c0 + (int64_t)hs * (P + off), kItem * hs, bar, policy);
+        }
+        // the scales of the item's pages, by lane 0 (and 1): used one step later
+        const int64_t pl = lane == 1 ? p1 : p0;
+        float2 sc = make_float2(NAN, NAN);
+        if (lane < 2 && pl >= 0) sc = __ldg(reinterpret_cast<const float2*>(a.c.scales) + pl * H + h);
+        return sc;
+    };
+    __syncthreads();  // barriers are ready
+#pragma unroll
+    for (int j = 0; j < kSlots; ++j)
+        if (j < items) sc_slot[j] = issue(j);
+
+    // the digits of the tile's rows, in the order of the A operand: two rows per warp
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int r8 = 2 * warp + i, r = rt * 8 + r8;
+        const bool have = r < rows;
+        const int64_t base = have ? (int64_t)(q.r0 + r / g) * a.ld_q + (int64_t)(h * g + r % g) * hs : 0;
+        float x[(HS + 127) / 128][4];
+        uint32_t m = 0;
+#pragma unroll
+        for (int b = 0; b < (HS + 127) / 128; ++b)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int d = b * 128 + lane * 4 + e;
+                x[b][e] = have && d < hs ? load_q(a, base + d) : 0.0f;
+                m = max(m, abs_bits(x[b][e]));
+            }
+        m = __reduce_max_sync(0xffffffffu, m);
+        constexpr float kTop = ND == 3 ? 8323072.0f : 32512.0f;  // 127 * 256^(ND - 1)
+        const float peak = __uint_as_float(m);
+        const bool fine = m < kInfBits && peak > 1e-30f;
+        const float inv = fine ? kTop / peak : 0.0f;
+        if (lane == 0) qscale[r8] = m >= kInfBits ? NAN : fine ? peak / kTop * a.scale : 0.0f;
+#pragma unroll
+        for (int b = 0; b < (HS + 127) / 128; ++b) {
+            const int d = b * 128 + lane * 4;
+            if (d >= HS) continue;
+            uint32_t w[3] = {};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                int n = m >= kInfBits ? 0 : __float2int_rn(x[b][e] * inv);
+                if (ND == 3) {
+                    const int d3 = (int)(int8_t)n;
+                    n = (n - d3) >> 8;
+                    w[2] |= (uint32_t)(d3 & 255) << (8 * e);
+                }
+                const int d2 = (int)(int8_t)n;
+                w[1] |= (uint32_t)(d2 & 255) << (8 * e);
+                w[0] |= (uint32_t)(((n - d2) >> 8) & 255) << (8 * e);
+            }
+            const int ks = d / 32, half = d % 32 / 16, L = r8 * 4 + d % 16 / 4;
+            uint32_t* f = reinterpret_cast<uint32_t*>(&qfrag[ks * NP * 32 + L]);
+            f[half * 2] = w[0];
+            f[half * 2 + 1] = w[1];
+            if (ND == 3) {
+                f[32 * 4 + half * 2] = w[2];
+                f[32 * 4 + half * 2 + 1] = 0;
+            }
+        }
+    }
+    __syncthreads();
+
+    const int r8 = lane >> 2, jj = lane & 3;
+    const int r = rt * 8 + r8;
+    const int pos = r < rows ? q.begin + r / g : -1;  // the row's last token
+    const float fs = qscale[r8];
+    float m = -INFINITY, l = 0.0f, poison = 0.0f;
+    float o[NT][2];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) o[t][0] = o[t][1] = 0.0f;
+
+    // strides of an item in shared memory: 16 tokens on, 16 dims on (K), V's start
+    const int cell = hs * P * 2;
+    const int k16 = P < kItem ? cell : 256, kc = P < kItem ? 256 : kItem * 16;
+    const int v0 = P < kItem ? cell / 2 : kItem * hs, v16 = P < kItem ? cell : hs * 16;
+    // ldmatrix rows of this lane: matrix mi = lane / 8, row lane % 8
+    const int mi = lane >> 3, mr = lane & 7, mj = mr >> 1;
+    const int ktok = 4 * mj + 2 * ((mi >> 1) ? 1 - (mj >> 1) : mj >> 1) + (mr & 1);
+    const int last_chunk = hs / 16 - 1;
+
+    for (int j = 0; j < items; ++j) {
+        const int slot = j % kSlots;
+        const float2 sc_lane = slot == 0 ? sc_slot[0] : sc_slot[1];
+        const uint32_t base = smem_addr(ring + slot * kItem * HS * 2);
+        const bool ok = mbar_wait(&bars[warp * kSlots + slot], (uint32_t)((j / kSlots) & 1), err, DEV_TIMEOUT_FULL);
+        if (!__all_sync(0xffffffffu, ok)) {
+            // confirm the copies still in flight before anything else is written there
+            for (int k = j; k < min(j + kSlots, items); ++k)
+                mbar_wait(&bars[warp * kSlots + k % kSlots], (uint32_t)((k / kSlots) & 1), err, DEV_TIMEOUT_DRAIN);
+            __syncwarp();
+            break;
+        }
+        const int t0 = ta + (warp + kFewWarps * j) * kItem;
+        float sk[2], sv[2];
+        sk[0] = __shfl_sync(0xffffffffu, sc_lane.x, 0);
+        sv[0] = __shfl_sync(0xffffffffu, sc_lane.y, 0);
+        sk[1] = sk[0];
+        sv[1] = sv[0];
+        if (P < kItem) {
+            sk[1] = __shfl_sync(0xffffffffu, sc_lane.x, 1);
+            sv[1] = __shfl_sync(0xffffffffu, sc_lane.y, 1);
+        }
+        const bool two = t0 + 16 < tb;
+        // a scale that is not finite takes the rows that see its page with it
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+            if (!(sv[c] < INFINITY)) {
+                if (t0 + 16 * c <= pos && (c == 0 || two)) poison = NAN;
+                sv[c] = 0.0f;
+            }
+        const float svm = fmaxf(sv[0], sv[1]);
+        float top_new = m;
+        float x[4][2];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {  // 16 tokens: tiles 2c and 2c + 1
+            int d[2][NP][4];
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int p = 0; p < NP; ++p)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) d[i][p][e] = kBiasBits;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                if (!EXACT && ks * 32 >= hs) break;
+                uint32_t b[4];
+                const int chunk = EXACT ? 2 * ks + (mi & 1) : min(2 * ks + (mi & 1), last_chunk);
+                ldsm4(base + c * k16 + chunk * kc + ktok * 16, b);
+#pragma unroll
+                for (int p = 0; p < NP; ++p) {
+                    const uint4 f = qfrag[(ks * NP + p) * 32 + lane];
+                    mma_s8(d[0][p], f, b[0], b[1]);
+                    mma_s8(d[1][p], f, b[2], b[3]);
+                }
+            }
+            const float f = fs * sk[c];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int t = t0 + 16 * c + 4 * jj + 2 * (i ? 1 - (jj >> 1) : jj >> 1);
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float v = fmaf(unbias(d[i][0][e]), 256.0f, unbias(d[i][0][2 + e]));
+                    if (ND == 3) v = fmaf(v, 256.0f, unbias(d[i][NP - 1][e]));
+                    v *= f;
+                    if (t + e > pos) v = -INFINITY;
+                    x[2 * c + i][e] = v;
+                    top_new = fmaxf(top_new, v);
+                }
+            }
+        }
+        top_new = fmaxf(top_new, __shfl_xor_sync(0xffffffffu, top_new, 1));
+        top_new = fmaxf(top_new, __shfl_xor_sync(0xffffffffu, top_new, 2));
+        const float mref = top_new == -INFINITY ? 0.0f : top_new;
+        const float corr = exp2_fast(m - mref);  // 0 for the first tokens
+        m = top_new;
+        l *= corr;
+        // weights in fixed point; their bytes are the A operand
+        uint4 pa, pb;
+        uint32_t* pw[2] = {reinterpret_cast<uint32_t*>(&pa), reinterpret_cast<uint32_t*>(&pb)};
+        pb = make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            constexpr float kOne = ND == 3 ? 16777215.0f : 65535.0f;
+            const float w = svm > 0.0f ? sv[c] / svm * kOne : 0.0f;
+            uint32_t u[2][2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const float p = exp2_fast(x[2 * c + i][e] - mref);
+                    l += p;
+                    u[i][e] = ND == 3 ? __float2uint_rn(p * w) : __float_as_uint(p * w + 8388608.0f);
+                }
+            const uint32_t order = jj < 2 ? 0x5410u : 0x1054u;
+#pragma unroll
+            for (int k = 0; k < ND; ++k) {  // byte ND - 1 - k of the four weights
+                const uint32_t sel = ((4u + ND - 1 - k) << 4) | (ND - 1 - k);
+                const uint32_t word = __byte_perm(__byte_perm(u[0][0], u[0][1], sel), __byte_perm(u[1][0], u[1][1], sel), order);
+                if (k < 2)
+                    pw[0][c * 2 + k] = word;
+                else
+                    pw[1][c * 2] = word;
+            }
+        }
+        const float of = svm * (ND == 3 ? 1.0f / 16777215.0f : 1.0f / 65535.0f);
+        const bool turn = __any_sync(0xffffffffu, corr != 1.0f);
+#pragma unroll
+        for (int t = 0; t < NT; t += 2) {
+            if (!EXACT && t * 8 >= hs) break;
+            uint32_t b[4];
+            ldsm4(base + v0 + (mi & 1) * v16 + ((t + (mi >> 1)) * 8 + mr) * 16, b);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                int d[4] = {kBiasBits, kBiasBits, kBiasBits, kBiasBits}, d3[4] = {kBiasBits, kBiasBits, kBiasBits, kBiasBits};
+                mma_u8(d, pa, b[2 * i], b[2 * i + 1]);
+                if (ND == 3) mma_u8(d3, pb, b[2 * i], b[2 * i + 1]);
+                if (turn) {
+                    o[t + i][0] *= corr;
+                    o[t + i][1] *= corr;
+                }
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float v = fmaf(unbias(d[e]), 256.0f, unbias(d[2 + e]));
+                    if (ND == 3) v = fmaf(v, 256.0f, unbias(d3[e]));
+                    o[t + i][e] = fmaf(v, of, o[t + i][e]);
+                }
+            }
+        }
+        if (j + kSlots < items) {
+            const float2 sc = issue(j + kSlots);
+            if (slot == 0)
+                sc_slot[0] = sc;
+            else
+                sc_slot[1] = sc;
+        }
+    }
+    l += __shfl_xor_sync(0xffffffffu, l, 1);
+    l += __shfl_xor_sync(0xffffffffu, l, 2);
+
+    // join the warps: [warp][8][hs + 2] over the rings
+    __syncthreads();
+    float* join = reinterpret_cast<float*>(ring_all);
+    const int w1 = hs + 2;
+    {
+        float* mine = join + (warp * 8 + r8) * w1;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            if (!EXACT && t * 8 >= hs) break;
+            mine[t * 8 + 2 * jj] = o[t][0] + poison;
+            mine[t * 8 + 2 * jj + 1] = o[t][1] + poison;
+        }
+        if (jj == 0) {
+            mine[hs] = m;
+            mine[hs + 1] = l;
+        }
+    }
+    __syncthreads();
+    const int64_t job = (int64_t)blockIdx.x;
+    float* part = a.part + (job * gridDim.y + split) * 8 * w1;
+    // a row's parts src[i], i < n: joined value of dim d, and the row's max and sum
+    auto joined = [&](const float* src, int64_t step, int n, int d, float& mm, float& ll) {
+        mm = -INFINITY;
+        for (int i = 0; i < n; ++i) mm = fmaxf(mm, __ldcg(src + i * step + hs));
+        const float ref = mm == -INFINITY ? 0.0f : mm;
+        float v = 0.0f;
+        ll = 0.0f;
+        for (int i = 0; i < n; ++i) {
+            const float c = exp2_fast(__ldcg(src + i * step + hs) - ref);
+            ll = fmaf(__ldcg(src + i * step + hs + 1), c, ll);
+            v = fmaf(__ldcg(src + i * step + d), c, v);
+        }
+        return v;
+    };
+    auto finish = [&](int rr, int d, float v, float mm, float ll) {
+        const int row = q.r0 + rr / g, head = h * g + rr % g;
+        store_out(a, (int64_t)row * a.ld_out + (int64_t)head * hs + d, v / ll);
+        if (a.lse && d == 0) a.lse[(int64_t)row * a.n_heads + head] = (mm + log2f(ll)) * kLn2;
+    };
+    const int valid = top + 1 - rt * 8;
+    for (int i = tid; i < valid * hs; i += kFewThreads) {
+        const int row8 = i / hs, d = i % hs;
+        float mm = -INFINITY, ll = 0.0f, v = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kFewWarps; ++w) mm = fmaxf(mm, join[(w * 8 + row8) * w1 + hs]);
+        const float ref = mm == -INFINITY ? 0.0f : mm;
+#pragma unroll
+        for (int w = 0; w < kFewWarps; ++w) {
+            const float* src = join + (w * 8 + row8) * w1;
+            const float c = exp2_fast(src[hs] - ref);
+            ll = fmaf(src[hs + 1], c, ll);
+            v = fmaf(src[d], c, v);
+        }
+        if (splits == 1) {
+            finish(rt * 8 + row8, d, v, mm, ll);
+        } else {
+            __stcg(part + row8 * w1 + d, v);
+            if (d == 0) {
+                __stcg(part + row8 * w1 + hs, mm);
+                __stcg(part + row8 * w1 + hs + 1, ll);
+            }
+        }
+    }
+    if (splits == 1) return;
+    __threadfence();
+    __syncthreads();
+    if (tid == 0) {
+        const int n = atomicAdd(a.cnt + job, 1);
+        last_flag = n == splits - 1;
+        if (last_flag) a.cnt[job] = 0;  // as the next launch expects it
+    }
+    __syncthreads();
+    if (!last_flag) return;
+    __threadfence();
+    const float* all = a.part + job * gridDim.y * 8 * w1;
+    for (int i = tid; i < valid * hs; i += kFewThreads) {
+        const int row8 = i / hs, d = i % hs;
+        float mm, ll;
+        const float v = joined(all + row8 * w1, 8 * w1, splits, d, mm, ll);
+        finish(rt * 8 + row8, d, v, mm, ll);
+    }
+}
+
+template <int ND, int HS, bool EXACT>
+cudaError_t few_launch(const AttArgs& a, dim3 grid, cudaStream_t st) {
+    auto kern = attend_few_kernel<ND, HS, EXACT>;
+    constexpr int join = kFewWarps * 8 * (HS + 2) * 4;
+    constexpr int smem = few_smem<HS>() > join ? few_smem<HS>() : join;
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e == cudaSuccess)
+        e = cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    if (e != cudaSuccess) return e;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(kFewThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kern, a);
+}
+
+template <int ND>
+cudaError_t few_launch(const AttArgs& a, dim3 grid, cudaStream_t st) {
+    const int hs = a.c.head_size;
+    if (hs == 64) return few_launch<ND, 64, true>(a, grid, st);
+    if (hs == 128) return few_launch<ND, 128, true>(a, grid, st);
+    if (hs == 256) return few_launch<ND, 256, true>(a, grid, st);
+    if (hs < 64) return few_launch<ND, 64, false>(a, grid, st);
+    if (hs < 128) return few_launch<ND, 128, false>(a, grid, st);
+    return few_launch<ND, 256, false>(a, grid, st);
+}
+
+// ---------------------------------------------------------------------------
+// Many rows per kv head: one warp per (row, head), the cache token by token.
+
+__global__ void __launch_bounds__(128) attend_many_kernel(const __grid_constant__ AttArgs a) {
     const int lane = threadIdx.x & 31;
     const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
     const int row = (int)(w / a.n_heads), head = (int)(w % a.n_heads);
@@ -36,11 +541,13 @@ __global__ void __launch_bounds__(128) attend_kernel(const __grid_constant__ Att
     int last = -1;
     if (s >= 0) {
         const SeqRows q = seq_rows(a.b, s, a.err);
+        if (q.n * a.group <= kFewRows) return;
         if (row >= q.r0 && row < q.r0 + q.n) last = q.begin + row - q.r0;
     }
+    if (last < 0) return;
     float qv[8], o[8] = {};
-    const T* qp = static_cast<const T*>(a.q) + row * a.ld_q + (int64_t)head * hs;
-    for (int j = 0; j < 8; ++j) qv[j] = lane + 32 * j < hs ? to_f32(qp[lane + 32 * j]) : 0.0f;
+    for (int j = 0; j < 8; ++j)
+        qv[j] = lane + 32 * j < hs ? load_q(a, row * a.ld_q + (int64_t)head * hs + lane + 32 * j) : 0.0f;
     float m = -INFINITY, l = 0.0f;
     for (int t = 0; t <= last; ++t) {
         const int64_t page = page_of(a.c, a.b, s, t / P, a.err);
@@ -55,7 +562,7 @@ __global__ void __launch_bounds__(128) attend_kernel(const __grid_constant__ Att
             const int e = lane + 32 * j;
             if (e < hs) d += qv[j] * (float)kc[((int64_t)(e / 16) * P + u) * 16 + e % 16];
         }
-        d = warp_sum(d) * (sk * a.scale);
+        d = warp_sum(d) * (sk * a.scale * kLn2);
         const float mn = fmaxf(m, d);
         const float c = m == -INFINITY ? 0.0f : expf(m - mn), p = d != d ? d : expf(d - mn);
         l = l * c + p;
@@ -65,10 +572,9 @@ __global__ void __launch_bounds__(128) attend_kernel(const __grid_constant__ Att
         }
         m = mn;
     }
-    T* op = static_cast<T*>(a.out) + row * a.ld_out + (int64_t)head * hs;
     for (int j = 0; j < 8; ++j)
-        if (lane + 32 * j < hs) op[lane + 32 * j] = from_f32<T>(last < 0 ? 0.0f : o[j] / l);
-    if (a.lse && lane == 0) a.lse[(int64_t)row * a.n_heads + head] = last < 0 ? -INFINITY : m + logf(l);
+        if (lane + 32 * j < hs) store_out(a, row * a.ld_out + (int64_t)head * hs + lane + 32 * j, o[j] / l);
+    if (a.lse && lane == 0) a.lse[(int64_t)row * a.n_heads + head] = m + logf(l);
 }
 
 }  // namespace
@@ -82,7 +588,7 @@ extern "C" int paged_attention(void* out, int64_t ld_out, const void* q, int64_t
     if (rc) return rc;
     if (n_heads <= 0) return lq_fail(LQ_EINVAL, "paged_attention: %d query heads", n_heads);
     if (!(scale == scale) || std::isinf(scale)) return lq_fail(LQ_EINVAL, "paged_attention: scale is not finite");
-    if (batch->n_rows == 0) return LQ_OK;
+    if (batch->n_seqs == 0 || batch->n_rows == 0) return LQ_OK;
     const int64_t row = (int64_t)n_heads * cache->head_size;
     if (!out || !q || ld_out < row || ld_q < row)
         return lq_fail(LQ_EINVAL, "paged_attention: out or q not set, or rows closer than %lld elements", (long long)row);
@@ -92,15 +598,50 @@ extern "C" int paged_attention(void* out, int64_t ld_out, const void* q, int64_t
         return lq_fail(LQ_EINVAL, "paged_attention: a tensor is not aligned to its elements");
     DevCtx* c = ctx();
     if (!c) return lq_fail(LQ_ECUDA, "no CUDA device context (no device, or first use inside a graph capture)");
-    AttArgs a = {*cache, *batch, q, out, lse, ld_q, ld_out, n_heads, scale, c->err};
-    const int64_t blocks = ((int64_t)batch->n_rows * n_heads + 3) / 4;
-    if (blocks > INT32_MAX) return lq_fail(LQ_EUNSUPPORTED, "paged_attention: too many rows and heads");
-    if (type == LQ_F32)
-        attend_kernel<float><<<(unsigned)blocks, 128, 0, stream()>>>(a);
-    else if (type == LQ_F16)
-        attend_kernel<__half><<<(unsigned)blocks, 128, 0, stream()>>>(a);
-    else
-        attend_kernel<__nv_bfloat16><<<(unsigned)blocks, 128, 0, stream()>>>(a);
-    cudaError_t e = cudaGetLastError();
-    return e == cudaSuccess ? LQ_OK : cuda_fail(e, "paged_attention launch");
+    AttArgs a = {};
+    a.c = *cache;
+    a.b = *batch;
+    a.q = q;
+    a.out = out;
+    a.lse = lse;
+    a.ld_q = ld_q;
+    a.ld_out = ld_out;
+    a.n_heads = n_heads;
+    a.group = n_heads / cache->n_kv_heads;
+    a.type = type;
+    a.scale = scale * kLog2e;
+    a.err = c->err;
+    // few rows: every (sequence, kv head, row tile) is cut into splits of the
+    // context until the GPU's CTA slots are filled, 128 tokens at least
+    const int64_t most_rows = (int64_t)batch->max_rows * a.group;
+    a.row_tiles = (int)(((most_rows < kFewRows ? most_rows : kFewRows) + 7) / 8);
+    if (a.row_tiles < 1) a.row_tiles = 1;
+    const int64_t jobs = (int64_t)batch->n_seqs * cache->n_kv_heads * a.row_tiles;
+    const int64_t slots = 3 * c->num_sms;
+    int64_t splits = jobs <= kWsCounters ? slots / jobs : 1;
+    const int64_t most = (batch->max_context + 127) / 128;
+    if (splits > most) splits = most;
+    if (splits < 1) splits = 1;
+    a.chunk = (int)(((batch->max_context + splits - 1) / splits + 127) / 128 * 128);
+    if (a.chunk < 128) a.chunk = 128;
+    splits = (batch->max_context + a.chunk - 1) / a.chunk;
+    if (splits < 1) splits = 1;
+    if (jobs > INT32_MAX) return lq_fail(LQ_EUNSUPPORTED, "paged_attention: %lld (sequence, kv head) pairs", (long long)jobs);
+    void* part = nullptr;
+    if (splits > 1) {
+        rc = stream_workspace(c, (size_t)jobs * splits * 8 * (cache->head_size + 2) * sizeof(float), &a.cnt, &part);
+        if (rc) return rc;
+    }
+    a.part = static_cast<float*>(part);
+    const dim3 grid((unsigned)jobs, (unsigned)splits);
+    cudaError_t e = type == LQ_F32 ? few_launch<3>(a, grid, stream()) : few_launch<2>(a, grid, stream());
+    if (e != cudaSuccess) return cuda_fail(e, "paged_attention launch");
+    if (most_rows > kFewRows) {
+        const int64_t blocks = ((int64_t)batch->n_rows * n_heads + 3) / 4;
+        if (blocks > INT32_MAX) return lq_fail(LQ_EUNSUPPORTED, "paged_attention: too many rows and heads");
+        attend_many_kernel<<<(unsigned)blocks, 128, 0, stream()>>>(a);
+        e = cudaGetLastError();
+        if (e != cudaSuccess) return cuda_fail(e, "paged_attention launch");
+    }
+    return LQ_OK;
 }
