@@ -41,7 +41,7 @@ struct AttArgs {
     float scale;      // log2(e) times the caller's
     int row_tiles;    // tiles of 8 (token, head) rows of a sequence and kv head
     int chunk;        // tokens per split
-    float* part;      // [job][split][8][head_size + 2]: out, max, sum
+    float* part;      // [job][split][8][head_size + 8]: out, max, sum
     int* cnt;         // [job] arrivals
     int* err;
 };
@@ -118,7 +118,7 @@ constexpr int few_smem() {
 }
 
 template <int ND, int HS, bool EXACT>
-__global__ void __launch_bounds__(kFewThreads) attend_few_kernel(const __grid_constant__ AttArgs a) {
+__global__ void __launch_bounds__(kFewThreads, HS <= 128 ? 3 : 1) attend_few_kernel(const __grid_constant__ AttArgs a) {
     constexpr int KS = HS / 32;       // k steps of q . K
     constexpr int NP = ND == 3 ? 2 : 1;  // MMAs per tile
     constexpr int NT = HS / 8;        // column tiles of p . V
@@ -410,17 +410,17 @@ __global__ void __launch_bounds__(kFewThreads) attend_few_kernel(const __grid_co
     l += __shfl_xor_sync(0xffffffffu, l, 1);
     l += __shfl_xor_sync(0xffffffffu, l, 2);
 
-    // join the warps: [warp][8][hs + 2] over the rings
+    // join the warps: [warp][8][hs + 8] over the rings (8 more: a row's stores
+    // then fall into other banks than its neighbours')
     __syncthreads();
     float* join = reinterpret_cast<float*>(ring_all);
-    const int w1 = hs + 2;
+    const int w1 = hs + 8;
     {
         float* mine = join + (warp * 8 + r8) * w1;
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
             if (!EXACT && t * 8 >= hs) break;
-            mine[t * 8 + 2 * jj] = o[t][0] + poison;
-            mine[t * 8 + 2 * jj + 1] = o[t][1] + poison;
+            *reinterpret_cast<float2*>(mine + t * 8 + 2 * jj) = make_float2(o[t][0] + poison, o[t][1] + poison);
         }
         if (jj == 0) {
             mine[hs] = m;
@@ -430,20 +430,6 @@ __global__ void __launch_bounds__(kFewThreads) attend_few_kernel(const __grid_co
     __syncthreads();
     const int64_t job = (int64_t)blockIdx.x;
     float* part = a.part + (job * gridDim.y + split) * 8 * w1;
-    // a row's parts src[i], i < n: joined value of dim d, and the row's max and sum
-    auto joined = [&](const float* src, int64_t step, int n, int d, float& mm, float& ll) {
-        mm = -INFINITY;
-        for (int i = 0; i < n; ++i) mm = fmaxf(mm, __ldcg(src + i * step + hs));
-        const float ref = mm == -INFINITY ? 0.0f : mm;
-        float v = 0.0f;
-        ll = 0.0f;
-        for (int i = 0; i < n; ++i) {
-            const float c = exp2_fast(__ldcg(src + i * step + hs) - ref);
-            ll = fmaf(__ldcg(src + i * step + hs + 1), c, ll);
-            v = fmaf(__ldcg(src + i * step + d), c, v);
-        }
-        return v;
-    };
     auto finish = [&](int rr, int d, float v, float mm, float ll) {
         const int row = q.r0 + rr / g, head = h * g + rr % g;
         store_out(a, (int64_t)row * a.ld_out + (int64_t)head * hs + d, v / ll);
@@ -484,19 +470,53 @@ __global__ void __launch_bounds__(kFewThreads) attend_few_kernel(const __grid_co
     __syncthreads();
     if (!last_flag) return;
     __threadfence();
+    // weights of a row's splits (a warp per row), then the weighted sums
     const float* all = a.part + job * gridDim.y * 8 * w1;
+    float* weight = join;  // [8][splits], then [8] maxima and [8] sums
+    float *row_max = weight + 8 * splits, *row_sum = row_max + 8;
+    for (int row8 = warp; row8 < valid; row8 += kFewWarps) {
+        const float* src = all + row8 * w1 + hs;
+        float mm = -INFINITY, ll = 0.0f;
+        for (int i = lane; i < splits; i += 32) {
+            const float v = __ldcg(src + (int64_t)i * 8 * w1);
+            weight[row8 * splits + i] = v;
+            mm = fmaxf(mm, v);
+        }
+        mm = warp_max(mm);
+        const float ref = mm == -INFINITY ? 0.0f : mm;
+        for (int i = lane; i < splits; i += 32) {
+            const float c = exp2_fast(weight[row8 * splits + i] - ref);
+            weight[row8 * splits + i] = c;
+            ll = fmaf(__ldcg(src + (int64_t)i * 8 * w1 + 1), c, ll);
+        }
+        ll = warp_sum(ll);
+        if (lane == 0) {
+            row_max[row8] = mm;
+            row_sum[row8] = ll;
+        }
+    }
+    __syncthreads();
     for (int i = tid; i < valid * hs; i += kFewThreads) {
         const int row8 = i / hs, d = i % hs;
-        float mm, ll;
-        const float v = joined(all + row8 * w1, 8 * w1, splits, d, mm, ll);
-        finish(rt * 8 + row8, d, v, mm, ll);
+        const float *src = all + row8 * w1 + d, *w = weight + row8 * splits;
+        float v = 0.0f;
+        int k = 0;
+        for (; k + 8 <= splits; k += 8) {
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = __ldcg(src + (int64_t)(k + e) * 8 * w1);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v = fmaf(x[e], w[k + e], v);
+        }
+        for (; k < splits; ++k) v = fmaf(__ldcg(src + (int64_t)k * 8 * w1), w[k], v);
+        finish(rt * 8 + row8, d, v, row_max[row8], row_sum[row8]);
     }
 }
 
 template <int ND, int HS, bool EXACT>
 cudaError_t few_launch(const AttArgs& a, dim3 grid, cudaStream_t st) {
     auto kern = attend_few_kernel<ND, HS, EXACT>;
-    constexpr int join = kFewWarps * 8 * (HS + 2) * 4;
+    constexpr int join = kFewWarps * 8 * (HS + 8) * 4;
     constexpr int smem = few_smem<HS>() > join ? few_smem<HS>() : join;
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e == cudaSuccess)
@@ -611,25 +631,25 @@ extern "C" int paged_attention(void* out, int64_t ld_out, const void* q, int64_t
     a.type = type;
     a.scale = scale * kLog2e;
     a.err = c->err;
-    // few rows: every (sequence, kv head, row tile) is cut into splits of the
-    // context until the GPU's CTA slots are filled, 128 tokens at least
+    // few rows: every (sequence, kv head, row tile) is cut into splits of the context
     const int64_t most_rows = (int64_t)batch->max_rows * a.group;
     a.row_tiles = (int)(((most_rows < kFewRows ? most_rows : kFewRows) + 7) / 8);
     if (a.row_tiles < 1) a.row_tiles = 1;
     const int64_t jobs = (int64_t)batch->n_seqs * cache->n_kv_heads * a.row_tiles;
+    // so many that all fit the GPU's CTA slots at once (a second round costs
+    // more than uneven contexts: 16 sequences of the 70B shape 27 us in one, 35 us
+    // in two), 256 tokens at least (two steps of every warp)
     const int64_t slots = 3 * c->num_sms;
     int64_t splits = jobs <= kWsCounters ? slots / jobs : 1;
-    const int64_t most = (batch->max_context + 127) / 128;
-    if (splits > most) splits = most;
     if (splits < 1) splits = 1;
     a.chunk = (int)(((batch->max_context + splits - 1) / splits + 127) / 128 * 128);
-    if (a.chunk < 128) a.chunk = 128;
+    if (a.chunk < 256) a.chunk = 256;
     splits = (batch->max_context + a.chunk - 1) / a.chunk;
     if (splits < 1) splits = 1;
     if (jobs > INT32_MAX) return lq_fail(LQ_EUNSUPPORTED, "paged_attention: %lld (sequence, kv head) pairs", (long long)jobs);
     void* part = nullptr;
     if (splits > 1) {
-        rc = stream_workspace(c, (size_t)jobs * splits * 8 * (cache->head_size + 2) * sizeof(float), &a.cnt, &part);
+        rc = stream_workspace(c, (size_t)jobs * splits * 8 * (cache->head_size + 8) * sizeof(float), &a.cnt, &part);
         if (rc) return rc;
     }
     a.part = static_cast<float*>(part);
