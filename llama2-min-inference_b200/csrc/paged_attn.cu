@@ -19,6 +19,7 @@
 #include "lq_ctx.h"
 #include "lq_paged.cuh"
 #include "lq_paged_host.h"
+#include "lq_tc.cuh"
 #include "lq_types.cuh"
 
 namespace lq {
@@ -60,6 +61,37 @@ __device__ __forceinline__ void store_out(const AttArgs& a, int64_t i, float v) 
     else
         static_cast<__nv_bfloat16*>(a.out)[i] = from_f32<__nv_bfloat16>(v);
 }
+
+// 16 neighbouring outputs x * f + bad
+__device__ __forceinline__ void store_row16(const AttArgs& a, int64_t i, const int (&x)[16], float f, float bad) {
+    float v[16];
+#pragma unroll
+    for (int k = 0; k < 16; ++k) v[k] = fmaf(__int_as_float(x[k]), f, bad);
+    auto put = [&](auto* p) {
+        using T = std::remove_reference_t<decltype(*p)>;
+        if (reinterpret_cast<uintptr_t>(p) % 16 == 0) {
+            constexpr int W = 4 / sizeof(T);
+            uint32_t w[16 / W];
+#pragma unroll
+            for (int k = 0; k < 16 / W; ++k) w[k] = pack_word<T>(v + k * W);
+#pragma unroll
+            for (int k = 0; k < 4 / W; ++k)
+                reinterpret_cast<uint4*>(p)[k] = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+        } else {
+#pragma unroll
+            for (int k = 0; k < 16; ++k) p[k] = from_f32<T>(v[k]);
+        }
+    };
+    if (a.type == LQ_F32)
+        put(static_cast<float*>(a.out) + i);
+    else if (a.type == LQ_F16)
+        put(static_cast<__half*>(a.out) + i);
+    else
+        put(static_cast<__nv_bfloat16*>(a.out) + i);
+}
+
+// 2^k for -126 <= k <= 127
+__device__ __forceinline__ float lq_exp2i(int k) { return __int_as_float((k + 127) << 23); }
 
 __device__ __forceinline__ float exp2_fast(float x) {
     float y;
@@ -547,54 +579,497 @@ cudaError_t few_launch(const AttArgs& a, dim3 grid, cudaStream_t st) {
 }
 
 // ---------------------------------------------------------------------------
-// Many rows per kv head: one warp per (row, head), the cache token by token.
+// Many rows per kv head (prompts): bound by arithmetic, on tcgen05.
+//
+// One CTA per NQ tiles of 128 (token, head) rows of a sequence and kv head,
+// which walk the context together in tiles of TK tokens.  Codes become f16
+// exactly; a row of q is scaled by a power of two to fill f16's range and is
+// one f16 (the 16-bit types) or two (fp32: 22 bits); so are the weights.
+// Products accumulate in fp32 in tensor memory.
+//
+//   warps 0-3, 4-7   softmax of one row tile each: a thread per row reads its
+//                    scores from tensor memory, writes its weights over them
+//                    as the A operand of the second product, 2 x (32 columns
+//                    of scores -> 16 of f16 pairs, the second ones for fp32)
+//   warps 8-11       convert codes: global -> registers (a tile ahead) -> f16 in
+//                    shared memory (128-byte swizzle)
+//   warp 12          issues the MMAs: while one row tile is in softmax, the
+//                    other's products run
+//
+// s_K multiplies scores by 16-token granules (one FMA with the exponent's
+// shift); s_V enters as its logarithm: a weight's exponent gets log2(s_V / max
+// s_V over the context), so O needs no second scaling, and the sum divides it
+// out again per granule.  O is rescaled only when a row's maximum has grown by
+// more than 2^8 since its last one: weights carry 2^6 to stay in f16's range.
 
-__global__ void __launch_bounds__(128) attend_many_kernel(const __grid_constant__ AttArgs a) {
-    const int lane = threadIdx.x & 31;
-    const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-    const int row = (int)(w / a.n_heads), head = (int)(w % a.n_heads);
-    if (row >= a.b.n_rows) return;
-    int s = -1;
-    for (int i = 0; i < a.b.n_seqs && a.b.row_start[i] <= row; ++i) s = i;
-    const int hs = a.c.head_size, P = a.c.page_size, H = a.c.n_kv_heads;
-    const int kvh = head / (a.n_heads / H);
-    int last = -1;
-    if (s >= 0) {
-        const SeqRows q = seq_rows(a.b, s, a.err);
-        if (q.n * a.group <= kFewRows) return;
-        if (row >= q.r0 && row < q.r0 + q.n) last = q.begin + row - q.r0;
+constexpr int kManyWarps = 13;
+constexpr int kManyThreads = 32 * kManyWarps;
+constexpr float kGrow = 8.0f, kUnit = 6.0f;
+
+struct Granule {  // 16 tokens
+    float sk, shift, inv, bad;  // s_K, log2(weight) + kUnit, 1 / (weight * 2^kUnit), NaN where s_V is not finite
+};
+
+struct ManyBars {
+    uint64_t qfull[2], kfull[2], kempty[2], vfull[2], vempty[2], sfull[2], pfull[2], pvdone[2], done;
+    uint32_t tmem_base;
+    int abort_flag;
+    float peak[4];
+    Granule gran[4][8];  // by tile, four deep
+    float fs[256];       // rows' factors of the scores
+};
+
+template <int HS, int PARTS, int NQ, int TK, int NB>
+struct ManyLayout {
+    static constexpr int kQ = 128 * HS * 2 * PARTS;        // one row tile: [part][64 dims][128][128 bytes]
+    static constexpr int kK = TK * HS * 2, kV = TK * HS * 2;
+    static constexpr int kSmem = 1024 + NQ * kQ + NB * (kK + kV) + (int)sizeof(ManyBars);
+    static_assert(kSmem <= 227 * 1024 && HS % 64 == 0, "shared memory");
+    static_assert(NQ * (TK + HS) <= 512, "tensor memory");
+};
+
+// 4 codes to 2 x 2 halves: bytes + 128 as the low mantissa of 1024, minus 1152
+__device__ __forceinline__ uint2 codes_f16(uint32_t w) {
+    w ^= 0x80808080u;
+    const uint32_t lo = __byte_perm(w, 0x64646464u, 0x4140), hi = __byte_perm(w, 0x64646464u, 0x4342);
+    const __half2 off = __floats2half2_rn(1152.0f, 1152.0f);
+    const __half2 a = __hsub2(*reinterpret_cast<const __half2*>(&lo), off);
+    const __half2 b = __hsub2(*reinterpret_cast<const __half2*>(&hi), off);
+    return make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+}
+
+template <int HS, int PARTS, int NQ, int TK, int NB>
+__global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const __grid_constant__ AttArgs a) {
+    using Lay = ManyLayout<HS, PARTS, NQ, TK, NB>;
+    constexpr int kPieces = HS / 16;  // 16-byte pieces of K (and of V) per converting thread and 128 tokens
+    constexpr int kLoads = kPieces * TK / 128;
+    extern __shared__ __align__(1024) unsigned char raw[];
+    unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+    unsigned char *sq = sm, *sk = sq + NQ * Lay::kQ, *sv = sk + NB * Lay::kK;
+    ManyBars* bars = reinterpret_cast<ManyBars*>(sv + NB * Lay::kV);
+    volatile int* abort_flag = &bars->abort_flag;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int hs = a.c.head_size, P = a.c.page_size, H = a.c.n_kv_heads, g = a.group;
+    const int tile = gridDim.x - 1 - blockIdx.x;  // long ones first
+    const int h = blockIdx.y, s = blockIdx.z;
+
+    pdl_trigger();
+    pdl_wait();
+    const SeqRows q = seq_rows(a.b, s, nullptr);
+    const int rows = q.n * g, base_row = tile * NQ * 128;
+    if (rows <= kFewRows || base_row >= rows) return;
+    int n[NQ];  // token tiles that each row tile sees
+#pragma unroll
+    for (int i = 0; i < NQ; ++i) {
+        const int lo = base_row + i * 128, hi = min(rows, lo + 128) - 1;
+        n[i] = lo < rows ? (q.begin + hi / g) / TK + 1 : 0;
     }
-    if (last < 0) return;
-    float qv[8], o[8] = {};
-    for (int j = 0; j < 8; ++j)
-        qv[j] = lane + 32 * j < hs ? load_q(a, row * a.ld_q + (int64_t)head * hs + lane + 32 * j) : 0.0f;
-    float m = -INFINITY, l = 0.0f;
-    for (int t = 0; t <= last; ++t) {
-        const int64_t page = page_of(a.c, a.b, s, t / P, a.err);
-        if (page < 0) continue;
-        const int64_t cell = page * H + kvh;
-        const int8_t* kc = static_cast<const int8_t*>(a.c.codes) + cell * 2 * hs * P;
-        const int8_t* vc = kc + (int64_t)hs * P;
-        const float sk = a.c.scales[cell * 2], sv = a.c.scales[cell * 2 + 1];
-        const int u = t % P;
-        float d = 0.0f;
-        for (int j = 0; j < 8; ++j) {
-            const int e = lane + 32 * j;
-            if (e < hs) d += qv[j] * (float)kc[((int64_t)(e / 16) * P + u) * 16 + e % 16];
+    int tiles = n[0];
+    if (NQ == 2 && n[NQ - 1] > tiles) tiles = n[NQ - 1];
+    const int seen = q.begin + (min(rows, base_row + NQ * 128) - 1) / g + 1;
+
+    if (tid == 0) {
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&bars->qfull[i], 4);
+            mbar_init(&bars->kfull[i], 4);
+            mbar_init(&bars->vfull[i], 4);
+            mbar_init(&bars->kempty[i], 1);
+            mbar_init(&bars->vempty[i], 1);
+            mbar_init(&bars->sfull[i], 1);
+            mbar_init(&bars->pfull[i], 4);
+            mbar_init(&bars->pvdone[i], 1);
         }
-        d = warp_sum(d) * (sk * a.scale * kLn2);
-        const float mn = fmaxf(m, d);
-        const float c = m == -INFINITY ? 0.0f : expf(m - mn), p = d != d ? d : expf(d - mn);
-        l = l * c + p;
-        for (int j = 0; j < 8; ++j) {
-            const int e = lane + 32 * j;
-            if (e < hs) o[j] = o[j] * c + p * sv * (float)vc[((int64_t)(u / 16) * hs + e) * 16 + u % 16];
-        }
-        m = mn;
+        mbar_init(&bars->done, 1);
+        bars->abort_flag = 0;
+        fence_mbar_init();
     }
-    for (int j = 0; j < 8; ++j)
-        if (lane + 32 * j < hs) store_out(a, row * a.ld_out + (int64_t)head * hs + lane + 32 * j, o[j] / l);
-    if (a.lse && lane == 0) a.lse[(int64_t)row * a.n_heads + head] = m + logf(l);
+    if (warp == 12) tmem_alloc<1, 512>(&bars->tmem_base);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = bars->tmem_base;
+    const int8_t* codes = static_cast<const int8_t*>(a.c.codes);
+    const int64_t cell = (int64_t)hs * P * 2;
+
+    if (warp >= 8 && warp < 12) {
+        // ---------------- conversion ----------------
+        const int t = tid - 256;  // 0..127
+        int* const err = a.err;
+        // the largest finite s_V of the context
+        uint32_t pk = 0;
+        for (int lp = t; lp * P < seen; lp += 128) {
+            const int64_t p = page_of(a.c, a.b, s, lp, err);
+            if (p < 0) continue;
+            const uint32_t v = abs_bits(__ldg(a.c.scales + (p * H + h) * 2 + 1));
+            if (v < kInfBits) pk = max(pk, v);
+        }
+        pk = __reduce_max_sync(0xffffffffu, pk);
+        if (lane == 0) bars->peak[warp - 8] = __uint_as_float(pk);
+        named_bar_sync(1, 128);
+        float svm = fmaxf(fmaxf(bars->peak[0], bars->peak[1]), fmaxf(bars->peak[2], bars->peak[3]));
+        if (svm == 0.0f) svm = 1.0f;
+        uint4 kr[kLoads], vr[kLoads];
+        // K: token t (two per thread for TK of 64: half the dims each)
+        const int kt = TK == 128 ? t : t & 63, kc0 = TK == 128 ? 0 : (t >> 6);
+        constexpr int kcs = TK == 128 ? 1 : 2;
+        float sc_k = 0.0f, sc_v = 0.0f;  // of the token's page, for the granule table
+        auto page_at = [&](int tok) -> int64_t { return tok < seen ? page_of(a.c, a.b, s, tok / P, err) : -1; };
+        auto load_k = [&](int j) {
+            const int tok = j * TK + kt;
+            const int64_t p = page_at(tok);
+            const uint4* src = reinterpret_cast<const uint4*>(codes + (p * H + h) * cell) + tok % P;
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                const int c = kc0 + i * kcs;
+                kr[i] = p >= 0 && c * 16 < hs ? __ldg(src + (int64_t)c * P) : make_uint4(0, 0, 0, 0);
+            }
+            sc_k = sc_v = NAN;
+            if (p >= 0 && kt % 16 == 0) {
+                const float2 v = __ldg(reinterpret_cast<const float2*>(a.c.scales) + p * H + h);
+                sc_k = v.x;
+                sc_v = v.y;
+            }
+        };
+        auto load_v = [&](int j) {
+            int tc = t / hs, d = t % hs;  // the tile's piece t, t + 128, ...: 16 tokens of dim d
+            int at = -1;
+            int64_t p = -1;
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                if (tc < TK / 16) {
+                    const int tok = j * TK + tc * 16;
+                    if (tc != at) {
+                        at = tc;
+                        p = page_at(tok);
+                    }
+                    vr[i] = p >= 0 ? __ldg(reinterpret_cast<const uint4*>(codes + (p * H + h) * cell + hs * P) +
+                                           tok % P / 16 * hs + d)
+                                   : make_uint4(0, 0, 0, 0);
+                }
+                d += 128;
+                while (d >= hs) {
+                    d -= hs;
+                    ++tc;
+                }
+            }
+        };
+        // 16 codes to two 16-byte chunks of row `row`, chunk pair `cc` of a 128-byte row
+        auto put = [&](unsigned char* block, int row, int cc, uint4 w) {
+            const uint2 x = codes_f16(w.x), y = codes_f16(w.y), z = codes_f16(w.z), u = codes_f16(w.w);
+            unsigned char* r = block + row * 128;
+            *reinterpret_cast<uint4*>(r + (((2 * cc) ^ (row & 7)) << 4)) = make_uint4(x.x, x.y, y.x, y.y);
+            *reinterpret_cast<uint4*>(r + (((2 * cc + 1) ^ (row & 7)) << 4)) = make_uint4(z.x, z.y, u.x, u.y);
+        };
+        load_k(0);
+        load_v(0);
+        for (int j = 0; j < tiles; ++j) {
+            const int buf = j % NB;
+            const uint32_t par = (uint32_t)((j / NB) & 1);
+            if (!__all_sync(0xffffffffu, qwait(&bars->kempty[buf], par ^ 1u, a.err, DEV_TIMEOUT_EMPTY, abort_flag))) break;
+            unsigned char* kb = sk + buf * Lay::kK;
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                const int c = kc0 + i * kcs;
+                if (c * 16 < hs) put(kb + (c >> 2) * (TK * 128), kt, c & 3, kr[i]);
+            }
+            if (kt % 16 == 0 && kc0 == 0) {
+                Granule& gr = bars->gran[j & 3][kt / 16];
+                const bool fine = sc_v < INFINITY;
+                const float w = fine ? fmaxf(sc_v / svm, 9.094947e-13f) : 1.0f;  // 2^-40 at least
+                const float sh = log2f(w) + kUnit;
+                gr.sk = sc_k;
+                gr.shift = sh;
+                gr.inv = exp2f(-sh);
+                gr.bad = fine ? 0.0f : NAN;
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars->kfull[buf]);
+            if (j + 1 < tiles) load_k(j + 1);
+            if (!__all_sync(0xffffffffu, qwait(&bars->vempty[buf], par ^ 1u, a.err, DEV_TIMEOUT_EMPTY, abort_flag))) break;
+            unsigned char* vb = sv + buf * Lay::kV;
+            int tc = t / hs, d = t % hs;
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                if (tc < TK / 16) put(vb + (tc >> 2) * (hs * 128), d, tc & 3, vr[i]);
+                d += 128;
+                while (d >= hs) {
+                    d -= hs;
+                    ++tc;
+                }
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars->vfull[buf]);
+            if (j + 1 < tiles) load_v(j + 1);
+        }
+    } else if (warp == 12) {
+        // ---------------- MMA issue ----------------
+        const uint32_t id_s = (1u << 4) | ((uint32_t)(TK >> 3) << 17) | (8u << 24);  // f32 += f16 x f16, M 128
+        const uint32_t id_o = (1u << 4) | ((uint32_t)(hs >> 3) << 17) | (8u << 24);
+        const uint64_t dq = smem_desc_sw128(smem_addr(sq)), dk = smem_desc_sw128(smem_addr(sk)),
+                       dv = smem_desc_sw128(smem_addr(sv));
+        const int steps = hs / 16;
+        bool ok = true;
+        auto wait = [&](uint64_t* bar, uint32_t parity, int code) {
+            ok = ok && __all_sync(0xffffffffu, qwait(bar, parity, a.err, code, abort_flag));
+        };
+        auto scores = [&](int i, int j) {  // row tile i, token tile j
+            wait(&bars->kfull[j % NB], (uint32_t)((j / NB) & 1), DEV_TIMEOUT_FULL);
+            if (!ok) return;
+            tc_fence_after();
+            if (elect_one()) {
+                const uint32_t dst = tmem + i * TK;
+                const uint64_t kd = dk + (uint32_t)((j % NB) * Lay::kK >> 4);
+#pragma unroll
+                for (int p = 0; p < PARTS; ++p) {
+                    const uint64_t qd = dq + (uint32_t)((i * Lay::kQ + p * (Lay::kQ / PARTS)) >> 4);
+                    for (int k = 0; k < steps; ++k)  // 64 dims a block of 128-byte rows, 32 bytes a step
+                        mma_f16(dst, qd + (uint32_t)((k >> 2) * (128 * 128) >> 4) + 2 * (k & 3),
+                                kd + (uint32_t)((k >> 2) * (TK * 128) >> 4) + 2 * (k & 3), id_s, k > 0 || p > 0);
+                }
+                mma_commit(&bars->sfull[i]);
+                if (i == NQ - 1 || j >= n[NQ - 1]) mma_commit(&bars->kempty[j % NB]);
+            }
+            __syncwarp();
+        };
+#pragma unroll
+        for (int i = 0; i < NQ; ++i)
+            if (n[i] > 0) {
+                wait(&bars->qfull[i], 0, DEV_TIMEOUT_FULL);
+                if (ok) scores(i, 0);
+            }
+        for (int j = 0; ok && j < tiles; ++j) {
+#pragma unroll
+            for (int i = 0; i < NQ; ++i) {
+                if (!ok || j >= n[i]) continue;
+                wait(&bars->pfull[i], (uint32_t)(j & 1), DEV_TIMEOUT_FULL);
+                wait(&bars->vfull[j % NB], (uint32_t)((j / NB) & 1), DEV_TIMEOUT_FULL);
+                if (!ok) break;
+                tc_fence_after();
+                if (elect_one()) {
+                    const uint32_t dst = tmem + NQ * TK + i * HS, src = tmem + i * TK;
+                    const uint64_t vd = dv + (uint32_t)((j % NB) * Lay::kV >> 4);
+#pragma unroll
+                    for (int k = 0; k < TK / 16; ++k)
+#pragma unroll
+                        for (int p = 0; p < PARTS; ++p)
+                            mma_f16_ts(dst, src + (k >> 1) * 32 + p * 16 + (k & 1) * 8,
+                                       vd + (uint32_t)((k >> 2) * (hs * 128) >> 4) + 2 * (k & 3), id_o,
+                                       j > 0 || k > 0 || p > 0);
+                    mma_commit(&bars->pvdone[i]);
+                    if (i == NQ - 1 || j >= n[NQ - 1]) mma_commit(&bars->vempty[j % NB]);
+                }
+                __syncwarp();
+                if (j + 1 < n[i]) scores(i, j + 1);
+            }
+        }
+        if (elect_one()) mma_commit(&bars->done);
+        __syncwarp();
+        mbar_wait(&bars->done, 0, a.err, DEV_TIMEOUT_MMA);  // every MMA is done before the memory is freed
+    } else if (warp < 4 * NQ && n[warp >> 2] > 0) {
+        // ---------------- softmax ----------------
+        const int i = warp >> 2, w4 = warp & 3;
+        const int n_i = i == 0 ? n[0] : n[NQ - 1];
+        // q of this warp's 32 rows, a row at a time: 4 dims a lane
+        for (int rr = 0; rr < 32; ++rr) {
+            const int row = w4 * 32 + rr, r = base_row + i * 128 + row;
+            const bool have = r < rows;
+            const int64_t at = have ? (int64_t)(q.r0 + r / g) * a.ld_q + (int64_t)(h * g + r % g) * hs : 0;
+            float x[(HS + 127) / 128][4];
+            uint32_t m = 0;
+#pragma unroll
+            for (int b = 0; b < (HS + 127) / 128; ++b)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int d = b * 128 + lane * 4 + e;
+                    x[b][e] = have && d < hs ? load_q(a, at + d) : 0.0f;
+                    m = max(m, abs_bits(x[b][e]));
+                }
+            m = __reduce_max_sync(0xffffffffu, m);
+            // a power of two that takes the largest into [2^13, 2^14)
+            int ex = (int)(m >> 23) - 127;
+            ex = max(-114, min(100, 13 - ex));
+            const float up = a.scale < 0.0f ? -lq_exp2i(ex) : lq_exp2i(ex);
+            if (lane == 0)
+                bars->fs[i * 128 + row] = m >= kInfBits ? NAN : fabsf(a.scale) * lq_exp2i(-ex);
+#pragma unroll
+            for (int b = 0; b < (HS + 127) / 128; ++b) {
+                const int d = b * 128 + lane * 4;
+                if (d >= hs) continue;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[b][e] = m >= kInfBits ? 0.0f : x[b][e] * up;
+#pragma unroll
+                for (int p = 0; p < PARTS; ++p) {
+                    const __half2 u = __floats2half2_rn(x[b][0], x[b][1]), v = __floats2half2_rn(x[b][2], x[b][3]);
+                    unsigned char* dst = sq + i * Lay::kQ + p * (Lay::kQ / PARTS) + (d >> 6) * (128 * 128) + row * 128 +
+                                         ((((d & 63) >> 3) ^ (row & 7)) << 4) + (d & 4) * 2;
+                    *reinterpret_cast<uint2*>(dst) =
+                        make_uint2(*reinterpret_cast<const uint32_t*>(&u), *reinterpret_cast<const uint32_t*>(&v));
+                    const float2 fu = __half22float2(u), fv = __half22float2(v);
+                    x[b][0] -= fu.x;
+                    x[b][1] -= fu.y;
+                    x[b][2] -= fv.x;
+                    x[b][3] -= fv.y;
+                }
+            }
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->qfull[i]);
+
+        const int row = w4 * 32 + lane, r = base_row + i * 128 + row;
+        const int pos = r < rows ? q.begin + r / g : -1;
+        const float fs = bars->fs[i * 128 + row];
+        const uint32_t ts = tmem + ((uint32_t)(w4 * 32) << 16) + i * TK;
+        const uint32_t to = tmem + ((uint32_t)(w4 * 32) << 16) + NQ * TK + i * HS;
+        float mref = 0.0f, l = 0.0f, poison = 0.0f;
+        bool ok = true;
+        for (int j = 0; j < n_i; ++j) {
+            ok = __all_sync(0xffffffffu, qwait(&bars->sfull[i], (uint32_t)(j & 1), a.err, DEV_TIMEOUT_TFULL, abort_flag));
+            if (!ok) break;
+            tc_fence_after();
+            const Granule* gr = bars->gran[j & 3];
+            const int left = pos - j * TK;  // the tile's last token that this row sees
+            const bool masked = __any_sync(0xffffffffu, left < TK - 1);
+            float m = -INFINITY;
+            int x[32];
+#pragma unroll
+            for (int c = 0; c < TK / 32; ++c) {
+                tmem_ld<32>(ts + c * 32, x);
+                tmem_ld_wait();
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float mx = -INFINITY;
+                    if (masked) {
+#pragma unroll
+                        for (int k = 0; k < 16; ++k)
+                            mx = fmaxf(mx, c * 32 + e * 16 + k <= left ? __int_as_float(x[e * 16 + k]) : -INFINITY);
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < 16; ++k) mx = fmaxf(mx, __int_as_float(x[e * 16 + k]));
+                    }
+                    m = fmaxf(m, mx * (fs * gr[2 * c + e].sk));
+                }
+            }
+            const bool grown = j == 0 ? m > -INFINITY : m > mref + kGrow;
+            if (__any_sync(0xffffffffu, grown)) {
+                const float next = grown ? m : mref;
+                const float f = exp2_fast(mref - next);
+                mref = next;
+                if (j > 0) {
+                    l *= f;
+                    ok = __all_sync(0xffffffffu, qwait(&bars->pvdone[i], (uint32_t)((j - 1) & 1), a.err, DEV_TIMEOUT_TFULL,
+                                                       abort_flag));
+                    if (!ok) break;
+                    tc_fence_after();
+                    for (int c = 0; c < hs; c += 16) {
+                        int y[16];
+                        tmem_ld<16>(to + c, y);
+                        tmem_ld_wait();
+                        uint32_t z[16];
+#pragma unroll
+                        for (int k = 0; k < 16; ++k) z[k] = __float_as_uint(__int_as_float(y[k]) * f);
+                        tmem_st16(to + c, z);
+                    }
+                }
+            }
+#pragma unroll
+            for (int c = 0; c < TK / 32; ++c) {
+                tmem_ld<32>(ts + c * 32, x);
+                tmem_ld_wait();
+                uint32_t hi[16], lo[16];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const Granule gg = gr[2 * c + e];
+                    const float f = fs * gg.sk, b = gg.shift - mref;
+                    if (c * 32 + e * 16 <= left) poison += gg.bad;
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int k = 0; k < 16; k += 2) {
+                        float p0 = exp2_fast(fmaf(__int_as_float(x[e * 16 + k]), f, b));
+                        float p1 = exp2_fast(fmaf(__int_as_float(x[e * 16 + k + 1]), f, b));
+                        if (masked) {
+                            if (c * 32 + e * 16 + k > left) p0 = 0.0f;
+                            if (c * 32 + e * 16 + k + 1 > left) p1 = 0.0f;
+                        }
+                        sum += p0;
+                        sum += p1;
+                        const __half2 u = __floats2half2_rn(p0, p1);
+                        hi[e * 8 + k / 2] = *reinterpret_cast<const uint32_t*>(&u);
+                        if (PARTS == 2) {
+                            const float2 fu = __half22float2(u);
+                            const __half2 v = __floats2half2_rn(p0 - fu.x, p1 - fu.y);
+                            lo[e * 8 + k / 2] = *reinterpret_cast<const uint32_t*>(&v);
+                        }
+                    }
+                    l = fmaf(sum, gg.inv, l);
+                }
+                tmem_st16(ts + c * 32, hi);
+                if (PARTS == 2) tmem_st16(ts + c * 32 + 16, lo);
+            }
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars->pfull[i]);
+        }
+        if (ok)
+            ok = __all_sync(0xffffffffu, qwait(&bars->pvdone[i], (uint32_t)((n_i - 1) & 1), a.err, DEV_TIMEOUT_TFULL, abort_flag));
+        tc_fence_after();
+        if (ok) {
+            const float svm = [&] {
+                const float v = fmaxf(fmaxf(bars->peak[0], bars->peak[1]), fmaxf(bars->peak[2], bars->peak[3]));
+                return v == 0.0f ? 1.0f : v;
+            }();
+            const float f = svm * (1.0f / 64.0f) / l;  // 2^-kUnit
+            const int64_t at = (int64_t)(q.r0 + r / g) * a.ld_out + (int64_t)(h * g + r % g) * hs;
+            for (int c = 0; c < hs; c += 16) {
+                int y[16];
+                tmem_ld<16>(to + c, y);
+                tmem_ld_wait();
+                if (r < rows) store_row16(a, at + c, y, f, poison);
+            }
+            if (a.lse && r < rows)
+                a.lse[(int64_t)(q.r0 + r / g) * a.n_heads + h * g + r % g] = (mref + log2f(l)) * kLn2;
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 12) {
+        tc_fence_after();
+        tmem_free<1, 512>(tmem);
+    }
+}
+
+template <int HS, int PARTS, int NQ, int TK, int NB>
+cudaError_t many_launch_t(const AttArgs& a, cudaStream_t st) {
+    using Lay = ManyLayout<HS, PARTS, NQ, TK, NB>;
+    auto kern = attend_many_kernel<HS, PARTS, NQ, TK, NB>;
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Lay::kSmem);
+    if (e != cudaSuccess) return e;
+    const int64_t x = ((int64_t)a.b.max_rows * a.group + NQ * 128 - 1) / (NQ * 128);
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)x, (unsigned)a.c.n_kv_heads, (unsigned)a.b.n_seqs);
+    cfg.blockDim = dim3(kManyThreads);
+    cfg.dynamicSmemBytes = Lay::kSmem;
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kern, a);
+}
+
+cudaError_t many_launch(const AttArgs& a, cudaStream_t st) {
+    const int hs = a.c.head_size;
+    if (a.type == LQ_F32)
+        return hs <= 64    ? many_launch_t<64, 2, 2, 128, 2>(a, st)
+               : hs <= 128 ? many_launch_t<128, 2, 2, 128, 1>(a, st)
+                           : many_launch_t<256, 2, 1, 64, 1>(a, st);
+    return hs <= 64    ? many_launch_t<64, 1, 2, 128, 2>(a, st)
+           : hs <= 128 ? many_launch_t<128, 1, 2, 128, 2>(a, st)
+                       : many_launch_t<256, 1, 1, 128, 1>(a, st);
 }
 
 }  // namespace
@@ -657,10 +1132,7 @@ extern "C" int paged_attention(void* out, int64_t ld_out, const void* q, int64_t
     cudaError_t e = type == LQ_F32 ? few_launch<3>(a, grid, stream()) : few_launch<2>(a, grid, stream());
     if (e != cudaSuccess) return cuda_fail(e, "paged_attention launch");
     if (most_rows > kFewRows) {
-        const int64_t blocks = ((int64_t)batch->n_rows * n_heads + 3) / 4;
-        if (blocks > INT32_MAX) return lq_fail(LQ_EUNSUPPORTED, "paged_attention: too many rows and heads");
-        attend_many_kernel<<<(unsigned)blocks, 128, 0, stream()>>>(a);
-        e = cudaGetLastError();
+        e = many_launch(a, stream());
         if (e != cudaSuccess) return cuda_fail(e, "paged_attention launch");
     }
     return LQ_OK;
