@@ -39,6 +39,8 @@ struct AttArgs {
     float* lse;
     int64_t ld_q, ld_out;
     int n_heads, group, type;
+    int q_vec;        // 4 elements of q are one aligned load
+    int few_rows;     // (token, head) rows of a sequence and kv head that the first kernel takes
     float scale;      // log2(e) times the caller's
     int row_tiles;    // tiles of 8 (token, head) rows of a sequence and kv head
     int chunk;        // tokens per split
@@ -47,11 +49,44 @@ struct AttArgs {
     int* err;
 };
 
-__device__ __forceinline__ float load_q(const AttArgs& a, int64_t i) {
-    if (a.type == LQ_F32) return static_cast<const float*>(a.q)[i];
-    if (a.type == LQ_F16) return to_f32(static_cast<const __half*>(a.q)[i]);
-    return to_f32(static_cast<const __nv_bfloat16*>(a.q)[i]);
-}
+// four neighbouring elements of q as they lie: fp32 (PARTS 2) or 16-bit
+template <int PARTS>
+struct RawQ {
+    uint32_t w[2 * PARTS];
+    __device__ __forceinline__ void load(const AttArgs& a, int64_t i) {
+        if constexpr (PARTS == 2) {
+            const float* p = static_cast<const float*>(a.q) + i;
+            if (a.q_vec) {
+                const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
+                w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[e] = __float_as_uint(__ldg(p + e));
+            }
+        } else {
+            const uint16_t* p = static_cast<const uint16_t*>(a.q) + i;
+            if (a.q_vec) {
+                const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
+                w[0] = v.x, w[1] = v.y;
+            } else {
+                w[0] = __ldg(p) | (uint32_t)__ldg(p + 1) << 16;
+                w[1] = __ldg(p + 2) | (uint32_t)__ldg(p + 3) << 16;
+            }
+        }
+    }
+    __device__ __forceinline__ void get(const AttArgs& a, float (&v)[4]) const {
+        if constexpr (PARTS == 2) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = __uint_as_float(w[e]);
+        } else if (a.type == LQ_F16) {
+            unpack_word<__half>(w[0], v);
+            unpack_word<__half>(w[1], v + 2);
+        } else {
+            unpack_word<__nv_bfloat16>(w[0], v);
+            unpack_word<__nv_bfloat16>(w[1], v + 2);
+        }
+    }
+};
 
 __device__ __forceinline__ void store_out(const AttArgs& a, int64_t i, float v) {
     if (a.type == LQ_F32)
@@ -88,6 +123,26 @@ __device__ __forceinline__ void store_row16(const AttArgs& a, int64_t i, const i
         put(static_cast<__half*>(a.out) + i);
     else
         put(static_cast<__nv_bfloat16*>(a.out) + i);
+}
+
+// the outputs of a sequence's rows that attend to nothing, for one kv head
+__device__ __forceinline__ void zero_rows(const AttArgs& a, const SeqRows& q, int h) {
+    const int hs = a.c.head_size, w = a.group * hs;
+    for (int64_t i = threadIdx.x; i < (int64_t)(q.r0 - q.first) * w; i += blockDim.x) {
+        const int64_t row = q.first + i / w;
+        const int d = (int)(i % w);
+        store_out(a, row * a.ld_out + (int64_t)h * w + d, 0.0f);
+        if (a.lse && d % hs == 0) a.lse[row * a.n_heads + h * a.group + d / hs] = -INFINITY;
+    }
+}
+
+template <int N>
+__device__ __forceinline__ void regs_up() {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void regs_down() {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 
 // 2^k for -126 <= k <= 127
@@ -170,15 +225,9 @@ __global__ void __launch_bounds__(kFewThreads, HS <= 128 ? 3 : 1) attend_few_ker
     pdl_trigger();
     pdl_wait();
     const SeqRows q = seq_rows(a.b, s, split == 0 && rt == 0 && h == 0 && tid == 0 ? a.err : nullptr);
-    if (split == 0 && rt == 0) {  // rows that attend to nothing
-        for (int i = tid; i < (q.r0 - q.first) * g * hs; i += kFewThreads) {
-            const int row = q.first + i / (g * hs), d = i % (g * hs);
-            store_out(a, (int64_t)row * a.ld_out + (int64_t)h * g * hs + d, 0.0f);
-            if (a.lse && d % hs == 0) a.lse[(int64_t)row * a.n_heads + h * g + d / hs] = -INFINITY;
-        }
-    }
+    if (split == 0 && rt == 0) zero_rows(a, q, h);
     const int rows = q.n * g;
-    if (rows > kFewRows || rt * 8 >= rows) return;
+    if (rows > a.few_rows || rt * 8 >= rows) return;
     const int top = min(rows, rt * 8 + 8) - 1;            // the tile's last row
     const int seen = q.begin + top / g + 1;               // tokens that it sees
     const int splits = (seen + a.chunk - 1) / a.chunk;
@@ -243,13 +292,18 @@ __global__ void __launch_bounds__(kFewThreads, HS <= 128 ? 3 : 1) attend_few_ker
         float x[(HS + 127) / 128][4];
         uint32_t m = 0;
 #pragma unroll
-        for (int b = 0; b < (HS + 127) / 128; ++b)
+        for (int b = 0; b < (HS + 127) / 128; ++b) {
+            const int d = b * 128 + lane * 4;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int d = b * 128 + lane * 4 + e;
-                x[b][e] = have && d < hs ? load_q(a, base + d) : 0.0f;
-                m = max(m, abs_bits(x[b][e]));
+            for (int e = 0; e < 4; ++e) x[b][e] = 0.0f;
+            if (have && d < hs) {
+                RawQ<ND - 1> raw;
+                raw.load(a, base + d);
+                raw.get(a, x[b]);
             }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) m = max(m, abs_bits(x[b][e]));
+        }
         m = __reduce_max_sync(0xffffffffu, m);
         constexpr float kTop = ND == 3 ? 8323072.0f : 32512.0f;  // 127 * 256^(ND - 1)
         const float peak = __uint_as_float(m);
@@ -595,6 +649,7 @@ cudaError_t few_launch(const AttArgs& a, dim3 grid, cudaStream_t st) {
 //                    shared memory (128-byte swizzle)
 //   warp 12          issues the MMAs: while one row tile is in softmax, the
 //                    other's products run
+//   warp 13          looks up pages and scales, up to four tiles ahead
 //
 // s_K multiplies scores by 16-token granules (one FMA with the exponent's
 // shift); s_V enters as its logarithm: a weight's exponent gets log2(s_V / max
@@ -602,7 +657,7 @@ cudaError_t few_launch(const AttArgs& a, dim3 grid, cudaStream_t st) {
 // out again per granule.  O is rescaled only when a row's maximum has grown by
 // more than 2^8 since its last one: weights carry 2^6 to stay in f16's range.
 
-constexpr int kManyWarps = 13;
+constexpr int kManyWarps = 16;  // the last two idle: registers are dealt to warpgroups
 constexpr int kManyThreads = 32 * kManyWarps;
 constexpr float kGrow = 8.0f, kUnit = 6.0f;
 
@@ -612,10 +667,12 @@ struct Granule {  // 16 tokens
 
 struct ManyBars {
     uint64_t qfull[2], kfull[2], kempty[2], vfull[2], vempty[2], sfull[2], pfull[2], pvdone[2], done;
+    uint64_t tabfull[4], tabempty[4];
     uint32_t tmem_base;
     int abort_flag;
-    float peak[4];
+    uint32_t peak;       // bits of the largest finite s_V of the context
     Granule gran[4][8];  // by tile, four deep
+    int64_t cell[4][8];  // the granules' pages: byte offset of the head's codes, or -1
     float fs[256];       // rows' factors of the scores
 };
 
@@ -655,9 +712,10 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const __gr
 
     pdl_trigger();
     pdl_wait();
-    const SeqRows q = seq_rows(a.b, s, nullptr);
+    const SeqRows q = seq_rows(a.b, s, a.few_rows == 0 && tile == 0 && h == 0 && tid == 0 ? a.err : nullptr);
     const int rows = q.n * g, base_row = tile * NQ * 128;
-    if (rows <= kFewRows || base_row >= rows) return;
+    if (a.few_rows == 0 && tile == 0) zero_rows(a, q, h);
+    if (rows <= a.few_rows || base_row >= rows) return;
     int n[NQ];  // token tiles that each row tile sees
 #pragma unroll
     for (int i = 0; i < NQ; ++i) {
@@ -679,78 +737,70 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const __gr
             mbar_init(&bars->pfull[i], 4);
             mbar_init(&bars->pvdone[i], 1);
         }
+        for (int i = 0; i < 4; ++i) {
+            mbar_init(&bars->tabfull[i], 1);
+            mbar_init(&bars->tabempty[i], 1);
+        }
         mbar_init(&bars->done, 1);
         bars->abort_flag = 0;
+        bars->peak = 0;
         fence_mbar_init();
     }
     if (warp == 12) tmem_alloc<1, 512>(&bars->tmem_base);
+    const int lp2 = __ffs(P) - 1;
+    const int32_t* pages = a.b.pages + (int64_t)s * a.b.max_pages;
+    uint32_t pk = 0;
+    for (int lp = tid; lp << lp2 < seen && lp < a.b.max_pages; lp += kManyThreads) {
+        const int p = __ldg(pages + lp);
+        if (p < 0 || p >= a.c.n_pages) continue;  // reported below
+        const uint32_t v = abs_bits(__ldg(a.c.scales + ((int64_t)p * H + h) * 2 + 1));
+        if (v < kInfBits) pk = max(pk, v);
+    }
+    pk = __reduce_max_sync(0xffffffffu, pk);
     tc_fence_before();
+    __syncthreads();
+    if (lane == 0 && pk) atomicMax(&bars->peak, pk);
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = bars->tmem_base;
+    const float svm = bars->peak ? __uint_as_float(bars->peak) : 1.0f;
     const int8_t* codes = static_cast<const int8_t*>(a.c.codes);
-    const int64_t cell = (int64_t)hs * P * 2;
 
+    // 512 threads hold 65536 registers: 2 x 128 x 168 + 128 x 104 + 128 x 72
     if (warp >= 8 && warp < 12) {
         // ---------------- conversion ----------------
+        regs_down<104>();
         const int t = tid - 256;  // 0..127
-        int* const err = a.err;
-        // the largest finite s_V of the context
-        uint32_t pk = 0;
-        for (int lp = t; lp * P < seen; lp += 128) {
-            const int64_t p = page_of(a.c, a.b, s, lp, err);
-            if (p < 0) continue;
-            const uint32_t v = abs_bits(__ldg(a.c.scales + (p * H + h) * 2 + 1));
-            if (v < kInfBits) pk = max(pk, v);
-        }
-        pk = __reduce_max_sync(0xffffffffu, pk);
-        if (lane == 0) bars->peak[warp - 8] = __uint_as_float(pk);
-        named_bar_sync(1, 128);
-        float svm = fmaxf(fmaxf(bars->peak[0], bars->peak[1]), fmaxf(bars->peak[2], bars->peak[3]));
-        if (svm == 0.0f) svm = 1.0f;
         uint4 kr[kLoads], vr[kLoads];
-        // K: token t (two per thread for TK of 64: half the dims each)
+        // K: token t (two threads a token for TK of 64, half the dims each)
         const int kt = TK == 128 ? t : t & 63, kc0 = TK == 128 ? 0 : (t >> 6);
         constexpr int kcs = TK == 128 ? 1 : 2;
-        float sc_k = 0.0f, sc_v = 0.0f;  // of the token's page, for the granule table
-        auto page_at = [&](int tok) -> int64_t { return tok < seen ? page_of(a.c, a.b, s, tok / P, err) : -1; };
+        // V: the tile's pieces t, t + 128, ...: piece tc * hs + d is 16 tokens of dim d
+        int pd[kLoads], ptc[kLoads];
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            ptc[i] = (t + 128 * i) / hs;
+            pd[i] = (t + 128 * i) - ptc[i] * hs;
+        }
+        bool ok = true;
         auto load_k = [&](int j) {
-            const int tok = j * TK + kt;
-            const int64_t p = page_at(tok);
-            const uint4* src = reinterpret_cast<const uint4*>(codes + (p * H + h) * cell) + tok % P;
+            ok = ok && __all_sync(0xffffffffu, qwait(&bars->tabfull[j & 3], (uint32_t)((j >> 2) & 1), a.err,
+                                                     DEV_TIMEOUT_FULL, abort_flag));
+            const int64_t at = ok ? bars->cell[j & 3][kt >> 4] : -1;
+            const uint4* src = reinterpret_cast<const uint4*>(codes + at) + ((j * TK + kt) & (P - 1));
 #pragma unroll
             for (int i = 0; i < kLoads; ++i) {
                 const int c = kc0 + i * kcs;
-                kr[i] = p >= 0 && c * 16 < hs ? __ldg(src + (int64_t)c * P) : make_uint4(0, 0, 0, 0);
-            }
-            sc_k = sc_v = NAN;
-            if (p >= 0 && kt % 16 == 0) {
-                const float2 v = __ldg(reinterpret_cast<const float2*>(a.c.scales) + p * H + h);
-                sc_k = v.x;
-                sc_v = v.y;
+                kr[i] = at >= 0 && c * 16 < hs ? __ldg(src + c * P) : make_uint4(0, 0, 0, 0);
             }
         };
-        auto load_v = [&](int j) {
-            int tc = t / hs, d = t % hs;  // the tile's piece t, t + 128, ...: 16 tokens of dim d
-            int at = -1;
-            int64_t p = -1;
+        auto load_v = [&](int j) {  // after load_k(j)
 #pragma unroll
             for (int i = 0; i < kLoads; ++i) {
-                if (tc < TK / 16) {
-                    const int tok = j * TK + tc * 16;
-                    if (tc != at) {
-                        at = tc;
-                        p = page_at(tok);
-                    }
-                    vr[i] = p >= 0 ? __ldg(reinterpret_cast<const uint4*>(codes + (p * H + h) * cell + hs * P) +
-                                           tok % P / 16 * hs + d)
-                                   : make_uint4(0, 0, 0, 0);
-                }
-                d += 128;
-                while (d >= hs) {
-                    d -= hs;
-                    ++tc;
-                }
+                const int64_t at = ok && ptc[i] < TK / 16 ? bars->cell[j & 3][ptc[i]] : -1;
+                const uint4* src = reinterpret_cast<const uint4*>(codes + at) + (hs >> 4) * P +
+                                   (((j * TK + ptc[i] * 16) & (P - 1)) >> 4) * hs + pd[i];
+                vr[i] = at >= 0 ? __ldg(src) : make_uint4(0, 0, 0, 0);
             }
         };
         // 16 codes to two 16-byte chunks of row `row`, chunk pair `cc` of a 128-byte row
@@ -765,45 +815,32 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const __gr
         for (int j = 0; j < tiles; ++j) {
             const int buf = j % NB;
             const uint32_t par = (uint32_t)((j / NB) & 1);
-            if (!__all_sync(0xffffffffu, qwait(&bars->kempty[buf], par ^ 1u, a.err, DEV_TIMEOUT_EMPTY, abort_flag))) break;
+            ok = ok && __all_sync(0xffffffffu, qwait(&bars->kempty[buf], par ^ 1u, a.err, DEV_TIMEOUT_EMPTY, abort_flag));
+            if (!ok) break;
             unsigned char* kb = sk + buf * Lay::kK;
 #pragma unroll
             for (int i = 0; i < kLoads; ++i) {
                 const int c = kc0 + i * kcs;
                 if (c * 16 < hs) put(kb + (c >> 2) * (TK * 128), kt, c & 3, kr[i]);
             }
-            if (kt % 16 == 0 && kc0 == 0) {
-                Granule& gr = bars->gran[j & 3][kt / 16];
-                const bool fine = sc_v < INFINITY;
-                const float w = fine ? fmaxf(sc_v / svm, 9.094947e-13f) : 1.0f;  // 2^-40 at least
-                const float sh = log2f(w) + kUnit;
-                gr.sk = sc_k;
-                gr.shift = sh;
-                gr.inv = exp2f(-sh);
-                gr.bad = fine ? 0.0f : NAN;
-            }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) mbar_arrive(&bars->kfull[buf]);
             if (j + 1 < tiles) load_k(j + 1);
-            if (!__all_sync(0xffffffffu, qwait(&bars->vempty[buf], par ^ 1u, a.err, DEV_TIMEOUT_EMPTY, abort_flag))) break;
+            ok = ok && __all_sync(0xffffffffu, qwait(&bars->vempty[buf], par ^ 1u, a.err, DEV_TIMEOUT_EMPTY, abort_flag));
+            if (!ok) break;
             unsigned char* vb = sv + buf * Lay::kV;
-            int tc = t / hs, d = t % hs;
 #pragma unroll
-            for (int i = 0; i < kLoads; ++i) {
-                if (tc < TK / 16) put(vb + (tc >> 2) * (hs * 128), d, tc & 3, vr[i]);
-                d += 128;
-                while (d >= hs) {
-                    d -= hs;
-                    ++tc;
-                }
-            }
+            for (int i = 0; i < kLoads; ++i)
+                if (ptc[i] < TK / 16) put(vb + (ptc[i] >> 2) * (hs * 128), pd[i], ptc[i] & 3, vr[i]);
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) mbar_arrive(&bars->vfull[buf]);
             if (j + 1 < tiles) load_v(j + 1);
         }
-    } else if (warp == 12) {
+    } else if (warp >= 12) {
+        regs_down<72>();
+        if (warp == 12) {
         // ---------------- MMA issue ----------------
         const uint32_t id_s = (1u << 4) | ((uint32_t)(TK >> 3) << 17) | (8u << 24);  // f32 += f16 x f16, M 128
         const uint32_t id_o = (1u << 4) | ((uint32_t)(hs >> 3) << 17) | (8u << 24);
@@ -858,7 +895,10 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const __gr
                                        vd + (uint32_t)((k >> 2) * (hs * 128) >> 4) + 2 * (k & 3), id_o,
                                        j > 0 || k > 0 || p > 0);
                     mma_commit(&bars->pvdone[i]);
-                    if (i == NQ - 1 || j >= n[NQ - 1]) mma_commit(&bars->vempty[j % NB]);
+                    if (i == NQ - 1 || j >= n[NQ - 1]) {
+                        mma_commit(&bars->vempty[j % NB]);
+                        mma_commit(&bars->tabempty[j & 3]);
+                    }
                 }
                 __syncwarp();
                 if (j + 1 < n[i]) scores(i, j + 1);
@@ -867,50 +907,99 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const __gr
         if (elect_one()) mma_commit(&bars->done);
         __syncwarp();
         mbar_wait(&bars->done, 0, a.err, DEV_TIMEOUT_MMA);  // every MMA is done before the memory is freed
-    } else if (warp < 4 * NQ && n[warp >> 2] > 0) {
+        } else if (warp == 13) {
+        // ---------------- pages and scales ----------------
+        for (int j = 0; j < tiles; ++j) {
+            const int tok = j * TK + lane * 16;
+            int64_t p = -1;
+            float2 sc = make_float2(NAN, NAN);
+            if (lane < TK / 16 && tok < seen) {
+                p = page_of(a.c, a.b, s, tok >> lp2, a.err);
+                if (p >= 0) sc = __ldg(reinterpret_cast<const float2*>(a.c.scales) + p * H + h);
+            }
+            const bool fine = sc.y < INFINITY;
+            const float w = fine ? fmaxf(sc.y / svm, 9.094947e-13f) : 1.0f;  // 2^-40 at least
+            const float shift = log2f(w) + kUnit, inv = exp2f(-shift);
+            if (!__all_sync(0xffffffffu, qwait(&bars->tabempty[j & 3], (uint32_t)(((j >> 2) & 1) ^ 1), a.err,
+                                               DEV_TIMEOUT_EMPTY, abort_flag)))
+                break;
+            if (lane < TK / 16) {
+                bars->gran[j & 3][lane] = {sc.x, shift, inv, fine ? 0.0f : NAN};
+                bars->cell[j & 3][lane] = p >= 0 ? (p * H + h) * (int64_t)(hs * P * 2) : -1;
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars->tabfull[j & 3]);
+        }
+        }
+    } else {
         // ---------------- softmax ----------------
+        regs_up<168>();
+        if (warp < 4 * NQ && (warp < 4 ? n[0] : n[NQ - 1]) > 0) {
         const int i = warp >> 2, w4 = warp & 3;
         const int n_i = i == 0 ? n[0] : n[NQ - 1];
-        // q of this warp's 32 rows, a row at a time: 4 dims a lane
-        for (int rr = 0; rr < 32; ++rr) {
-            const int row = w4 * 32 + rr, r = base_row + i * 128 + row;
-            const bool have = r < rows;
-            const int64_t at = have ? (int64_t)(q.r0 + r / g) * a.ld_q + (int64_t)(h * g + r % g) * hs : 0;
-            float x[(HS + 127) / 128][4];
-            uint32_t m = 0;
+        // q of this warp's 32 rows, a few at a time (all their loads before the
+        // first use), 4 dims a lane
+        constexpr int kB = (HS + 127) / 128, kBatch = 8 / kB;
+        const int first = base_row + i * 128 + w4 * 32;
+        int tok = min(first, rows - 1) / g, head = min(first, rows - 1) - tok * g;
+        for (int r0 = 0; r0 < 32; r0 += kBatch) {
+            RawQ<PARTS> raw[kBatch][kB];
 #pragma unroll
-            for (int b = 0; b < (HS + 127) / 128; ++b)
+            for (int u = 0; u < kBatch; ++u) {
+                const int64_t at = (int64_t)(q.r0 + tok) * a.ld_q + (int64_t)(h * g + head) * hs;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int d = b * 128 + lane * 4 + e;
-                    x[b][e] = have && d < hs ? load_q(a, at + d) : 0.0f;
-                    m = max(m, abs_bits(x[b][e]));
+                for (int b = 0; b < kB; ++b) raw[u][b].load(a, at + min(b * 128 + lane * 4, hs - 4));
+                if (first + r0 + u + 1 < rows && ++head == g) {
+                    head = 0;
+                    ++tok;
                 }
-            m = __reduce_max_sync(0xffffffffu, m);
-            // a power of two that takes the largest into [2^13, 2^14)
-            int ex = (int)(m >> 23) - 127;
-            ex = max(-114, min(100, 13 - ex));
-            const float up = a.scale < 0.0f ? -lq_exp2i(ex) : lq_exp2i(ex);
-            if (lane == 0)
-                bars->fs[i * 128 + row] = m >= kInfBits ? NAN : fabsf(a.scale) * lq_exp2i(-ex);
+            }
+            float x[kBatch][kB][4];
 #pragma unroll
-            for (int b = 0; b < (HS + 127) / 128; ++b) {
-                const int d = b * 128 + lane * 4;
-                if (d >= hs) continue;
+            for (int u = 0; u < kBatch; ++u) {
+                const bool have = first + r0 + u < rows;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) x[b][e] = m >= kInfBits ? 0.0f : x[b][e] * up;
+                for (int b = 0; b < kB; ++b) {
+                    raw[u][b].get(a, x[u][b]);
 #pragma unroll
-                for (int p = 0; p < PARTS; ++p) {
-                    const __half2 u = __floats2half2_rn(x[b][0], x[b][1]), v = __floats2half2_rn(x[b][2], x[b][3]);
-                    unsigned char* dst = sq + i * Lay::kQ + p * (Lay::kQ / PARTS) + (d >> 6) * (128 * 128) + row * 128 +
-                                         ((((d & 63) >> 3) ^ (row & 7)) << 4) + (d & 4) * 2;
-                    *reinterpret_cast<uint2*>(dst) =
-                        make_uint2(*reinterpret_cast<const uint32_t*>(&u), *reinterpret_cast<const uint32_t*>(&v));
-                    const float2 fu = __half22float2(u), fv = __half22float2(v);
-                    x[b][0] -= fu.x;
-                    x[b][1] -= fu.y;
-                    x[b][2] -= fv.x;
-                    x[b][3] -= fv.y;
+                    for (int e = 0; e < 4; ++e)
+                        if (!have || b * 128 + lane * 4 >= hs) x[u][b][e] = 0.0f;
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < kBatch; ++u) {
+                const int row = w4 * 32 + r0 + u;
+                uint32_t m = 0;
+#pragma unroll
+                for (int b = 0; b < kB; ++b)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) m = max(m, abs_bits(x[u][b][e]));
+                m = __reduce_max_sync(0xffffffffu, m);
+                // a power of two that takes the largest into [2^13, 2^14)
+                int ex = (int)(m >> 23) - 127;
+                ex = max(-114, min(100, 13 - ex));
+                const float up = m >= kInfBits ? 0.0f : a.scale < 0.0f ? -lq_exp2i(ex) : lq_exp2i(ex);
+                if (lane == 0) bars->fs[i * 128 + row] = m >= kInfBits ? NAN : fabsf(a.scale) * lq_exp2i(-ex);
+#pragma unroll
+                for (int b = 0; b < kB; ++b) {
+                    const int d = b * 128 + lane * 4;
+                    if (d >= hs) continue;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[u][b][e] = up == 0.0f ? 0.0f : x[u][b][e] * up;
+#pragma unroll
+                    for (int p = 0; p < PARTS; ++p) {
+                        const uint32_t w0 = pack_word<__half>(x[u][b]), w1 = pack_word<__half>(x[u][b] + 2);
+                        unsigned char* dst = sq + i * Lay::kQ + p * (Lay::kQ / PARTS) + (d >> 6) * (128 * 128) +
+                                             row * 128 + ((((d & 63) >> 3) ^ (row & 7)) << 4) + (d & 4) * 2;
+                        *reinterpret_cast<uint2*>(dst) = make_uint2(w0, w1);
+                        if (p + 1 < PARTS) {  // what the first part leaves
+                            float y[4];
+                            unpack_word<__half>(w0, y);
+                            unpack_word<__half>(w1, y + 2);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) x[u][b][e] -= y[e];
+                        }
+                    }
                 }
             }
         }
@@ -931,26 +1020,27 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const __gr
             tc_fence_after();
             const Granule* gr = bars->gran[j & 3];
             const int left = pos - j * TK;  // the tile's last token that this row sees
-            const bool masked = __any_sync(0xffffffffu, left < TK - 1);
+            float x[TK / 32][32];
+#pragma unroll
+            for (int c = 0; c < TK / 32; ++c) tmem_ld<32>(ts + c * 32, reinterpret_cast<int(&)[32]>(x[c]));
+            tmem_ld_wait();
+            if (__any_sync(0xffffffffu, left < TK - 1)) {
+#pragma unroll
+                for (int c = 0; c < TK / 32; ++c)
+#pragma unroll
+                    for (int k = 0; k < 32; ++k)
+                        if (c * 32 + k > left) x[c][k] = -INFINITY;
+            }
             float m = -INFINITY;
-            int x[32];
 #pragma unroll
-            for (int c = 0; c < TK / 32; ++c) {
-                tmem_ld<32>(ts + c * 32, x);
-                tmem_ld_wait();
+            for (int e = 0; e < TK / 16; ++e) {
+                const float* y = &x[e / 2][(e & 1) * 16];
+                float t[8];
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    float mx = -INFINITY;
-                    if (masked) {
+                for (int k = 0; k < 8; ++k) t[k] = fmaxf(y[k], y[k + 8]);
 #pragma unroll
-                        for (int k = 0; k < 16; ++k)
-                            mx = fmaxf(mx, c * 32 + e * 16 + k <= left ? __int_as_float(x[e * 16 + k]) : -INFINITY);
-                    } else {
-#pragma unroll
-                        for (int k = 0; k < 16; ++k) mx = fmaxf(mx, __int_as_float(x[e * 16 + k]));
-                    }
-                    m = fmaxf(m, mx * (fs * gr[2 * c + e].sk));
-                }
+                for (int k = 0; k < 4; ++k) t[k] = fmaxf(t[k], t[k + 4]);
+                m = fmaxf(m, fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])) * (fs * gr[e].sk));
             }
             const bool grown = j == 0 ? m > -INFINITY : m > mref + kGrow;
             if (__any_sync(0xffffffffu, grown)) {
@@ -976,25 +1066,24 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const __gr
             }
 #pragma unroll
             for (int c = 0; c < TK / 32; ++c) {
-                tmem_ld<32>(ts + c * 32, x);
-                tmem_ld_wait();
                 uint32_t hi[16], lo[16];
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     const Granule gg = gr[2 * c + e];
-                    const float f = fs * gg.sk, b = gg.shift - mref;
-                    if (c * 32 + e * 16 <= left) poison += gg.bad;
-                    float sum = 0.0f;
+                    // a masked -infinity has to stay one: no factor of zero, and
+                    // no NaN from a granule that the row does not see
+                    const bool sees = c * 32 + e * 16 <= left;
+                    float f = sees ? fs * gg.sk : 1e-38f;
+                    if (f == 0.0f) f = 1e-38f;
+                    const float b = gg.shift - mref;
+                    if (sees) poison += gg.bad;
+                    float sum[2] = {};
 #pragma unroll
                     for (int k = 0; k < 16; k += 2) {
-                        float p0 = exp2_fast(fmaf(__int_as_float(x[e * 16 + k]), f, b));
-                        float p1 = exp2_fast(fmaf(__int_as_float(x[e * 16 + k + 1]), f, b));
-                        if (masked) {
-                            if (c * 32 + e * 16 + k > left) p0 = 0.0f;
-                            if (c * 32 + e * 16 + k + 1 > left) p1 = 0.0f;
-                        }
-                        sum += p0;
-                        sum += p1;
+                        const float p0 = exp2_fast(fmaf(x[c][e * 16 + k], f, b));
+                        const float p1 = exp2_fast(fmaf(x[c][e * 16 + k + 1], f, b));
+                        sum[0] += p0;
+                        sum[1] += p1;
                         const __half2 u = __floats2half2_rn(p0, p1);
                         hi[e * 8 + k / 2] = *reinterpret_cast<const uint32_t*>(&u);
                         if (PARTS == 2) {
@@ -1003,7 +1092,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const __gr
                             lo[e * 8 + k / 2] = *reinterpret_cast<const uint32_t*>(&v);
                         }
                     }
-                    l = fmaf(sum, gg.inv, l);
+                    l = fmaf(sum[0] + sum[1], gg.inv, l);
                 }
                 tmem_st16(ts + c * 32, hi);
                 if (PARTS == 2) tmem_st16(ts + c * 32 + 16, lo);
@@ -1017,10 +1106,6 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const __gr
             ok = __all_sync(0xffffffffu, qwait(&bars->pvdone[i], (uint32_t)((n_i - 1) & 1), a.err, DEV_TIMEOUT_TFULL, abort_flag));
         tc_fence_after();
         if (ok) {
-            const float svm = [&] {
-                const float v = fmaxf(fmaxf(bars->peak[0], bars->peak[1]), fmaxf(bars->peak[2], bars->peak[3]));
-                return v == 0.0f ? 1.0f : v;
-            }();
             const float f = svm * (1.0f / 64.0f) / l;  // 2^-kUnit
             const int64_t at = (int64_t)(q.r0 + r / g) * a.ld_out + (int64_t)(h * g + r % g) * hs;
             for (int c = 0; c < hs; c += 16) {
@@ -1031,6 +1116,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const __gr
             }
             if (a.lse && r < rows)
                 a.lse[(int64_t)(q.r0 + r / g) * a.n_heads + h * g + r % g] = (mref + log2f(l)) * kLn2;
+        }
         }
     }
     tc_fence_before();
@@ -1104,6 +1190,7 @@ extern "C" int paged_attention(void* out, int64_t ld_out, const void* q, int64_t
     a.n_heads = n_heads;
     a.group = n_heads / cache->n_kv_heads;
     a.type = type;
+    a.q_vec = reinterpret_cast<uintptr_t>(q) % (4 * size) == 0 && ld_q % 4 == 0;
     a.scale = scale * kLog2e;
     a.err = c->err;
     // few rows: every (sequence, kv head, row tile) is cut into splits of the context
@@ -1128,8 +1215,11 @@ extern "C" int paged_attention(void* out, int64_t ld_out, const void* q, int64_t
         if (rc) return rc;
     }
     a.part = static_cast<float*>(part);
+    // one sequence with many rows leaves nothing to the first kernel
+    a.few_rows = batch->n_seqs == 1 && most_rows > kFewRows && (int64_t)batch->n_rows * a.group > kFewRows ? 0 : kFewRows;
     const dim3 grid((unsigned)jobs, (unsigned)splits);
-    cudaError_t e = type == LQ_F32 ? few_launch<3>(a, grid, stream()) : few_launch<2>(a, grid, stream());
+    cudaError_t e = cudaSuccess;
+    if (a.few_rows) e = type == LQ_F32 ? few_launch<3>(a, grid, stream()) : few_launch<2>(a, grid, stream());
     if (e != cudaSuccess) return cuda_fail(e, "paged_attention launch");
     if (most_rows > kFewRows) {
         e = many_launch(a, stream());
