@@ -39,7 +39,7 @@ struct AttArgs {
     float* lse;
     int64_t ld_q, ld_out;
     int n_heads, group, type;
-    int q_vec;        // 4 elements of q are one aligned load
+    int q_vec;        // rows of q are 16-byte aligned
     int few_rows;     // (token, head) rows of a sequence and kv head that the first kernel takes
     float scale;      // log2(e) times the caller's
     int row_tiles;    // tiles of 8 (token, head) rows of a sequence and kv head
@@ -636,10 +636,11 @@ cudaError_t few_launch(const AttArgs& a, dim3 grid, cudaStream_t st) {
 // Many rows per kv head (prompts): bound by arithmetic, on tcgen05.
 //
 // One CTA per NQ tiles of 128 (token, head) rows of a sequence and kv head,
-// which walk the context together in tiles of TK tokens.  Codes become f16
-// exactly; a row of q is scaled by a power of two to fill f16's range and is
-// one f16 (the 16-bit types) or two (fp32: 22 bits); so are the weights.
-// Products accumulate in fp32 in tensor memory.
+// which walk the context together in tiles of TK tokens.  Codes become f16 or
+// bf16 exactly.  q of the 16-bit types is taken as it is (K in q's type); an fp32
+// row is scaled by a power of two to fill f16's range and is two f16 (22
+// bits); the weights are one or two f16 (V in f16).  Products accumulate in
+// fp32 in tensor memory.
 //
 //   warps 0-3, 4-7   softmax of one row tile each: a thread per row reads its
 //                    scores from tensor memory, writes its weights over them
@@ -655,11 +656,12 @@ cudaError_t few_launch(const AttArgs& a, dim3 grid, cudaStream_t st) {
 // shift); s_V enters as its logarithm: a weight's exponent gets log2(s_V / max
 // s_V over the context), so O needs no second scaling, and the sum divides it
 // out again per granule.  O is rescaled only when a row's maximum has grown by
-// more than 2^8 since its last one: weights carry 2^6 to stay in f16's range.
+// more than 2^13 since its last one: weights are 2^kUnit at that maximum, 2^14 at
+// most, within f16's range.
 
 constexpr int kManyWarps = 16;  // the last two idle: registers are dealt to warpgroups
 constexpr int kManyThreads = 32 * kManyWarps;
-constexpr float kGrow = 8.0f, kUnit = 6.0f;
+constexpr float kGrow = 13.0f, kUnit = 1.0f;
 
 struct Granule {  // 16 tokens
     float sk, shift, inv, bad;  // s_K, log2(weight) + kUnit, 1 / (weight * 2^kUnit), NaN where s_V is not finite
@@ -676,16 +678,17 @@ struct ManyBars {
     float fs[256];       // rows' factors of the scores
 };
 
-template <int HS, int PARTS, int NQ, int TK, int NB>
+template <int HS, int TYPE, int NQ, int TK, int NB>
 struct ManyLayout {
-    static constexpr int kQ = 128 * HS * 2 * PARTS;        // one row tile: [part][64 dims][128][128 bytes]
+    static constexpr int kParts = TYPE == LQ_F32 ? 2 : 1;
+    static constexpr int kQ = 128 * HS * 2 * kParts;       // one row tile: [part][64 dims][128][128 bytes]
     static constexpr int kK = TK * HS * 2, kV = TK * HS * 2;
     static constexpr int kSmem = 1024 + NQ * kQ + NB * (kK + kV) + (int)sizeof(ManyBars);
     static_assert(kSmem <= 227 * 1024 && HS % 64 == 0, "shared memory");
     static_assert(NQ * (TK + HS) <= 512, "tensor memory");
 };
 
-// 4 codes to 2 x 2 halves: bytes + 128 as the low mantissa of 1024, minus 1152
+// 4 codes to 2 x 2 f16: bytes + 128 as the low mantissa of 1024, minus 1152
 __device__ __forceinline__ uint2 codes_f16(uint32_t w) {
     w ^= 0x80808080u;
     const uint32_t lo = __byte_perm(w, 0x64646464u, 0x4140), hi = __byte_perm(w, 0x64646464u, 0x4342);
@@ -695,9 +698,33 @@ __device__ __forceinline__ uint2 codes_f16(uint32_t w) {
     return make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
 }
 
-template <int HS, int PARTS, int NQ, int TK, int NB>
+// 4 codes to 2 x 2 bf16: the low 7 bits as the mantissa of 128, minus 128 (a
+// code of 0 to 127) or 256 (a negative one), which its sign bit makes of 128
+__device__ __forceinline__ uint2 codes_bf16(uint32_t w) {
+    auto two = [](uint32_t x) {
+        const uint32_t m = (x & 0x007F007Fu) | 0x43004300u, off = (x & 0x00800080u) | 0x43004300u;
+        const __nv_bfloat162 r =
+            __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&m), *reinterpret_cast<const __nv_bfloat162*>(&off));
+        return *reinterpret_cast<const uint32_t*>(&r);
+    };
+    return make_uint2(two(__byte_perm(w, 0, 0x4140)), two(__byte_perm(w, 0, 0x4342)));
+}
+
+// 16 codes to two 16-byte chunks (2 * pair, 2 * pair + 1) of row `row` of 128-byte swizzled rows
+template <bool BF16>
+__device__ __forceinline__ void put_codes(unsigned char* block, int row, int pair, uint4 w) {
+    const uint2 x = BF16 ? codes_bf16(w.x) : codes_f16(w.x), y = BF16 ? codes_bf16(w.y) : codes_f16(w.y);
+    const uint2 z = BF16 ? codes_bf16(w.z) : codes_f16(w.z), u = BF16 ? codes_bf16(w.w) : codes_f16(w.w);
+    const uint32_t at = row * 128 + ((row & 7) << 4);
+    *reinterpret_cast<uint4*>(block + (at ^ (pair << 5))) = make_uint4(x.x, x.y, y.x, y.y);
+    *reinterpret_cast<uint4*>(block + (at ^ (pair << 5) ^ 16)) = make_uint4(z.x, z.y, u.x, u.y);
+}
+
+template <int HS, int TYPE, int NQ, int TK, int NB, bool EXACT>
 __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const __grid_constant__ AttArgs a) {
-    using Lay = ManyLayout<HS, PARTS, NQ, TK, NB>;
+    using Lay = ManyLayout<HS, TYPE, NQ, TK, NB>;
+    constexpr int PARTS = Lay::kParts;
+    constexpr bool kBf16 = TYPE == LQ_BF16;
     constexpr int kPieces = HS / 16;  // 16-byte pieces of K (and of V) per converting thread and 128 tokens
     constexpr int kLoads = kPieces * TK / 128;
     extern __shared__ __align__(1024) unsigned char raw[];
@@ -706,7 +733,8 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const __gr
     ManyBars* bars = reinterpret_cast<ManyBars*>(sv + NB * Lay::kV);
     volatile int* abort_flag = &bars->abort_flag;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int hs = a.c.head_size, P = a.c.page_size, H = a.c.n_kv_heads, g = a.group;
+    const int hs = EXACT ? HS : a.c.head_size;
+    const int P = a.c.page_size, H = a.c.n_kv_heads, g = a.group;
     const int tile = gridDim.x - 1 - blockIdx.x;  // long ones first
     const int h = blockIdx.y, s = blockIdx.z;
 
@@ -803,13 +831,6 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const __gr
                 vr[i] = at >= 0 ? __ldg(src) : make_uint4(0, 0, 0, 0);
             }
         };
-        // 16 codes to two 16-byte chunks of row `row`, chunk pair `cc` of a 128-byte row
-        auto put = [&](unsigned char* block, int row, int cc, uint4 w) {
-            const uint2 x = codes_f16(w.x), y = codes_f16(w.y), z = codes_f16(w.z), u = codes_f16(w.w);
-            unsigned char* r = block + row * 128;
-            *reinterpret_cast<uint4*>(r + (((2 * cc) ^ (row & 7)) << 4)) = make_uint4(x.x, x.y, y.x, y.y);
-            *reinterpret_cast<uint4*>(r + (((2 * cc + 1) ^ (row & 7)) << 4)) = make_uint4(z.x, z.y, u.x, u.y);
-        };
         load_k(0);
         load_v(0);
         for (int j = 0; j < tiles; ++j) {
@@ -821,7 +842,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const __gr
 #pragma unroll
             for (int i = 0; i < kLoads; ++i) {
                 const int c = kc0 + i * kcs;
-                if (c * 16 < hs) put(kb + (c >> 2) * (TK * 128), kt, c & 3, kr[i]);
+                if (c * 16 < hs) put_codes<kBf16>(kb + (c >> 2) * (TK * 128), kt, c & 3, kr[i]);
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
@@ -832,7 +853,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const __gr
             unsigned char* vb = sv + buf * Lay::kV;
 #pragma unroll
             for (int i = 0; i < kLoads; ++i)
-                if (ptc[i] < TK / 16) put(vb + (ptc[i] >> 2) * (hs * 128), pd[i], ptc[i] & 3, vr[i]);
+                if (ptc[i] < TK / 16) put_codes<false>(vb + (ptc[i] >> 2) * (hs * 128), pd[i], ptc[i] & 3, vr[i]);
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) mbar_arrive(&bars->vfull[buf]);
@@ -842,7 +863,8 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const __gr
         regs_down<72>();
         if (warp == 12) {
         // ---------------- MMA issue ----------------
-        const uint32_t id_s = (1u << 4) | ((uint32_t)(TK >> 3) << 17) | (8u << 24);  // f32 += f16 x f16, M 128
+        // f32 += f16 x f16 (or bf16 x bf16), M 128
+        const uint32_t id_s = (1u << 4) | (kBf16 ? (1u << 7) | (1u << 10) : 0u) | ((uint32_t)(TK >> 3) << 17) | (8u << 24);
         const uint32_t id_o = (1u << 4) | ((uint32_t)(hs >> 3) << 17) | (8u << 24);
         const uint64_t dq = smem_desc_sw128(smem_addr(sq)), dk = smem_desc_sw128(smem_addr(sk)),
                        dv = smem_desc_sw128(smem_addr(sv));
@@ -937,67 +959,105 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const __gr
         if (warp < 4 * NQ && (warp < 4 ? n[0] : n[NQ - 1]) > 0) {
         const int i = warp >> 2, w4 = warp & 3;
         const int n_i = i == 0 ? n[0] : n[NQ - 1];
-        // q of this warp's 32 rows, a few at a time (all their loads before the
-        // first use), 4 dims a lane
-        constexpr int kB = (HS + 127) / 128, kBatch = 8 / kB;
+        // q of this warp's 32 rows
         const int first = base_row + i * 128 + w4 * 32;
-        int tok = min(first, rows - 1) / g, head = min(first, rows - 1) - tok * g;
-        for (int r0 = 0; r0 < 32; r0 += kBatch) {
-            RawQ<PARTS> raw[kBatch][kB];
+        if constexpr (PARTS == 1) {
+            // as it is: 16-byte pieces, the warp's lanes along a row
+            const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
+            const int per = hs / 8, total = 32 * per;  // pieces of a row, of the warp
+            constexpr int kAt = 8;
+            for (int p0 = 0; p0 < total; p0 += 32 * kAt) {
+                uint4 v[kAt];
 #pragma unroll
-            for (int u = 0; u < kBatch; ++u) {
-                const int64_t at = (int64_t)(q.r0 + tok) * a.ld_q + (int64_t)(h * g + head) * hs;
+                for (int u = 0; u < kAt; ++u) {
+                    const int pc = p0 + u * 32 + lane, rr = pc / per, d = (pc - rr * per) * 8;
+                    v[u] = make_uint4(0, 0, 0, 0);
+                    if (pc < total && first + rr < rows) {
+                        const int r = first + rr;
+                        const uint16_t* src = static_cast<const uint16_t*>(a.q) + (int64_t)(q.r0 + r / g) * a.ld_q +
+                                              (int64_t)(h * g + r % g) * hs + d;
+                        if (a.q_vec) {
+                            v[u] = __ldg(reinterpret_cast<const uint4*>(src));
+                        } else {
+                            uint32_t w[4];
 #pragma unroll
-                for (int b = 0; b < kB; ++b) raw[u][b].load(a, at + min(b * 128 + lane * 4, hs - 4));
-                if (first + r0 + u + 1 < rows && ++head == g) {
-                    head = 0;
-                    ++tok;
+                            for (int k = 0; k < 4; ++k) w[k] = __ldg(src + 2 * k) | (uint32_t)__ldg(src + 2 * k + 1) << 16;
+                            v[u] = make_uint4(w[0], w[1], w[2], w[3]);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < kAt; ++u) {
+                    const int pc = p0 + u * 32 + lane, rr = pc / per, ck = pc - rr * per, row = w4 * 32 + rr;
+                    if (pc < total)
+                        *reinterpret_cast<uint4*>(sq + i * Lay::kQ + (ck >> 3) * (128 * 128) + row * 128 +
+                                                  (((ck & 7) ^ (row & 7)) << 4)) =
+                            make_uint4(v[u].x ^ flip, v[u].y ^ flip, v[u].z ^ flip, v[u].w ^ flip);
                 }
             }
-            float x[kBatch][kB][4];
+            bars->fs[i * 128 + w4 * 32 + lane] = fabsf(a.scale);
+        } else {
+            // scaled and split, a few rows at a time (all their loads before the
+            // first use), 4 dims a lane
+            constexpr int kB = (HS + 127) / 128, kBatch = 8 / kB;
+            int tok = min(first, rows - 1) / g, head = min(first, rows - 1) - tok * g;
+            for (int r0 = 0; r0 < 32; r0 += kBatch) {
+                RawQ<2> raw[kBatch][kB];
 #pragma unroll
-            for (int u = 0; u < kBatch; ++u) {
-                const bool have = first + r0 + u < rows;
+                for (int u = 0; u < kBatch; ++u) {
+                    const int64_t at = (int64_t)(q.r0 + tok) * a.ld_q + (int64_t)(h * g + head) * hs;
 #pragma unroll
-                for (int b = 0; b < kB; ++b) {
-                    raw[u][b].get(a, x[u][b]);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (!have || b * 128 + lane * 4 >= hs) x[u][b][e] = 0.0f;
+                    for (int b = 0; b < kB; ++b) raw[u][b].load(a, at + min(b * 128 + lane * 4, hs - 4));
+                    if (first + r0 + u + 1 < rows && ++head == g) {
+                        head = 0;
+                        ++tok;
+                    }
                 }
-            }
+                float x[kBatch][kB][4];
 #pragma unroll
-            for (int u = 0; u < kBatch; ++u) {
-                const int row = w4 * 32 + r0 + u;
-                uint32_t m = 0;
+                for (int u = 0; u < kBatch; ++u) {
+                    const bool have = first + r0 + u < rows;
 #pragma unroll
-                for (int b = 0; b < kB; ++b)
+                    for (int b = 0; b < kB; ++b) {
+                        raw[u][b].get(a, x[u][b]);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) m = max(m, abs_bits(x[u][b][e]));
-                m = __reduce_max_sync(0xffffffffu, m);
-                // a power of two that takes the largest into [2^13, 2^14)
-                int ex = (int)(m >> 23) - 127;
-                ex = max(-114, min(100, 13 - ex));
-                const float up = m >= kInfBits ? 0.0f : a.scale < 0.0f ? -lq_exp2i(ex) : lq_exp2i(ex);
-                if (lane == 0) bars->fs[i * 128 + row] = m >= kInfBits ? NAN : fabsf(a.scale) * lq_exp2i(-ex);
+                        for (int e = 0; e < 4; ++e)
+                            if (!have || b * 128 + lane * 4 >= hs) x[u][b][e] = 0.0f;
+                    }
+                }
 #pragma unroll
-                for (int b = 0; b < kB; ++b) {
-                    const int d = b * 128 + lane * 4;
-                    if (d >= hs) continue;
+                for (int u = 0; u < kBatch; ++u) {
+                    const int row = w4 * 32 + r0 + u;
+                    uint32_t m = 0;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) x[u][b][e] = up == 0.0f ? 0.0f : x[u][b][e] * up;
+                    for (int b = 0; b < kB; ++b)
 #pragma unroll
-                    for (int p = 0; p < PARTS; ++p) {
-                        const uint32_t w0 = pack_word<__half>(x[u][b]), w1 = pack_word<__half>(x[u][b] + 2);
-                        unsigned char* dst = sq + i * Lay::kQ + p * (Lay::kQ / PARTS) + (d >> 6) * (128 * 128) +
-                                             row * 128 + ((((d & 63) >> 3) ^ (row & 7)) << 4) + (d & 4) * 2;
-                        *reinterpret_cast<uint2*>(dst) = make_uint2(w0, w1);
-                        if (p + 1 < PARTS) {  // what the first part leaves
-                            float y[4];
-                            unpack_word<__half>(w0, y);
-                            unpack_word<__half>(w1, y + 2);
+                        for (int e = 0; e < 4; ++e) m = max(m, abs_bits(x[u][b][e]));
+                    m = __reduce_max_sync(0xffffffffu, m);
+                    // a power of two that takes the largest into [2^13, 2^14)
+                    int ex = (int)(m >> 23) - 127;
+                    ex = max(-114, min(100, 13 - ex));
+                    const float up = m >= kInfBits ? 0.0f : a.scale < 0.0f ? -lq_exp2i(ex) : lq_exp2i(ex);
+                    if (lane == 0) bars->fs[i * 128 + row] = m >= kInfBits ? NAN : fabsf(a.scale) * lq_exp2i(-ex);
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) x[u][b][e] -= y[e];
+                    for (int b = 0; b < kB; ++b) {
+                        const int d = b * 128 + lane * 4;
+                        if (d >= hs) continue;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) x[u][b][e] = up == 0.0f ? 0.0f : x[u][b][e] * up;
+#pragma unroll
+                        for (int p = 0; p < PARTS; ++p) {
+                            const uint32_t w0 = pack_word<__half>(x[u][b]), w1 = pack_word<__half>(x[u][b] + 2);
+                            unsigned char* dst = sq + i * Lay::kQ + p * (Lay::kQ / PARTS) + (d >> 6) * (128 * 128) +
+                                                 row * 128 + ((((d & 63) >> 3) ^ (row & 7)) << 4) + (d & 4) * 2;
+                            *reinterpret_cast<uint2*>(dst) = make_uint2(w0, w1);
+                            if (p + 1 < PARTS) {  // what the first part leaves
+                                float y[4];
+                                unpack_word<__half>(w0, y);
+                                unpack_word<__half>(w1, y + 2);
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) x[u][b][e] -= y[e];
+                            }
                         }
                     }
                 }
@@ -1106,7 +1166,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const __gr
             ok = __all_sync(0xffffffffu, qwait(&bars->pvdone[i], (uint32_t)((n_i - 1) & 1), a.err, DEV_TIMEOUT_TFULL, abort_flag));
         tc_fence_after();
         if (ok) {
-            const float f = svm * (1.0f / 64.0f) / l;  // 2^-kUnit
+            const float f = svm * 0.5f / l;  // 2^-kUnit
             const int64_t at = (int64_t)(q.r0 + r / g) * a.ld_out + (int64_t)(h * g + r % g) * hs;
             for (int c = 0; c < hs; c += 16) {
                 int y[16];
@@ -1127,10 +1187,10 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const __gr
     }
 }
 
-template <int HS, int PARTS, int NQ, int TK, int NB>
+template <int HS, int TYPE, int NQ, int TK, int NB, bool EXACT>
 cudaError_t many_launch_t(const AttArgs& a, cudaStream_t st) {
-    using Lay = ManyLayout<HS, PARTS, NQ, TK, NB>;
-    auto kern = attend_many_kernel<HS, PARTS, NQ, TK, NB>;
+    using Lay = ManyLayout<HS, TYPE, NQ, TK, NB>;
+    auto kern = attend_many_kernel<HS, TYPE, NQ, TK, NB, EXACT>;
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Lay::kSmem);
     if (e != cudaSuccess) return e;
     const int64_t x = ((int64_t)a.b.max_rows * a.group + NQ * 128 - 1) / (NQ * 128);
@@ -1147,15 +1207,15 @@ cudaError_t many_launch_t(const AttArgs& a, cudaStream_t st) {
     return cudaLaunchKernelEx(&cfg, kern, a);
 }
 
+// Two row tiles of 128 for the usual head sizes, whose kernels have their
+// addresses at compile time; one for any other (their accumulators and operands
+// would not fit twice at the largest).
+template <int TYPE>
 cudaError_t many_launch(const AttArgs& a, cudaStream_t st) {
-    const int hs = a.c.head_size;
-    if (a.type == LQ_F32)
-        return hs <= 64    ? many_launch_t<64, 2, 2, 128, 2>(a, st)
-               : hs <= 128 ? many_launch_t<128, 2, 2, 128, 1>(a, st)
-                           : many_launch_t<256, 2, 1, 64, 1>(a, st);
-    return hs <= 64    ? many_launch_t<64, 1, 2, 128, 2>(a, st)
-           : hs <= 128 ? many_launch_t<128, 1, 2, 128, 2>(a, st)
-                       : many_launch_t<256, 1, 1, 128, 1>(a, st);
+    constexpr bool f32 = TYPE == LQ_F32;
+    if (a.c.head_size == 64) return many_launch_t<64, TYPE, 2, 128, 2, true>(a, st);
+    if (a.c.head_size == 128) return many_launch_t<128, TYPE, 2, 128, f32 ? 1 : 2, true>(a, st);
+    return many_launch_t<256, TYPE, 1, f32 ? 64 : 128, 1, false>(a, st);
 }
 
 }  // namespace
@@ -1190,7 +1250,7 @@ extern "C" int paged_attention(void* out, int64_t ld_out, const void* q, int64_t
     a.n_heads = n_heads;
     a.group = n_heads / cache->n_kv_heads;
     a.type = type;
-    a.q_vec = reinterpret_cast<uintptr_t>(q) % (4 * size) == 0 && ld_q % 4 == 0;
+    a.q_vec = reinterpret_cast<uintptr_t>(q) % 16 == 0 && ld_q * size % 16 == 0;
     a.scale = scale * kLog2e;
     a.err = c->err;
     // few rows: every (sequence, kv head, row tile) is cut into splits of the context
@@ -1222,7 +1282,9 @@ extern "C" int paged_attention(void* out, int64_t ld_out, const void* q, int64_t
     if (a.few_rows) e = type == LQ_F32 ? few_launch<3>(a, grid, stream()) : few_launch<2>(a, grid, stream());
     if (e != cudaSuccess) return cuda_fail(e, "paged_attention launch");
     if (most_rows > kFewRows) {
-        e = many_launch(a, stream());
+        e = type == LQ_F32   ? many_launch<LQ_F32>(a, stream())
+            : type == LQ_F16 ? many_launch<LQ_F16>(a, stream())
+                             : many_launch<LQ_BF16>(a, stream());
         if (e != cudaSuccess) return cuda_fail(e, "paged_attention launch");
     }
     return LQ_OK;
