@@ -127,12 +127,12 @@ __device__ __forceinline__ void store_row16(const AttArgs& a, int64_t i, const i
 
 // the outputs of a sequence's rows that attend to nothing, for one kv head
 __device__ __forceinline__ void zero_rows(const AttArgs& a, const SeqRows& q, int h) {
-    const int hs = a.c.head_size, w = a.group * hs;
-    for (int64_t i = threadIdx.x; i < (int64_t)(q.r0 - q.first) * w; i += blockDim.x) {
-        const int64_t row = q.first + i / w;
-        const int d = (int)(i % w);
-        store_out(a, row * a.ld_out + (int64_t)h * w + d, 0.0f);
-        if (a.lse && d % hs == 0) a.lse[row * a.n_heads + h * a.group + d / hs] = -INFINITY;
+    const int w = a.group * a.c.head_size;
+#pragma unroll 1
+    for (int row = q.first; row < q.r0; ++row) {
+        for (int d = threadIdx.x; d < w; d += blockDim.x) store_out(a, (int64_t)row * a.ld_out + (int64_t)h * w + d, 0.0f);
+        for (int e = threadIdx.x; a.lse && e < a.group; e += blockDim.x)
+            a.lse[(int64_t)row * a.n_heads + h * a.group + e] = -INFINITY;
     }
 }
 
@@ -144,6 +144,11 @@ template <int N>
 __device__ __forceinline__ void regs_down() {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
+
+__device__ __forceinline__ void cp_async16(void* dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_addr(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 // 2^k for -126 <= k <= 127
 __device__ __forceinline__ float lq_exp2i(int k) { return __int_as_float((k + 127) << 23); }
@@ -962,39 +967,22 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const __gr
         // q of this warp's 32 rows
         const int first = base_row + i * 128 + w4 * 32;
         if constexpr (PARTS == 1) {
-            // as it is: 16-byte pieces, the warp's lanes along a row
-            const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
-            const int per = hs / 8, total = 32 * per;  // pieces of a row, of the warp
-            constexpr int kAt = 8;
-            for (int p0 = 0; p0 < total; p0 += 32 * kAt) {
-                uint4 v[kAt];
-#pragma unroll
-                for (int u = 0; u < kAt; ++u) {
-                    const int pc = p0 + u * 32 + lane, rr = pc / per, d = (pc - rr * per) * 8;
-                    v[u] = make_uint4(0, 0, 0, 0);
-                    if (pc < total && first + rr < rows) {
-                        const int r = first + rr;
-                        const uint16_t* src = static_cast<const uint16_t*>(a.q) + (int64_t)(q.r0 + r / g) * a.ld_q +
-                                              (int64_t)(h * g + r % g) * hs + d;
-                        if (a.q_vec) {
-                            v[u] = __ldg(reinterpret_cast<const uint4*>(src));
-                        } else {
-                            uint32_t w[4];
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) w[k] = __ldg(src + 2 * k) | (uint32_t)__ldg(src + 2 * k + 1) << 16;
-                            v[u] = make_uint4(w[0], w[1], w[2], w[3]);
-                        }
-                    }
-                }
-#pragma unroll
-                for (int u = 0; u < kAt; ++u) {
-                    const int pc = p0 + u * 32 + lane, rr = pc / per, ck = pc - rr * per, row = w4 * 32 + rr;
-                    if (pc < total)
-                        *reinterpret_cast<uint4*>(sq + i * Lay::kQ + (ck >> 3) * (128 * 128) + row * 128 +
-                                                  (((ck & 7) ^ (row & 7)) << 4)) =
-                            make_uint4(v[u].x ^ flip, v[u].y ^ flip, v[u].z ^ flip, v[u].w ^ flip);
+            // as it is, in 16-byte pieces: a short loop of asynchronous copies (its
+            // unrolled form was bound by fetching instructions that run once)
+            const int per = hs / 8;  // pieces of a row
+#pragma unroll 1
+            for (int pc = lane; pc < 32 * per; pc += 32) {
+                const int rr = pc / per, ck = pc - rr * per, row = w4 * 32 + rr, r = min(first + rr, rows - 1);
+                const uint16_t* src = static_cast<const uint16_t*>(a.q) + (int64_t)(q.r0 + r / g) * a.ld_q +
+                                      (int64_t)(h * g + r % g) * hs + ck * 8;
+                unsigned char* dst = sq + i * Lay::kQ + (ck >> 3) * (128 * 128) + row * 128 + (((ck & 7) ^ (row & 7)) << 4);
+                if (a.q_vec) {
+                    cp_async16(dst, src);
+                } else {
+                    for (int k = 0; k < 8; ++k) reinterpret_cast<uint16_t*>(dst)[k] = __ldg(src + k);
                 }
             }
+            cp_async_wait();
             bars->fs[i * 128 + w4 * 32 + lane] = fabsf(a.scale);
         } else {
             // scaled and split, a few rows at a time (all their loads before the
@@ -1084,6 +1072,12 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const __gr
 #pragma unroll
             for (int c = 0; c < TK / 32; ++c) tmem_ld<32>(ts + c * 32, reinterpret_cast<int(&)[32]>(x[c]));
             tmem_ld_wait();
+            if (PARTS == 1 && a.scale < 0.0f) {  // the factors are positive
+#pragma unroll
+                for (int c = 0; c < TK / 32; ++c)
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) x[c][k] = -x[c][k];
+            }
             if (__any_sync(0xffffffffu, left < TK - 1)) {
 #pragma unroll
                 for (int c = 0; c < TK / 32; ++c)
@@ -1095,12 +1089,10 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const __gr
 #pragma unroll
             for (int e = 0; e < TK / 16; ++e) {
                 const float* y = &x[e / 2][(e & 1) * 16];
-                float t[8];
+                float t[5];
 #pragma unroll
-                for (int k = 0; k < 8; ++k) t[k] = fmaxf(y[k], y[k + 8]);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) t[k] = fmaxf(t[k], t[k + 4]);
-                m = fmaxf(m, fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])) * (fs * gr[e].sk));
+                for (int k = 0; k < 5; ++k) t[k] = max3(y[3 * k], y[3 * k + 1], y[3 * k + 2]);
+                m = fmaxf(m, fmaxf(max3(t[0], t[1], t[2]), max3(t[3], t[4], y[15])) * (fs * gr[e].sk));
             }
             const bool grown = j == 0 ? m > -INFINITY : m > mref + kGrow;
             if (__any_sync(0xffffffffu, grown)) {
@@ -1124,6 +1116,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const __gr
                     }
                 }
             }
+            uint64_t total[2] = {};
 #pragma unroll
             for (int c = 0; c < TK / 32; ++c) {
                 uint32_t hi[16], lo[16];
@@ -1135,28 +1128,30 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const __gr
                     const bool sees = c * 32 + e * 16 <= left;
                     float f = sees ? fs * gg.sk : 1e-38f;
                     if (f == 0.0f) f = 1e-38f;
-                    const float b = gg.shift - mref;
                     if (sees) poison += gg.bad;
-                    float sum[2] = {};
+                    const uint64_t f2 = f2_pack(f, f), b2 = f2_pack(gg.shift - mref, gg.shift - mref);
+                    uint64_t sum[2];
 #pragma unroll
-                    for (int k = 0; k < 16; k += 2) {
-                        const float p0 = exp2_fast(fmaf(x[c][e * 16 + k], f, b));
-                        const float p1 = exp2_fast(fmaf(x[c][e * 16 + k + 1], f, b));
-                        sum[0] += p0;
-                        sum[1] += p1;
-                        const __half2 u = __floats2half2_rn(p0, p1);
-                        hi[e * 8 + k / 2] = *reinterpret_cast<const uint32_t*>(&u);
+                    for (int k = 0; k < 8; ++k) {
+                        const uint64_t z = f2_fma(f2_pack(x[c][e * 16 + 2 * k], x[c][e * 16 + 2 * k + 1]), f2, b2);
+                        const float y[2] = {exp2_fast(f2_lo(z)), exp2_fast(f2_hi(z))};
+                        const uint64_t w = f2_pack(y[0], y[1]);
+                        sum[k & 1] = k < 2 ? w : f2_add(sum[k & 1], w);
+                        hi[e * 8 + k] = pack_word<__half>(y);
                         if (PARTS == 2) {
-                            const float2 fu = __half22float2(u);
-                            const __half2 v = __floats2half2_rn(p0 - fu.x, p1 - fu.y);
-                            lo[e * 8 + k / 2] = *reinterpret_cast<const uint32_t*>(&v);
+                            float u[2];
+                            unpack_word<__half>(hi[e * 8 + k], u);
+                            u[0] = y[0] - u[0];
+                            u[1] = y[1] - u[1];
+                            lo[e * 8 + k] = pack_word<__half>(u);
                         }
                     }
-                    l = fmaf(sum[0] + sum[1], gg.inv, l);
+                    total[e] = f2_fma(f2_add(sum[0], sum[1]), f2_pack(gg.inv, gg.inv), total[e]);
                 }
                 tmem_st16(ts + c * 32, hi);
                 if (PARTS == 2) tmem_st16(ts + c * 32 + 16, lo);
             }
+            l += (f2_lo(total[0]) + f2_hi(total[0])) + (f2_lo(total[1]) + f2_hi(total[1]));
             tmem_st_wait();
             tc_fence_before();
             __syncwarp();
