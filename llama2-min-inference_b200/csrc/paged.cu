@@ -10,15 +10,16 @@
 namespace lq {
 namespace {
 
-constexpr int kAppendThreads = 128;
+constexpr int kAppendThreads = 256;
+constexpr int kAppendWarps = kAppendThreads / 32;
 
 struct AppendArgs {
     PagedKV c;
     KVBatch b;
     KVRows r;
     int* err;
-    int jobs;      // page jobs (per kv head)
-    int q_blocks;  // query blocks per row
+    int kv_blocks;  // blocks for keys and values; the others rotate queries
+    int q_parts;    // warps that share a row of queries
 };
 
 // dims d .. d + 3 of a row, rotated as its position asks.  d is a multiple of
@@ -53,69 +54,209 @@ __device__ __forceinline__ float append_scale(uint32_t amax_bits, float old) {
     return m;
 }
 
-// Blocks [0, jobs * n_kv_heads): one (page, kv head) that receives tokens.
-// Sequence s owns the jobs from row_start[s] / page + 2 s on, which are at
-// least as many as the pages that its rows touch.
-// The other blocks: rotated queries, one row and a slice of its heads each.
+// the last sequence whose key (by its index) is at most `at`, keys ascending; -1: none
+template <typename F>
+__device__ __forceinline__ int find_seq(int n, int at, int lane, F key) {
+    int s = -1;
+    for (int i0 = 0; i0 < n; i0 += 32) {
+        const int c = __popc(__ballot_sync(0xffffffffu, i0 + lane < n && key(i0 + lane) <= at));
+        s += c;
+        if (c < 32) break;
+    }
+    return s;
+}
+
+// A warp's share of a row of queries: 8 dims a lane, 256 neighbouring ones at a
+// time.  The four pairs of 8 dims at d are the table's d / 2 .. d / 2 + 3 for
+// either mode: dims d .. d + 7, or d / 2 .. d / 2 + 3 of both halves.
+template <typename T, bool VEC>
+__device__ __forceinline__ void rotate_queries(const AppendArgs& a, int unit, int lane) {
+    const int hs = a.c.head_size, row = unit / a.q_parts, part = unit - row * a.q_parts;
+    if (row >= a.b.n_rows) return;
+    const int s = find_seq(a.b.n_seqs, row, lane, [&](int i) { return __ldg(a.b.row_start + i); });
+    if (s < 0) return;
+    const SeqRows q = seq_rows(a.b, s, lane == 0 ? a.err : nullptr);
+    if (row < q.r0 || row >= q.r0 + q.n) return;
+    const int pos = q.begin + (row - q.r0);
+    if (a.r.rope && pos >= a.r.rope_rows) {
+        if (lane == 0) set_err(a.err, DEV_BAD_POS);
+        return;
+    }
+    const float4* tab = reinterpret_cast<const float4*>(a.r.rope + (int64_t)pos * hs);
+    const T* x = static_cast<const T*>(a.r.q) + (int64_t)row * a.r.ld_q;
+    T* y = static_cast<T*>(a.r.q_out) + (int64_t)row * a.r.ld_q_out;
+    const int width = a.r.n_heads * hs, step = 256 * a.q_parts;
+    const bool fixed = step % hs == 0;  // a lane's dims are the same in every head: one look at the table
+    float4 t0 = make_float4(1.0f, 0.0f, 1.0f, 0.0f), t1 = t0;
+    int i = part * 256 + lane * 8, d = i % hs;
+    if (a.r.rope && fixed && i < width) {
+        t0 = tab[d / 4];
+        t1 = tab[d / 4 + 1];
+    }
+#pragma unroll 2
+    for (; i < width; i += step) {
+        if (!fixed) {
+            d = i % hs;
+            if (a.r.rope) {
+                t0 = tab[d / 4];
+                t1 = tab[d / 4 + 1];
+            }
+        }
+        const bool halves = a.r.rope_mode == LQ_ROPE_HALVES && a.r.rope;
+        const int e0 = halves ? i - d + d / 2 : i, e1 = halves ? e0 + hs / 2 : i + 4;
+        float u[4], v[4];
+        load_n<4, VEC>(x + e0, u);
+        load_n<4, VEC>(x + e1, v);
+        if (a.r.rope) {
+            const float c[4] = {t0.x, t0.z, t1.x, t1.z}, n[4] = {t0.y, t0.w, t1.y, t1.w};
+            if (halves) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const float p = u[k], q2 = v[k];
+                    u[k] = p * c[k] - q2 * n[k];
+                    v[k] = p * n[k] + q2 * c[k];
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const float p = u[2 * k], q2 = u[2 * k + 1], p3 = v[2 * k], q3 = v[2 * k + 1];
+                    u[2 * k] = p * c[k] - q2 * n[k];
+                    u[2 * k + 1] = p * n[k] + q2 * c[k];
+                    v[2 * k] = p3 * c[k + 2] - q3 * n[k + 2];
+                    v[2 * k + 1] = p3 * n[k + 2] + q3 * c[k + 2];
+                }
+            }
+        }
+        store_n<4, VEC>(y + e0, u);
+        store_n<4, VEC>(y + e1, v);
+    }
+}
+
+// codes of a word at a grown scale
+__device__ __forceinline__ uint32_t again(uint32_t word, float ratio) {
+    uint32_t o[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = (uint32_t)__float2int_rn((float)code_of(word >> (8 * e)) * ratio);
+    return pack8(o[0], o[1], o[2], o[3]);
+}
+
+// the first `keep` bytes of a word (4 and more: all) at a grown scale
+__device__ __forceinline__ uint32_t again(uint32_t word, float ratio, int keep) {
+    const uint32_t mask = keep >= 4 ? 0xFFFFFFFFu : (1u << (8 * keep)) - 1u;
+    return (again(word, ratio) & mask) | (word & ~mask);
+}
+
+// One new token per sequence: a warp per (sequence, kv head), 4 dims a lane.
+// Bound by the chain of dependent loads (lengths, page, scales).
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(kAppendThreads) append_one_kernel(const __grid_constant__ AppendArgs a) {
+    pdl_trigger();
+    pdl_wait();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    if (blockIdx.x >= a.kv_blocks) {
+        rotate_queries<T, VEC>(a, (blockIdx.x - a.kv_blocks) * kAppendWarps + warp, lane);
+        return;
+    }
+    const int hs = a.c.head_size, P = a.c.page_size, H = a.c.n_kv_heads;
+    const int per = (H + kAppendWarps - 1) / kAppendWarps;
+    const int s = blockIdx.x / per, h = blockIdx.x % per * kAppendWarps + warp;
+    if (h >= H) return;
+    int* const err = lane == 0 ? a.err : nullptr;
+    const SeqRows q = seq_rows(a.b, s, err);
+    if (q.n != 1) return;
+    const int pos = q.begin, lp = pos / P, off = pos - lp * P;
+    if (a.r.rope && pos >= a.r.rope_rows) {
+        set_err(err, DEV_BAD_POS);
+        return;
+    }
+    const int64_t page = page_of(a.c, a.b, s, lp, err);
+    const T* kr = static_cast<const T*>(a.r.k) + (int64_t)q.r0 * a.r.ld_k + (int64_t)h * hs;
+    const T* vr = static_cast<const T*>(a.r.v) + (int64_t)q.r0 * a.r.ld_v + (int64_t)h * hs;
+    const float* tab = a.r.rope ? a.r.rope + (int64_t)pos * hs : nullptr;
+    float k[2][4] = {}, v[2][4] = {};
+    uint32_t mk = 0, mv = 0;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int d = i * 128 + lane * 4;
+        if (d < hs) {
+            rotated4<T, VEC>(kr, tab, hs, a.r.rope_mode, d, k[i]);
+            load_n<4, VEC>(vr + d, v[i]);
+        }
+    }
+    if (page < 0) return;
+    const int64_t cell = page * H + h;
+    float2* const sc = reinterpret_cast<float2*>(a.c.scales) + cell;
+    const float2 old = off > 0 ? *sc : make_float2(0.0f, 0.0f);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            mk = max(mk, abs_bits(k[i][e]));
+            mv = max(mv, abs_bits(v[i][e]));
+        }
+    const float sk = append_scale(__reduce_max_sync(0xffffffffu, mk), old.x);
+    const float sv = append_scale(__reduce_max_sync(0xffffffffu, mv), old.y);
+    const Quant8 qk(sk), qv(sv);
+    if (lane == 0) *sc = make_float2(sk, sv);
+    int8_t* kc = static_cast<int8_t*>(a.c.codes) + cell * 2 * hs * P;
+    int8_t* vc = kc + (int64_t)hs * P;
+    if (off > 0 && sk != old.x) {
+        const float ratio = qk.bad ? 0.0f : old.x / sk;
+        for (int i = lane; i < off * (hs / 4); i += 32) {
+            const int t = i % off, w = i / off;
+            uint32_t* p = reinterpret_cast<uint32_t*>(kc + ((int64_t)(w / 4) * P + t) * 16) + (w & 3);
+            *p = again(*p, ratio);
+        }
+    }
+    if (off > 0 && sv != old.y) {
+        const float ratio = qv.bad ? 0.0f : old.y / sv;
+        for (int i = lane; i < (off + 3) / 4 * hs; i += 32) {
+            const int w = i / hs, d = i - w * hs;
+            uint32_t* p = reinterpret_cast<uint32_t*>(vc + ((int64_t)(w / 4) * hs + d) * 16) + (w & 3);
+            *p = again(*p, ratio, off - 4 * w);
+        }
+        __syncwarp();  // the new token's bytes may lie in these words
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int d = i * 128 + lane * 4;
+        if (d >= hs) continue;
+        const uint32_t ck = qk(k[i][0], k[i][1], k[i][2], k[i][3]), cv = qv(v[i][0], v[i][1], v[i][2], v[i][3]);
+        *reinterpret_cast<uint32_t*>(kc + ((int64_t)(d / 16) * P + off) * 16 + d % 16) = ck;
+        int8_t* vp = vc + ((int64_t)(off / 16) * hs + d) * 16 + off % 16;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) vp[16 * e] = (int8_t)(cv >> (8 * e));
+        const int64_t at = (int64_t)q.r0 * a.r.ld_kv_out + (int64_t)h * hs + d;
+        float o[4];
+        if (a.r.k_out) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = (float)code_of(ck >> (8 * e)) * sk;
+            store_n<4, VEC>(static_cast<T*>(a.r.k_out) + at, o);
+        }
+        if (a.r.v_out) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = (float)code_of(cv >> (8 * e)) * sv;
+            store_n<4, VEC>(static_cast<T*>(a.r.v_out) + at, o);
+        }
+    }
+}
+
+// Any rows: a block per (page, kv head) that receives tokens.  Sequence s owns
+// the jobs from row_start[s] / page + 2 s on, which are at least as many as the
+// pages that its rows touch.  The rows are read twice: for the maxima and, from
+// L1 or L2, for the codes.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_constant__ AppendArgs a) {
     pdl_trigger();
     pdl_wait();
-    const int tid = threadIdx.x;
-    const int hs = a.c.head_size, P = a.c.page_size, H = a.c.n_kv_heads;
-    const int64_t kv_blocks = (int64_t)a.jobs * H;
-    if (blockIdx.x >= kv_blocks) {
-        const int64_t qb = blockIdx.x - kv_blocks;
-        const int row = (int)(qb / a.q_blocks), part = (int)(qb % a.q_blocks);
-        int s = -1;  // the last sequence whose rows begin at or before `row`
-        for (int i0 = 0; i0 < a.b.n_seqs; i0 += kAppendThreads) {
-            const int c = __syncthreads_count(i0 + tid < a.b.n_seqs && __ldg(a.b.row_start + i0 + tid) <= row);
-            s += c;
-            if (c < kAppendThreads) break;
-        }
-        if (s < 0) return;
-        const SeqRows q = seq_rows(a.b, s, tid == 0 ? a.err : nullptr);
-        if (row < q.r0 || row >= q.r0 + q.n) return;
-        const int pos = q.begin + (row - q.r0);
-        const float* tab = nullptr;
-        if (a.r.rope) {
-            if (pos >= a.r.rope_rows) {
-                if (tid == 0) set_err(a.err, DEV_BAD_POS);
-                return;
-            }
-            tab = a.r.rope + (int64_t)pos * hs;
-        }
-        const int i = (part * kAppendThreads + tid) * 8;  // 8 dims of a head
-        if (i >= a.r.n_heads * hs) return;
-        const int h = i / hs, d = i - h * hs;
-        const T* x = static_cast<const T*>(a.r.q) + (int64_t)row * a.r.ld_q + (int64_t)h * hs;
-        T* y = static_cast<T*>(a.r.q_out) + (int64_t)row * a.r.ld_q_out + (int64_t)h * hs;
-        // in place, both halves of a pair have to be read before either is written
-        if (a.r.rope_mode == LQ_ROPE_HALVES && tab) {
-            const int half = hs / 2, p0 = d / 2;  // pairs p0 .. p0 + 3
-            float lo[4], hi[4];
-            rotated4<T, VEC>(x, tab, hs, LQ_ROPE_HALVES, p0, lo);
-            rotated4<T, VEC>(x, tab, hs, LQ_ROPE_HALVES, p0 + half, hi);
-            store_n<4, VEC>(y + p0, lo);
-            store_n<4, VEC>(y + p0 + half, hi);
-        } else {
-            float v0[4], v1[4];
-            rotated4<T, VEC>(x, tab, hs, LQ_ROPE_PAIRS, d, v0);
-            rotated4<T, VEC>(x, tab, hs, LQ_ROPE_PAIRS, d + 4, v1);
-            store_n<4, VEC>(y + d, v0);
-            store_n<4, VEC>(y + d + 4, v1);
-        }
+    const int tid = threadIdx.x, lane = tid & 31;
+    if (blockIdx.x >= a.kv_blocks) {
+        rotate_queries<T, VEC>(a, (blockIdx.x - a.kv_blocks) * kAppendWarps + (tid >> 5), lane);
         return;
     }
-
+    const int hs = a.c.head_size, P = a.c.page_size, H = a.c.n_kv_heads;
     const int job = blockIdx.x / H, h = blockIdx.x % H;
-    int s = -1;
-    for (int i0 = 0; i0 < a.b.n_seqs; i0 += kAppendThreads) {
-        const int i = i0 + tid;
-        const int c = __syncthreads_count(i < a.b.n_seqs && __ldg(a.b.row_start + i) / P + 2 * i <= job);
-        s += c;
-        if (c < kAppendThreads) break;
-    }
+    const int s = find_seq(a.b.n_seqs, job, lane, [&](int i) { return __ldg(a.b.row_start + i) / P + 2 * i; });
     if (s < 0) return;
     const SeqRows q = seq_rows(a.b, s, tid == 0 ? a.err : nullptr);
     if (q.n <= 0) return;
@@ -136,10 +277,12 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
     const T* vr = static_cast<const T*>(a.r.v) + (int64_t)row0 * a.r.ld_v + (int64_t)h * hs;
     const float* tab0 = a.r.rope ? a.r.rope + (int64_t)t0 * hs : nullptr;
 
-    // the maxima of the new tokens
+    // the maxima of the new tokens; hw words of 4 dims per token
+    const int hw = hs / 4;
     uint32_t mk = 0, mv = 0;
-    for (int i = tid; i < nt * (hs / 4); i += kAppendThreads) {
-        const int t = i / (hs / 4), d = 4 * (i - t * (hs / 4));
+#pragma unroll 4
+    for (int i = tid; i < nt * hw; i += kAppendThreads) {
+        const int t = i / hw, d = 4 * (i - t * hw);
         float k[4], v[4];
         rotated4<T, VEC>(kr + t * a.r.ld_k, tab0 ? tab0 + (int64_t)t * hs : nullptr, hs, a.r.rope_mode, d, k);
         load_n<4, VEC>(vr + t * a.r.ld_v + d, v);
@@ -149,10 +292,10 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
             mv = max(mv, abs_bits(v[e]));
         }
     }
-    __shared__ uint32_t wk[kAppendThreads / 32], wv[kAppendThreads / 32];
+    __shared__ uint32_t wk[kAppendWarps], wv[kAppendWarps];
     mk = __reduce_max_sync(0xffffffffu, mk);
     mv = __reduce_max_sync(0xffffffffu, mv);
-    if ((tid & 31) == 0) {
+    if (lane == 0) {
         wk[tid >> 5] = mk;
         wv[tid >> 5] = mv;
     }
@@ -163,7 +306,7 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
     }
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < kAppendThreads / 32; ++w) {
+    for (int w = 0; w < kAppendWarps; ++w) {
         mk = max(mk, wk[w]);
         mv = max(mv, wv[w]);
     }
@@ -175,23 +318,18 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
     }
     // earlier tokens at the grown scale (a NaN scale leaves nothing to keep)
     const bool grow_k = off > 0 && sk != old_k, grow_v = off > 0 && sv != old_v;
-    auto again = [](uint32_t word, float ratio) {
-        uint32_t o[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = (uint32_t)__float2int_rn((float)code_of(word >> (8 * e)) * ratio);
-        return pack8(o[0], o[1], o[2], o[3]);
-    };
     if (grow_k) {
         const float ratio = qk.bad ? 0.0f : old_k / sk;
-        for (int i = tid; i < off * (hs / 4); i += kAppendThreads) {
+        for (int i = tid; i < off * hw; i += kAppendThreads) {
             const int t = i % off, w = i / off;  // word w (4 dims) of token t
             uint32_t* p = reinterpret_cast<uint32_t*>(kc + ((int64_t)(w / 4) * P + t) * 16) + (w & 3);
             *p = again(*p, ratio);
         }
     }
     // new keys: 4 dims of a token are one word
-    for (int i = tid; i < nt * (hs / 4); i += kAppendThreads) {
-        const int t = i / (hs / 4), d = 4 * (i - t * (hs / 4));
+#pragma unroll 4
+    for (int i = tid; i < nt * hw; i += kAppendThreads) {
+        const int t = i / hw, d = 4 * (i - t * hw);
         float k[4];
         rotated4<T, VEC>(kr + t * a.r.ld_k, tab0 ? tab0 + (int64_t)t * hs : nullptr, hs, a.r.rope_mode, d, k);
         const uint32_t c = qk(k[0], k[1], k[2], k[3]);
@@ -206,16 +344,13 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
     // last new one, earlier tokens in them kept or rescaled, later bytes kept
     const float ratio_v = qv.bad ? 0.0f : old_v / sv;
     const int w0 = grow_v ? 0 : off / 4, w1 = (off + nt + 3) / 4;
+#pragma unroll 2
     for (int i = tid; i < (w1 - w0) * hs; i += kAppendThreads) {
         const int w = w0 + i / hs, d = i % hs;
         uint32_t* p = reinterpret_cast<uint32_t*>(vc + ((int64_t)(w / 4) * hs + d) * 16) + (w & 3);
         const bool whole = 4 * w >= off && 4 * w + 4 <= off + nt;
         uint32_t word = whole ? 0u : *p;
-        if (grow_v && 4 * w < off) {
-            const int keep = off - 4 * w;  // bytes of earlier tokens
-            const uint32_t mask = keep >= 4 ? 0xFFFFFFFFu : (1u << (8 * keep)) - 1u;
-            word = (again(word, ratio_v) & mask) | (word & ~mask);
-        }
+        if (grow_v && 4 * w < off) word = again(word, ratio_v, off - 4 * w);
         float x[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -237,24 +372,37 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
 }
 
 template <typename T>
-cudaError_t append_t(const AppendArgs& a, cudaStream_t st) {
+cudaError_t append_t(AppendArgs& a, int sms, cudaStream_t st) {
     const KVRows& r = a.r;
     const uintptr_t bytes = 4 * sizeof(T);
     auto fits = [&](const void* p, int64_t ld) { return !p || (reinterpret_cast<uintptr_t>(p) % bytes == 0 && ld % 4 == 0); };
     const bool vec = fits(r.q, r.ld_q) && fits(r.k, r.ld_k) && fits(r.v, r.ld_v) && fits(r.q_out, r.ld_q_out) &&
                      fits(r.k_out, r.ld_kv_out) && fits(r.v_out, r.ld_kv_out);
-    const int64_t blocks = (int64_t)a.jobs * a.c.n_kv_heads + (r.q ? (int64_t)a.b.n_rows * a.q_blocks : 0);
-    if (blocks > INT32_MAX) return cudaErrorInvalidConfiguration;
+    const bool one = a.b.max_rows <= 1;
+    int64_t kv = one ? (int64_t)a.b.n_seqs * ((a.c.n_kv_heads + kAppendWarps - 1) / kAppendWarps)
+                     : ((int64_t)a.b.n_rows / a.c.page_size + 2 * a.b.n_seqs) * a.c.n_kv_heads;
+    // a row of queries is cut into 256-dim parts until there are 8 warps per SM
+    int64_t q_blocks = 0;
+    a.q_parts = 1;
+    if (r.q) {
+        const int most = (r.n_heads * a.c.head_size + 255) / 256, want = 8 * sms / a.b.n_rows;
+        a.q_parts = want < 1 ? 1 : want < most ? want : most;
+        q_blocks = ((int64_t)a.b.n_rows * a.q_parts + kAppendWarps - 1) / kAppendWarps;
+    }
+    if (kv + q_blocks > INT32_MAX) return cudaErrorInvalidConfiguration;
+    a.kv_blocks = (int)kv;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)blocks);
+    cfg.gridDim = dim3((unsigned)(kv + q_blocks));
     cfg.blockDim = dim3(kAppendThreads);
     cfg.stream = st;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return vec ? cudaLaunchKernelEx(&cfg, append_kernel<T, true>, a) : cudaLaunchKernelEx(&cfg, append_kernel<T, false>, a);
+    auto kern = one ? (vec ? append_one_kernel<T, true> : append_one_kernel<T, false>)
+                    : (vec ? append_kernel<T, true> : append_kernel<T, false>);
+    return cudaLaunchKernelEx(&cfg, kern, a);
 }
 
 }  // namespace
@@ -331,12 +479,10 @@ int kv_append(const PagedKV* cache, const KVBatch* batch, const KVRows* rows) {
     a.b = *batch;
     a.r = *rows;
     a.err = c->err;
-    a.jobs = batch->n_rows / cache->page_size + 2 * batch->n_seqs;
-    a.q_blocks = (int)((qd + kAppendThreads * 8 - 1) / (kAppendThreads * 8));
     if (rows->q && rows->n_heads == 0) a.r.q = nullptr;
-    cudaError_t e = rows->type == LQ_F32   ? append_t<float>(a, stream())
-                    : rows->type == LQ_F16 ? append_t<__half>(a, stream())
-                                           : append_t<__nv_bfloat16>(a, stream());
+    cudaError_t e = rows->type == LQ_F32   ? append_t<float>(a, c->num_sms, stream())
+                    : rows->type == LQ_F16 ? append_t<__half>(a, c->num_sms, stream())
+                                           : append_t<__nv_bfloat16>(a, c->num_sms, stream());
     return e == cudaSuccess ? LQ_OK : cuda_fail(e, "kv_append launch");
 }
 
