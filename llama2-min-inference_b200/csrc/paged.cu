@@ -66,10 +66,12 @@ __device__ __forceinline__ int find_seq(int n, int at, int lane, F key) {
     return s;
 }
 
+constexpr int kNoRope = 2;  // MODE: LQ_ROPE_*, or this, or -1 for whichever at run time
+
 // A warp's share of a row of queries: 8 dims a lane, 256 neighbouring ones at a
 // time.  The four pairs of 8 dims at d are the table's d / 2 .. d / 2 + 3 for
 // either mode: dims d .. d + 7, or d / 2 .. d / 2 + 3 of both halves.
-template <typename T, bool VEC>
+template <typename T, bool VEC, int MODE>
 __device__ __forceinline__ void rotate_queries(const AppendArgs& a, int unit, int lane) {
     const int hs = a.c.head_size, row = unit / a.q_parts, part = unit - row * a.q_parts;
     if (row >= a.b.n_rows) return;
@@ -86,47 +88,66 @@ __device__ __forceinline__ void rotate_queries(const AppendArgs& a, int unit, in
     const T* x = static_cast<const T*>(a.r.q) + (int64_t)row * a.r.ld_q;
     T* y = static_cast<T*>(a.r.q_out) + (int64_t)row * a.r.ld_q_out;
     const int width = a.r.n_heads * hs, step = 256 * a.q_parts;
+    const bool turn = MODE < 0 ? a.r.rope != nullptr : MODE != kNoRope;
+    const bool halves = MODE < 0 ? turn && a.r.rope_mode == LQ_ROPE_HALVES : MODE == LQ_ROPE_HALVES;
     const bool fixed = step % hs == 0;  // a lane's dims are the same in every head: one look at the table
     float4 t0 = make_float4(1.0f, 0.0f, 1.0f, 0.0f), t1 = t0;
     int i = part * 256 + lane * 8, d = i % hs;
-    if (a.r.rope && fixed && i < width) {
+    if (turn && fixed && i < width) {
         t0 = tab[d / 4];
         t1 = tab[d / 4 + 1];
     }
-#pragma unroll 2
+    auto turned = [&](float (&u)[4], float (&v)[4]) {
+        if (!turn) return;
+        const float c[4] = {t0.x, t0.z, t1.x, t1.z}, n[4] = {t0.y, t0.w, t1.y, t1.w};
+        if (halves) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float p = u[k], r = v[k];
+                u[k] = p * c[k] - r * n[k];
+                v[k] = p * n[k] + r * c[k];
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const float p = u[2 * k], r = u[2 * k + 1], p2 = v[2 * k], r2 = v[2 * k + 1];
+                u[2 * k] = p * c[k] - r * n[k];
+                u[2 * k + 1] = p * n[k] + r * c[k];
+                v[2 * k] = p2 * c[k + 2] - r2 * n[k + 2];
+                v[2 * k + 1] = p2 * n[k + 2] + r2 * c[k + 2];
+            }
+        }
+    };
+    if (fixed) {
+        const int o0 = halves ? d / 2 - d : 0, o1 = halves ? o0 + hs / 2 : 4;
+        for (; i + 3 * step < width; i += 4 * step) {  // four steps' loads together
+            float u[4][4], v[4][4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                load_n<4, VEC>(x + i + k * step + o0, u[k]);
+                load_n<4, VEC>(x + i + k * step + o1, v[k]);
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                turned(u[k], v[k]);
+                store_n<4, VEC>(y + i + k * step + o0, u[k]);
+                store_n<4, VEC>(y + i + k * step + o1, v[k]);
+            }
+        }
+    }
     for (; i < width; i += step) {
         if (!fixed) {
             d = i % hs;
-            if (a.r.rope) {
+            if (turn) {
                 t0 = tab[d / 4];
                 t1 = tab[d / 4 + 1];
             }
         }
-        const bool halves = a.r.rope_mode == LQ_ROPE_HALVES && a.r.rope;
         const int e0 = halves ? i - d + d / 2 : i, e1 = halves ? e0 + hs / 2 : i + 4;
         float u[4], v[4];
         load_n<4, VEC>(x + e0, u);
         load_n<4, VEC>(x + e1, v);
-        if (a.r.rope) {
-            const float c[4] = {t0.x, t0.z, t1.x, t1.z}, n[4] = {t0.y, t0.w, t1.y, t1.w};
-            if (halves) {
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const float p = u[k], q2 = v[k];
-                    u[k] = p * c[k] - q2 * n[k];
-                    v[k] = p * n[k] + q2 * c[k];
-                }
-            } else {
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    const float p = u[2 * k], q2 = u[2 * k + 1], p3 = v[2 * k], q3 = v[2 * k + 1];
-                    u[2 * k] = p * c[k] - q2 * n[k];
-                    u[2 * k + 1] = p * n[k] + q2 * c[k];
-                    v[2 * k] = p3 * c[k + 2] - q3 * n[k + 2];
-                    v[2 * k + 1] = p3 * n[k + 2] + q3 * c[k + 2];
-                }
-            }
-        }
+        turned(u, v);
         store_n<4, VEC>(y + e0, u);
         store_n<4, VEC>(y + e1, v);
     }
@@ -154,7 +175,7 @@ __global__ void __launch_bounds__(kAppendThreads) append_one_kernel(const __grid
     pdl_wait();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     if (blockIdx.x >= a.kv_blocks) {
-        rotate_queries<T, VEC>(a, (blockIdx.x - a.kv_blocks) * kAppendWarps + warp, lane);
+        rotate_queries<T, VEC, -1>(a, (blockIdx.x - a.kv_blocks) * kAppendWarps + warp, lane);
         return;
     }
     const int hs = a.c.head_size, P = a.c.page_size, H = a.c.n_kv_heads;
@@ -243,15 +264,33 @@ __global__ void __launch_bounds__(kAppendThreads) append_one_kernel(const __grid
 
 // Any rows: a block per (page, kv head) that receives tokens.  Sequence s owns
 // the jobs from row_start[s] / page + 2 s on, which are at least as many as the
-// pages that its rows touch.  The rows are read twice: for the maxima and, from
-// L1 or L2, for the codes.
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_constant__ AppendArgs a) {
+// pages that its rows touch.  The rows are read twice, for the maxima and (from
+// L1 or L2) for the codes, in short loops by many threads: keeping the values in
+// registers between the two unrolled the code, whose instructions run once per
+// block, and was slower (69 us against 45 for 2048 fp32 tokens of 32 heads,
+// without queries).
+// i = q * n + r, advanced by a fixed step without dividing again
+struct Walk {
+    int q, r, dq, dr, n;
+    __device__ Walk(int i, int step, int n_) : q(i / n_), r(i - i / n_ * n_), dq(step / n_), dr(step - step / n_ * n_), n(n_) {}
+    __device__ __forceinline__ void next() {
+        q += dq;
+        r += dr;
+        if (r >= n) {
+            r -= n;
+            ++q;
+        }
+    }
+};
+
+template <typename T, bool VEC, int MODE>
+__global__ void __launch_bounds__(kAppendThreads, 4) append_kernel(const __grid_constant__ AppendArgs a) {
     pdl_trigger();
     pdl_wait();
+    constexpr int threads = kAppendThreads;
     const int tid = threadIdx.x, lane = tid & 31;
     if (blockIdx.x >= a.kv_blocks) {
-        rotate_queries<T, VEC>(a, (blockIdx.x - a.kv_blocks) * kAppendWarps + (tid >> 5), lane);
+        rotate_queries<T, VEC, MODE>(a, (blockIdx.x - a.kv_blocks) * kAppendWarps + (tid >> 5), lane);
         return;
     }
     const int hs = a.c.head_size, P = a.c.page_size, H = a.c.n_kv_heads;
@@ -277,20 +316,38 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
     const T* vr = static_cast<const T*>(a.r.v) + (int64_t)row0 * a.r.ld_v + (int64_t)h * hs;
     const float* tab0 = a.r.rope ? a.r.rope + (int64_t)t0 * hs : nullptr;
 
-    // the maxima of the new tokens; hw words of 4 dims per token
-    const int hw = hs / 4;
+    // K: 4 dims of a token at a time (a word of codes), hw of them per token.
+    // V: 4 tokens of a dim (a word), words wf .. w1 - 1 hold new tokens.
+    const int hw = hs / 4, nk = nt * hw, wf = off / 4, w1 = (off + nt + 3) / 4, nv = (w1 - wf) * hs;
+    const Walk k0(tid, threads, hw), v0(tid, threads, hs);
+    const int mode = MODE < 0 ? a.r.rope_mode : MODE;
+    const bool turn = MODE < 0 ? tab0 != nullptr : MODE != kNoRope;
+    auto load_k = [&](const Walk& i, float (&k)[4]) {
+        rotated4<T, VEC>(kr + i.q * a.r.ld_k, turn ? tab0 + i.q * hs : nullptr, hs, mode, 4 * i.r, k);
+    };
+    auto load_v = [&](const Walk& i, float (&x)[4]) {
+        const int t = 4 * (wf + i.q) - off;
+        const T* p = vr + t * a.r.ld_v + i.r;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = t + e >= 0 && t + e < nt ? to_f32(p[e * a.r.ld_v]) : 0.0f;
+    };
     uint32_t mk = 0, mv = 0;
+    Walk ki = k0, vi = v0;
 #pragma unroll 4
-    for (int i = tid; i < nt * hw; i += kAppendThreads) {
-        const int t = i / hw, d = 4 * (i - t * hw);
+    for (int i = tid; i < nk; i += threads, ki.next()) {
         float k[4], v[4];
-        rotated4<T, VEC>(kr + t * a.r.ld_k, tab0 ? tab0 + (int64_t)t * hs : nullptr, hs, a.r.rope_mode, d, k);
-        load_n<4, VEC>(vr + t * a.r.ld_v + d, v);
+        load_k(ki, k);
+        load_n<4, VEC>(vr + ki.q * a.r.ld_v + 4 * ki.r, v);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             mk = max(mk, abs_bits(k[e]));
             mv = max(mv, abs_bits(v[e]));
         }
+    }
+    float old_k = 0.0f, old_v = 0.0f;  // a page whose first token arrives now starts afresh
+    if (off > 0) {
+        old_k = a.c.scales[cell * 2];
+        old_v = a.c.scales[cell * 2 + 1];
     }
     __shared__ uint32_t wk[kAppendWarps], wv[kAppendWarps];
     mk = __reduce_max_sync(0xffffffffu, mk);
@@ -298,11 +355,6 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
     if (lane == 0) {
         wk[tid >> 5] = mk;
         wv[tid >> 5] = mv;
-    }
-    float old_k = 0.0f, old_v = 0.0f;  // a page whose first token arrives now starts afresh
-    if (off > 0) {
-        old_k = a.c.scales[cell * 2];
-        old_v = a.c.scales[cell * 2 + 1];
     }
     __syncthreads();
 #pragma unroll
@@ -320,54 +372,63 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
     const bool grow_k = off > 0 && sk != old_k, grow_v = off > 0 && sv != old_v;
     if (grow_k) {
         const float ratio = qk.bad ? 0.0f : old_k / sk;
-        for (int i = tid; i < off * hw; i += kAppendThreads) {
+        for (int i = tid; i < off * hw; i += threads) {
             const int t = i % off, w = i / off;  // word w (4 dims) of token t
             uint32_t* p = reinterpret_cast<uint32_t*>(kc + ((int64_t)(w / 4) * P + t) * 16) + (w & 3);
             *p = again(*p, ratio);
         }
     }
-    // new keys: 4 dims of a token are one word
-#pragma unroll 4
-    for (int i = tid; i < nt * hw; i += kAppendThreads) {
-        const int t = i / hw, d = 4 * (i - t * hw);
-        float k[4];
-        rotated4<T, VEC>(kr + t * a.r.ld_k, tab0 ? tab0 + (int64_t)t * hs : nullptr, hs, a.r.rope_mode, d, k);
+    const float ratio_v = qv.bad ? 0.0f : old_v / sv;
+    if (grow_v) {  // whole words of earlier tokens
+        for (int i = tid; i < wf * hs; i += threads) {
+            const int w = i / hs, d = i - w * hs;
+            uint32_t* p = reinterpret_cast<uint32_t*>(vc + ((int64_t)(w / 4) * hs + d) * 16) + (w & 3);
+            *p = again(*p, ratio_v);
+        }
+    }
+    auto store_k = [&](const Walk& i, float (&k)[4]) {
+        const int d = 4 * i.r;
         const uint32_t c = qk(k[0], k[1], k[2], k[3]);
-        *reinterpret_cast<uint32_t*>(kc + ((int64_t)(d / 16) * P + off + t) * 16 + d % 16) = c;
+        *reinterpret_cast<uint32_t*>(kc + ((d >> 4) * P + off + i.q) * 16 + (d & 15)) = c;
         if (a.r.k_out) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) k[e] = (float)code_of(c >> (8 * e)) * sk;
-            store_n<4, VEC>(static_cast<T*>(a.r.k_out) + (int64_t)(row0 + t) * a.r.ld_kv_out + (int64_t)h * hs + d, k);
+            store_n<4, VEC>(static_cast<T*>(a.r.k_out) + (int64_t)(row0 + i.q) * a.r.ld_kv_out + (int64_t)h * hs + d, k);
         }
-    }
-    // values: a word is 4 tokens of a dim; the words that hold tokens up to the
-    // last new one, earlier tokens in them kept or rescaled, later bytes kept
-    const float ratio_v = qv.bad ? 0.0f : old_v / sv;
-    const int w0 = grow_v ? 0 : off / 4, w1 = (off + nt + 3) / 4;
-#pragma unroll 2
-    for (int i = tid; i < (w1 - w0) * hs; i += kAppendThreads) {
-        const int w = w0 + i / hs, d = i % hs;
-        uint32_t* p = reinterpret_cast<uint32_t*>(vc + ((int64_t)(w / 4) * hs + d) * 16) + (w & 3);
-        const bool whole = 4 * w >= off && 4 * w + 4 <= off + nt;
-        uint32_t word = whole ? 0u : *p;
-        if (grow_v && 4 * w < off) word = again(word, ratio_v, off - 4 * w);
-        float x[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int t = 4 * w + e - off;
-            x[e] = t >= 0 && t < nt ? to_f32(vr[t * a.r.ld_v + d]) : 0.0f;
-        }
+    };
+    auto store_v = [&](const Walk& i, const float (&x)[4]) {
+        const int w = wf + i.q;
+        uint32_t* p = reinterpret_cast<uint32_t*>(vc + ((w >> 2) * hs + i.r) * 16) + (w & 3);
         const uint32_t c = qv(x[0], x[1], x[2], x[3]);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int t = 4 * w + e - off;
-            if (t < 0 || t >= nt) continue;
-            word = (word & ~(0xFFu << (8 * e))) | (c & (0xFFu << (8 * e)));
-            if (a.r.v_out)
-                static_cast<T*>(a.r.v_out)[(int64_t)(row0 + t) * a.r.ld_kv_out + (int64_t)h * hs + d] =
-                    from_f32<T>((float)code_of(c >> (8 * e)) * sv);
+        // a word at either end: earlier tokens kept or rescaled, later bytes kept
+        const int lo = max(off - 4 * w, 0), hi = min(off + nt - 4 * w, 4);  // its new bytes
+        uint32_t word = c;
+        if (lo > 0 || hi < 4) {
+            uint32_t was = *p;
+            if (grow_v && lo > 0) was = again(was, ratio_v, lo);
+            const uint32_t mask = (hi >= 4 ? 0xFFFFFFFFu : (1u << (8 * hi)) - 1u) & ~((1u << (8 * lo)) - 1u);
+            word = (c & mask) | (was & ~mask);
         }
         *p = word;
+        if (a.r.v_out) {
+            T* out = static_cast<T*>(a.r.v_out) + (row0 + 4 * w - off) * a.r.ld_kv_out + (int64_t)h * hs + i.r;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (e >= lo && e < hi) out[e * a.r.ld_kv_out] = from_f32<T>((float)code_of(c >> (8 * e)) * sv);
+        }
+    };
+    ki = k0;
+#pragma unroll 4
+    for (int i = tid; i < nk; i += threads, ki.next()) {
+        float k[4];
+        load_k(ki, k);
+        store_k(ki, k);
+    }
+#pragma unroll 2
+    for (int i = tid; i < nv; i += threads, vi.next()) {
+        float x[4];
+        load_v(vi, x);
+        store_v(vi, x);
     }
 }
 
@@ -401,7 +462,10 @@ cudaError_t append_t(AppendArgs& a, int sms, cudaStream_t st) {
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     auto kern = one ? (vec ? append_one_kernel<T, true> : append_one_kernel<T, false>)
-                    : (vec ? append_kernel<T, true> : append_kernel<T, false>);
+                : !vec    ? append_kernel<T, false, -1>
+                : !r.rope ? append_kernel<T, true, kNoRope>
+                : r.rope_mode == LQ_ROPE_HALVES ? append_kernel<T, true, LQ_ROPE_HALVES>
+                                                : append_kernel<T, true, LQ_ROPE_PAIRS>;
     return cudaLaunchKernelEx(&cfg, kern, a);
 }
 
