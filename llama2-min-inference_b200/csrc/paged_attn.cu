@@ -5,15 +5,15 @@
 // written in fixed point, as int8 digits:
 //
 //   q . K:  a row of q is qs * (65536 d1 + 256 d2 + d3), qs = max|q| / (127 *
-//           65536), the digits signed bytes (fp32; two digits for the 16-bit
-//           types).  The digits' dots with the codes are exact; the score is
-//           (65536 D1 + 256 D2 + D3) * qs * scale * s_K[page].
+//           65536), the digits signed bytes.  The digits' dots with the codes are
+//           exact; the score is (65536 D1 + 256 D2 + D3) * qs * scale * s_K[page].
+//           (Two digits would do for outputs of 16 bits, but not for lse.)
 //   p . V:  p * s_V[page] / max s_V of the 32 tokens is in [0, 1] and becomes 24
-//           (or 16) bits, whose bytes are unsigned digits.
+//           bits (16 for the 16-bit types), whose bytes are unsigned digits.
 //
-// A product's error so is 2^-25 of the row's largest term (2^-17 for the
-// 16-bit types, whose results carry 2^-9 or 2^-12), less than the rounding of
-// an fp32 sum.  Softmax statistics and the output's accumulator are fp32.
+// A product's error so is 2^-24 of the row's largest term (2^-17 in p . V of the
+// 16-bit types, whose results carry 2^-9 or 2^-12), as the rounding of an fp32
+// sum.  Softmax statistics and the output's accumulator are fp32.
 #include <cmath>
 
 #include "lq_ctx.h"
@@ -209,10 +209,11 @@ constexpr int few_smem() {
     return kFewWarps * kSlots * kItem * HS * 2;
 }
 
+// ND: digits of the weights
 template <int ND, int HS, bool EXACT>
 __global__ void __launch_bounds__(kFewThreads, HS <= 128 ? 3 : 1) attend_few_kernel(const __grid_constant__ AttArgs a) {
     constexpr int KS = HS / 32;       // k steps of q . K
-    constexpr int NP = ND == 3 ? 2 : 1;  // MMAs per tile
+    constexpr int NP = 2;             // MMAs of a tile of q . K: two digits, the third
     constexpr int NT = HS / 8;        // column tiles of p . V
     extern __shared__ __align__(128) unsigned char ring_all[];
     __shared__ uint4 qfrag[KS * NP * 32];
@@ -310,7 +311,7 @@ __global__ void __launch_bounds__(kFewThreads, HS <= 128 ? 3 : 1) attend_few_ker
             for (int e = 0; e < 4; ++e) m = max(m, abs_bits(x[b][e]));
         }
         m = __reduce_max_sync(0xffffffffu, m);
-        constexpr float kTop = ND == 3 ? 8323072.0f : 32512.0f;  // 127 * 256^(ND - 1)
+        constexpr float kTop = 8323072.0f;  // 127 * 256^2
         const float peak = __uint_as_float(m);
         const bool fine = m < kInfBits && peak > 1e-30f;
         const float inv = fine ? kTop / peak : 0.0f;
@@ -323,11 +324,9 @@ __global__ void __launch_bounds__(kFewThreads, HS <= 128 ? 3 : 1) attend_few_ker
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 int n = m >= kInfBits ? 0 : __float2int_rn(x[b][e] * inv);
-                if (ND == 3) {
-                    const int d3 = (int)(int8_t)n;
-                    n = (n - d3) >> 8;
-                    w[2] |= (uint32_t)(d3 & 255) << (8 * e);
-                }
+                const int d3 = (int)(int8_t)n;
+                n = (n - d3) >> 8;
+                w[2] |= (uint32_t)(d3 & 255) << (8 * e);
                 const int d2 = (int)(int8_t)n;
                 w[1] |= (uint32_t)(d2 & 255) << (8 * e);
                 w[0] |= (uint32_t)(((n - d2) >> 8) & 255) << (8 * e);
@@ -336,10 +335,8 @@ __global__ void __launch_bounds__(kFewThreads, HS <= 128 ? 3 : 1) attend_few_ker
             uint32_t* f = reinterpret_cast<uint32_t*>(&qfrag[ks * NP * 32 + L]);
             f[half * 2] = w[0];
             f[half * 2 + 1] = w[1];
-            if (ND == 3) {
-                f[32 * 4 + half * 2] = w[2];
-                f[32 * 4 + half * 2 + 1] = 0;
-            }
+            f[32 * 4 + half * 2] = w[2];
+            f[32 * 4 + half * 2 + 1] = 0;
         }
     }
     __syncthreads();
@@ -424,7 +421,7 @@ __global__ void __launch_bounds__(kFewThreads, HS <= 128 ? 3 : 1) attend_few_ker
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     float v = fmaf(unbias(d[i][0][e]), 256.0f, unbias(d[i][0][2 + e]));
-                    if (ND == 3) v = fmaf(v, 256.0f, unbias(d[i][NP - 1][e]));
+                    v = fmaf(v, 256.0f, unbias(d[i][1][e]));
                     v *= f;
                     if (t + e > pos) v = -INFINITY;
                     x[2 * c + i][e] = v;
