@@ -650,9 +650,15 @@ cudaError_t few_launch(const AttArgs& a, dim3 grid, cudaStream_t st) {
 //                    of scores -> 16 of f16 pairs, the second ones for fp32)
 //   warps 8-11       convert codes: global -> registers (a tile ahead) -> f16 in
 //                    shared memory (128-byte swizzle)
-//   warp 12          issues the MMAs: while one row tile is in softmax, the
-//                    other's products run
+//   warp 12 (and 14) issue the MMAs
 //   warp 13          looks up pages and scales, up to four tiles ahead
+//
+// The 16-bit types keep two buffers of scores per row tile, of 64 tokens each:
+// the next scores are computed while softmax is at these, and each row tile
+// has an issuing warp of its own.  fp32's two parts do not leave the tensor
+// pipe the time for such short tiles (an MMA of 64 columns takes as long as one
+// of 128): one buffer of 128 tokens, a row tile's products run while the other
+// is in softmax.
 //
 // s_K multiplies scores by 16-token granules (one FMA with the exponent's
 // shift); s_V enters as its logarithm: a weight's exponent gets log2(s_V / max
@@ -670,7 +676,7 @@ struct Granule {  // 16 tokens
 };
 
 struct ManyBars {
-    uint64_t qfull[2], kfull[2], kempty[2], vfull[2], vempty[2], sfull[2], pfull[2], pvdone[2], done;
+    uint64_t qfull[2], kfull[4], kempty[4], vfull[4], vempty[4], sfull[2][2], pfull[2][2], pvdone[2], done[2];
     uint64_t tabfull[4], tabempty[4];
     uint32_t tmem_base;
     int abort_flag;
@@ -680,14 +686,15 @@ struct ManyBars {
     float fs[256];       // rows' factors of the scores
 };
 
-template <int HS, int TYPE, int NQ, int TK, int NB>
+// NQ row tiles, TK tokens a tile, NS score buffers per row tile, NB buffers of K and of V
+template <int HS, int TYPE, int NQ, int TK, int NS, int NB>
 struct ManyLayout {
     static constexpr int kParts = TYPE == LQ_F32 ? 2 : 1;
     static constexpr int kQ = 128 * HS * 2 * kParts;       // one row tile: [part][64 dims][128][128 bytes]
     static constexpr int kK = TK * HS * 2, kV = TK * HS * 2;
     static constexpr int kSmem = 1024 + NQ * kQ + NB * (kK + kV) + (int)sizeof(ManyBars);
     static_assert(kSmem <= 227 * 1024 && HS % 64 == 0, "shared memory");
-    static_assert(NQ * (TK + HS) <= 512, "tensor memory");
+    static_assert(NQ * (NS * TK + HS) <= 512, "tensor memory");
 };
 
 // 4 codes to 2 x 2 f16: bytes + 128 as the low mantissa of 1024, minus 1152
@@ -722,9 +729,10 @@ __device__ __forceinline__ void put_codes(unsigned char* block, int row, int pai
     *reinterpret_cast<uint4*>(block + (at ^ (pair << 5) ^ 16)) = make_uint4(z.x, z.y, u.x, u.y);
 }
 
-template <int HS, int TYPE, int NQ, int TK, int NB, bool EXACT>
+template <int HS, int TYPE, int NQ, int TK, int NS, int NB, bool EXACT>
 __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const __grid_constant__ AttArgs a) {
-    using Lay = ManyLayout<HS, TYPE, NQ, TK, NB>;
+    using Lay = ManyLayout<HS, TYPE, NQ, TK, NS, NB>;
+    constexpr int kIssuers = NS == 2 ? NQ : 1;  // warps that issue MMAs: one per row tile, or one for all
     constexpr int PARTS = Lay::kParts;
     constexpr bool kBf16 = TYPE == LQ_BF16;
     constexpr int kPieces = HS / 16;  // 16-byte pieces of K (and of V) per converting thread and 128 tokens
@@ -759,19 +767,21 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const __gr
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
             mbar_init(&bars->qfull[i], 4);
-            mbar_init(&bars->kfull[i], 4);
-            mbar_init(&bars->vfull[i], 4);
-            mbar_init(&bars->kempty[i], 1);
-            mbar_init(&bars->vempty[i], 1);
-            mbar_init(&bars->sfull[i], 1);
-            mbar_init(&bars->pfull[i], 4);
+            for (int b = 0; b < 2; ++b) {
+                mbar_init(&bars->sfull[i][b], 1);
+                mbar_init(&bars->pfull[i][b], 4);
+            }
             mbar_init(&bars->pvdone[i], 1);
+            mbar_init(&bars->done[i], 1);
         }
         for (int i = 0; i < 4; ++i) {
             mbar_init(&bars->tabfull[i], 1);
-            mbar_init(&bars->tabempty[i], 1);
+            mbar_init(&bars->tabempty[i], kIssuers);
+            mbar_init(&bars->kfull[i], 4);
+            mbar_init(&bars->vfull[i], 4);
+            mbar_init(&bars->kempty[i], kIssuers);
+            mbar_init(&bars->vempty[i], kIssuers);
         }
-        mbar_init(&bars->done, 1);
         bars->abort_flag = 0;
         bars->peak = 0;
         fence_mbar_init();
@@ -796,10 +806,11 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const __gr
     const float svm = bars->peak ? __uint_as_float(bars->peak) : 1.0f;
     const int8_t* codes = static_cast<const int8_t*>(a.c.codes);
 
-    // 512 threads hold 65536 registers: 2 x 128 x 168 + 128 x 104 + 128 x 72
+    // 512 threads hold 65536 registers; 128 scores a thread take a share of 168
+    constexpr bool kDeal = NS == 1;  // 2 x 128 x 168 + 128 x 104 + 128 x 72
     if (warp >= 8 && warp < 12) {
         // ---------------- conversion ----------------
-        regs_down<104>();
+        if constexpr (kDeal) regs_down<104>();
         const int t = tid - 256;  // 0..127
         uint4 kr[kLoads], vr[kLoads];
         // K: token t (two threads a token for TK of 64, half the dims each)
@@ -862,54 +873,54 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const __gr
             if (j + 1 < tiles) load_v(j + 1);
         }
     } else if (warp >= 12) {
-        regs_down<72>();
-        if (warp == 12) {
+        if constexpr (kDeal) regs_down<72>();
+        if (warp != 13 && (warp - 12) / 2 < kIssuers && warp % 2 == 0) {
         // ---------------- MMA issue ----------------
         // f32 += f16 x f16 (or bf16 x bf16), M 128
         const uint32_t id_s = (1u << 4) | (kBf16 ? (1u << 7) | (1u << 10) : 0u) | ((uint32_t)(TK >> 3) << 17) | (8u << 24);
         const uint32_t id_o = (1u << 4) | ((uint32_t)(hs >> 3) << 17) | (8u << 24);
         const uint64_t dq = smem_desc_sw128(smem_addr(sq)), dk = smem_desc_sw128(smem_addr(sk)),
                        dv = smem_desc_sw128(smem_addr(sv));
-        const int steps = hs / 16;
+        const int steps = hs / 16, me = (warp - 12) / 2;
         bool ok = true;
         auto wait = [&](uint64_t* bar, uint32_t parity, int code) {
             ok = ok && __all_sync(0xffffffffu, qwait(bar, parity, a.err, code, abort_flag));
         };
+        // whether this warp's last use of token tile j is row tile i's
+        auto last_use = [&](int i, int j) { return NS == 2 || i == NQ - 1 || j >= n[NQ - 1]; };
         auto scores = [&](int i, int j) {  // row tile i, token tile j
+            if (NS == 1 && j >= n[i]) return;
             wait(&bars->kfull[j % NB], (uint32_t)((j / NB) & 1), DEV_TIMEOUT_FULL);
             if (!ok) return;
             tc_fence_after();
             if (elect_one()) {
-                const uint32_t dst = tmem + i * TK;
-                const uint64_t kd = dk + (uint32_t)((j % NB) * Lay::kK >> 4);
+                if (j < n[i]) {
+                    const uint32_t dst = tmem + (i * NS + j % NS) * TK;
+                    const uint64_t kd = dk + (uint32_t)((j % NB) * Lay::kK >> 4);
 #pragma unroll
-                for (int p = 0; p < PARTS; ++p) {
-                    const uint64_t qd = dq + (uint32_t)((i * Lay::kQ + p * (Lay::kQ / PARTS)) >> 4);
-                    for (int k = 0; k < steps; ++k)  // 64 dims a block of 128-byte rows, 32 bytes a step
-                        mma_f16(dst, qd + (uint32_t)((k >> 2) * (128 * 128) >> 4) + 2 * (k & 3),
-                                kd + (uint32_t)((k >> 2) * (TK * 128) >> 4) + 2 * (k & 3), id_s, k > 0 || p > 0);
+                    for (int p = 0; p < PARTS; ++p) {
+                        const uint64_t qd = dq + (uint32_t)((i * Lay::kQ + p * (Lay::kQ / PARTS)) >> 4);
+                        for (int k = 0; k < steps; ++k)  // 64 dims a block of 128-byte rows, 32 bytes a step
+                            mma_f16(dst, qd + (uint32_t)((k >> 2) * (128 * 128) >> 4) + 2 * (k & 3),
+                                    kd + (uint32_t)((k >> 2) * (TK * 128) >> 4) + 2 * (k & 3), id_s, k > 0 || p > 0);
+                    }
+                    mma_commit(&bars->sfull[i][j % NS]);
+                    if (last_use(i, j)) mma_commit(&bars->kempty[j % NB]);
+                } else {  // not a tile of this row tile's
+                    mbar_arrive(&bars->kempty[j % NB]);
                 }
-                mma_commit(&bars->sfull[i]);
-                if (i == NQ - 1 || j >= n[NQ - 1]) mma_commit(&bars->kempty[j % NB]);
             }
             __syncwarp();
         };
-#pragma unroll
-        for (int i = 0; i < NQ; ++i)
-            if (n[i] > 0) {
-                wait(&bars->qfull[i], 0, DEV_TIMEOUT_FULL);
-                if (ok) scores(i, 0);
-            }
-        for (int j = 0; ok && j < tiles; ++j) {
-#pragma unroll
-            for (int i = 0; i < NQ; ++i) {
-                if (!ok || j >= n[i]) continue;
-                wait(&bars->pfull[i], (uint32_t)(j & 1), DEV_TIMEOUT_FULL);
-                wait(&bars->vfull[j % NB], (uint32_t)((j / NB) & 1), DEV_TIMEOUT_FULL);
-                if (!ok) break;
-                tc_fence_after();
-                if (elect_one()) {
-                    const uint32_t dst = tmem + NQ * TK + i * HS, src = tmem + i * TK;
+        auto values = [&](int i, int j) {
+            if (NS == 1 && j >= n[i]) return;
+            if (j < n[i]) wait(&bars->pfull[i][j % NS], (uint32_t)((j / NS) & 1), DEV_TIMEOUT_FULL);
+            wait(&bars->vfull[j % NB], (uint32_t)((j / NB) & 1), DEV_TIMEOUT_FULL);
+            if (!ok) return;
+            tc_fence_after();
+            if (elect_one()) {
+                if (j < n[i]) {
+                    const uint32_t dst = tmem + NQ * NS * TK + i * HS, src = tmem + (i * NS + j % NS) * TK;
                     const uint64_t vd = dv + (uint32_t)((j % NB) * Lay::kV >> 4);
 #pragma unroll
                     for (int k = 0; k < TK / 16; ++k)
@@ -919,18 +930,42 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const __gr
                                        vd + (uint32_t)((k >> 2) * (hs * 128) >> 4) + 2 * (k & 3), id_o,
                                        j > 0 || k > 0 || p > 0);
                     mma_commit(&bars->pvdone[i]);
-                    if (i == NQ - 1 || j >= n[NQ - 1]) {
+                    if (last_use(i, j)) {
                         mma_commit(&bars->vempty[j % NB]);
                         mma_commit(&bars->tabempty[j & 3]);
                     }
+                } else {
+                    mbar_arrive(&bars->vempty[j % NB]);
+                    mbar_arrive(&bars->tabempty[j & 3]);
                 }
-                __syncwarp();
-                if (j + 1 < n[i]) scores(i, j + 1);
+            }
+            __syncwarp();
+        };
+        if constexpr (NS == 2) {
+            if (n[me] > 0) wait(&bars->qfull[me], 0, DEV_TIMEOUT_FULL);
+            if (ok) scores(me, 0);
+            for (int j = 0; ok && j < tiles; ++j) {
+                if (j + 1 < tiles) scores(me, j + 1);
+                if (ok) values(me, j);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < NQ; ++i)
+                if (ok && n[i] > 0) {
+                    wait(&bars->qfull[i], 0, DEV_TIMEOUT_FULL);
+                    if (ok) scores(i, 0);
+                }
+            for (int j = 0; ok && j < tiles; ++j) {
+#pragma unroll
+                for (int i = 0; i < NQ; ++i) {
+                    if (ok) values(i, j);
+                    if (ok) scores(i, j + 1);
+                }
             }
         }
-        if (elect_one()) mma_commit(&bars->done);
+        if (elect_one()) mma_commit(&bars->done[me]);
         __syncwarp();
-        mbar_wait(&bars->done, 0, a.err, DEV_TIMEOUT_MMA);  // every MMA is done before the memory is freed
+        mbar_wait(&bars->done[me], 0, a.err, DEV_TIMEOUT_MMA);  // every MMA is done before the memory is freed
         } else if (warp == 13) {
         // ---------------- pages and scales ----------------
         for (int j = 0; j < tiles; ++j) {
@@ -957,7 +992,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const __gr
         }
     } else {
         // ---------------- softmax ----------------
-        regs_up<168>();
+        if constexpr (kDeal) regs_up<168>();
         if (warp < 4 * NQ && (warp < 4 ? n[0] : n[NQ - 1]) > 0) {
         const int i = warp >> 2, w4 = warp & 3;
         const int n_i = i == 0 ? n[0] : n[NQ - 1];
@@ -1055,14 +1090,15 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const __gr
         const int row = w4 * 32 + lane, r = base_row + i * 128 + row;
         const int pos = r < rows ? q.begin + r / g : -1;
         const float fs = bars->fs[i * 128 + row];
-        const uint32_t ts = tmem + ((uint32_t)(w4 * 32) << 16) + i * TK;
-        const uint32_t to = tmem + ((uint32_t)(w4 * 32) << 16) + NQ * TK + i * HS;
+                const uint32_t to = tmem + ((uint32_t)(w4 * 32) << 16) + NQ * NS * TK + i * HS;
         float mref = 0.0f, l = 0.0f, poison = 0.0f;
         bool ok = true;
         for (int j = 0; j < n_i; ++j) {
-            ok = __all_sync(0xffffffffu, qwait(&bars->sfull[i], (uint32_t)(j & 1), a.err, DEV_TIMEOUT_TFULL, abort_flag));
+            ok = __all_sync(0xffffffffu, qwait(&bars->sfull[i][j % NS], (uint32_t)((j / NS) & 1), a.err,
+                                                DEV_TIMEOUT_TFULL, abort_flag));
             if (!ok) break;
             tc_fence_after();
+            const uint32_t ts = tmem + ((uint32_t)(w4 * 32) << 16) + (i * NS + j % NS) * TK;
             const Granule* gr = bars->gran[j & 3];
             const int left = pos - j * TK;  // the tile's last token that this row sees
             float x[TK / 32][32];
@@ -1152,7 +1188,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const __gr
             tmem_st_wait();
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&bars->pfull[i]);
+            if (lane == 0) mbar_arrive(&bars->pfull[i][j % NS]);
         }
         if (ok)
             ok = __all_sync(0xffffffffu, qwait(&bars->pvdone[i], (uint32_t)((n_i - 1) & 1), a.err, DEV_TIMEOUT_TFULL, abort_flag));
@@ -1179,10 +1215,10 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const __gr
     }
 }
 
-template <int HS, int TYPE, int NQ, int TK, int NB, bool EXACT>
+template <int HS, int TYPE, int NQ, int TK, int NS, int NB, bool EXACT>
 cudaError_t many_launch_t(const AttArgs& a, cudaStream_t st) {
-    using Lay = ManyLayout<HS, TYPE, NQ, TK, NB>;
-    auto kern = attend_many_kernel<HS, TYPE, NQ, TK, NB, EXACT>;
+    using Lay = ManyLayout<HS, TYPE, NQ, TK, NS, NB>;
+    auto kern = attend_many_kernel<HS, TYPE, NQ, TK, NS, NB, EXACT>;
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Lay::kSmem);
     if (e != cudaSuccess) return e;
     const int64_t x = ((int64_t)a.b.max_rows * a.group + NQ * 128 - 1) / (NQ * 128);
@@ -1205,9 +1241,10 @@ cudaError_t many_launch_t(const AttArgs& a, cudaStream_t st) {
 template <int TYPE>
 cudaError_t many_launch(const AttArgs& a, cudaStream_t st) {
     constexpr bool f32 = TYPE == LQ_F32;
-    if (a.c.head_size == 64) return many_launch_t<64, TYPE, 2, 128, 2, true>(a, st);
-    if (a.c.head_size == 128) return many_launch_t<128, TYPE, 2, 128, f32 ? 1 : 2, true>(a, st);
-    return many_launch_t<256, TYPE, 1, f32 ? 64 : 128, 1, false>(a, st);
+    constexpr int TK = f32 ? 128 : 64, NS = f32 ? 1 : 2;
+    if (a.c.head_size == 64) return many_launch_t<64, TYPE, 2, TK, NS, f32 ? 2 : 4, true>(a, st);
+    if (a.c.head_size == 128) return many_launch_t<128, TYPE, 2, TK, NS, f32 ? 1 : 3, true>(a, st);
+    return many_launch_t<256, TYPE, 1, f32 ? 64 : 128, 1, 1, false>(a, st);
 }
 
 }  // namespace
