@@ -44,7 +44,7 @@ struct AttArgs {
     float scale;      // log2(e) times the caller's
     int row_tiles;    // tiles of 8 (token, head) rows of a sequence and kv head
     int chunk;        // tokens per split
-    float* part;      // [job][split][8][head_size + 8]: out, max, sum
+    float* part;      // [job][split][rows of a tile][head_size + 8]: out, max, sum
     int* cnt;         // [job] arrivals
     int* err;
 };
@@ -179,6 +179,20 @@ __device__ __forceinline__ void mma_u8(int (&d)[4], uint4 a, uint32_t b0, uint32
         : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
 }
 
+// d += a (16 x 32 signed bytes) * b (32 x 8 unsigned bytes)
+__device__ __forceinline__ void mma_s8u8(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.u8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// the largest of a warp's values; a NaN among others is passed over
+__device__ __forceinline__ float max_redux(float v) {
+    float m;
+    asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v));
+    return m;
+}
+
 __device__ __forceinline__ float unbias(int d) { return __int_as_float(d) - kBias; }
 
 // ---------------------------------------------------------------------------
@@ -197,6 +211,13 @@ __device__ __forceinline__ float unbias(int d) { return __int_as_float(d) - kBia
 // p . V) and that the eight rows an ldmatrix reads lie in different banks:
 // column 2j + e of the even tile is token 4j + 2x + e with x = j / 2, of the odd
 // tile with x = 1 - j / 2.
+//
+// Measured, 128 dims: 64 sequences of up to 1100 tokens, 40 heads, fp32 120 us
+// (458 MB, 3.8 TB/s; 16-bit rows 91 us); 16 of up to 4000, 8 kv heads of 8 query
+// heads each, bf16 33 us (86 MB, 2.6 TB/s); one of 2048, 32 heads, fp32 14.5 us,
+// of which 10 us are a launch, the queries, one ring and the join.  What holds the
+// long ones is a step's chain (scores, maximum, weights, products, their unpacking)
+// and its issue slots, with twelve warps on an SM at 168 registers a thread.
 
 constexpr int kFewWarps = 4;
 constexpr int kFewThreads = 32 * kFewWarps;
@@ -209,14 +230,15 @@ constexpr int few_smem() {
     return kFewWarps * kSlots * kItem * HS * 2;
 }
 
-// ND: digits of the weights
-template <int ND, int HS, bool EXACT>
+// ND: digits of the weights.  ROWS: rows of a tile, 8 or 1
+template <int ND, int HS, bool EXACT, int ROWS>
 __global__ void __launch_bounds__(kFewThreads, HS <= 128 ? 3 : 1) attend_few_kernel(const __grid_constant__ AttArgs a) {
     constexpr int KS = HS / 32;       // k steps of q . K
     constexpr int NP = 2;             // MMAs of a tile of q . K: two digits, the third
     constexpr int NT = HS / 8;        // column tiles of p . V
     extern __shared__ __align__(128) unsigned char ring_all[];
-    __shared__ uint4 qfrag[KS * NP * 32];
+    __shared__ uint4 qfrag[ROWS == 8 ? KS * NP * 32 : HS / 4];  // one row: [digit, 4 with zeros][HS / 4] words
+    __shared__ uint4 weights[ROWS == 8 ? 1 : kFewWarps * kItem / 4];
     __shared__ float qscale[8];
     __shared__ uint64_t bars[kFewWarps * kSlots];
     __shared__ int last_flag;
@@ -233,8 +255,8 @@ __global__ void __launch_bounds__(kFewThreads, HS <= 128 ? 3 : 1) attend_few_ker
     const SeqRows q = seq_rows(a.b, s, split == 0 && rt == 0 && h == 0 && tid == 0 ? a.err : nullptr);
     if (split == 0 && rt == 0) zero_rows(a, q, h);
     const int rows = q.n * g;
-    if (rows > a.few_rows || rt * 8 >= rows) return;
-    const int top = min(rows, rt * 8 + 8) - 1;            // the tile's last row
+    if (rows > a.few_rows || rt * ROWS >= rows) return;
+    const int top = min(rows, rt * ROWS + ROWS) - 1;            // the tile's last row
     const int seen = q.begin + top / g + 1;               // tokens that it sees
     const int splits = (seen + a.chunk - 1) / a.chunk;
     if (split >= splits) return;
@@ -289,10 +311,12 @@ __global__ void __launch_bounds__(kFewThreads, HS <= 128 ? 3 : 1) attend_few_ker
     for (int j = 0; j < kSlots; ++j)
         if (j < items) sc_slot[j] = issue(j);
 
-    // the digits of the tile's rows, in the order of the A operand: two rows per warp
+    // the digits of the tile's rows, in the order of the MMA's operand: two rows
+    // per warp, or one by the first warp
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int r8 = 2 * warp + i, r = rt * 8 + r8;
+    for (int i = 0; i < (ROWS == 8 ? 2 : 1); ++i) {
+        if (ROWS == 1 && warp > 0) break;
+        const int r8 = 2 * warp + i, r = rt * ROWS + r8;
         const bool have = r < rows;
         const int64_t base = have ? (int64_t)(q.r0 + r / g) * a.ld_q + (int64_t)(h * g + r % g) * hs : 0;
         float x[(HS + 127) / 128][4];
@@ -331,24 +355,42 @@ __global__ void __launch_bounds__(kFewThreads, HS <= 128 ? 3 : 1) attend_few_ker
                 w[1] |= (uint32_t)(d2 & 255) << (8 * e);
                 w[0] |= (uint32_t)(((n - d2) >> 8) & 255) << (8 * e);
             }
-            const int ks = d / 32, half = d % 32 / 16, L = r8 * 4 + d % 16 / 4;
-            uint32_t* f = reinterpret_cast<uint32_t*>(&qfrag[ks * NP * 32 + L]);
-            f[half * 2] = w[0];
-            f[half * 2 + 1] = w[1];
-            f[32 * 4 + half * 2] = w[2];
-            f[32 * 4 + half * 2 + 1] = 0;
+            if constexpr (ROWS == 8) {
+                const int ks = d / 32, half = d % 32 / 16, L = r8 * 4 + d % 16 / 4;
+                uint32_t* f = reinterpret_cast<uint32_t*>(&qfrag[ks * NP * 32 + L]);
+                f[half * 2] = w[0];
+                f[half * 2 + 1] = w[1];
+                f[32 * 4 + half * 2] = w[2];
+                f[32 * 4 + half * 2 + 1] = 0;
+            } else {
+                uint32_t* f = reinterpret_cast<uint32_t*>(qfrag) + d / 4;
+                f[0] = w[0];
+                f[HS / 4] = w[1];
+                f[HS / 2] = w[2];
+                f[HS / 4 * 3] = 0;
+            }
         }
     }
     __syncthreads();
 
-    const int r8 = lane >> 2, jj = lane & 3;
-    const int r = rt * 8 + r8;
+    const int r8 = ROWS == 8 ? lane >> 2 : 0, jj = lane & 3;
+    const int r = rt * ROWS + r8;
     const int pos = r < rows ? q.begin + r / g : -1;  // the row's last token
     const float fs = qscale[r8];
     float m = -INFINITY, l = 0.0f, poison = 0.0f;
+    // rows of 8: [column tile][2]; one row: [tile of 16 dims][2][2]
     float o[NT][2];
 #pragma unroll
     for (int t = 0; t < NT; ++t) o[t][0] = o[t][1] = 0.0f;
+    uint32_t qd[ROWS == 8 ? 1 : KS][2];  // one row: digit (lane / 4) % 4 of q, the B operand
+    if constexpr (ROWS == 1) {
+        const uint32_t* f = reinterpret_cast<const uint32_t*>(qfrag) + (lane >> 2 & 3) * (HS / 4) + jj;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            qd[ks][0] = f[ks * 8];
+            qd[ks][1] = f[ks * 8 + 4];
+        }
+    }
 
     // strides of an item in shared memory: 16 tokens on, 16 dims on (K), V's start
     const int cell = hs * P * 2;
@@ -390,100 +432,171 @@ __global__ void __launch_bounds__(kFewThreads, HS <= 128 ? 3 : 1) attend_few_ker
                 sv[c] = 0.0f;
             }
         const float svm = fmaxf(sv[0], sv[1]);
-        float top_new = m;
-        float x[4][2];
+        if constexpr (ROWS == 1) {
+            // scores: the codes of 16 tokens are the A operand, q's digits the
+            // columns 0-2 and, again, 4-6.  A lane so finds one digit pair or third
+            // digit of four tokens, and trades with its neighbour for one token whole.
+            int d[2][4];
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {  // 16 tokens: tiles 2c and 2c + 1
-            int d[2][NP][4];
+            for (int c = 0; c < 2; ++c)
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int p = 0; p < NP; ++p)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) d[i][p][e] = kBiasBits;
+                for (int e = 0; e < 4; ++e) d[c][e] = kBiasBits;
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
                 if (!EXACT && ks * 32 >= hs) break;
-                uint32_t b[4];
-                const int chunk = EXACT ? 2 * ks + (mi & 1) : min(2 * ks + (mi & 1), last_chunk);
-                ldsm4(base + c * k16 + chunk * kc + ktok * 16, b);
+                const int chunk = EXACT ? 2 * ks + (mi >> 1) : min(2 * ks + (mi >> 1), last_chunk);
 #pragma unroll
-                for (int p = 0; p < NP; ++p) {
-                    const uint4 f = qfrag[(ks * NP + p) * 32 + lane];
-                    mma_s8(d[0][p], f, b[0], b[1]);
-                    mma_s8(d[1][p], f, b[2], b[3]);
+                for (int c = 0; c < 2; ++c) {
+                    uint32_t k[4];
+                    ldsm4(base + c * k16 + chunk * kc + ((mi & 1) * 8 + mr) * 16, k);
+                    mma_s8(d[c], make_uint4(k[0], k[1], k[2], k[3]), qd[ks][0], qd[ks][1]);
                 }
             }
-            const float f = fs * sk[c];
+            const bool odd = jj & 1, late = jj >> 1;  // the lane's token: 16 late + 8 odd + lane / 4
+            float y[4];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int t = t0 + 16 * c + 4 * jj + 2 * (i ? 1 - (jj >> 1) : jj >> 1);
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    float v = fmaf(unbias(d[i][0][e]), 256.0f, unbias(d[i][0][2 + e]));
-                    v = fmaf(v, 256.0f, unbias(d[i][1][e]));
-                    v *= f;
-                    if (t + e > pos) v = -INFINITY;
-                    x[2 * c + i][e] = v;
-                    top_new = fmaxf(top_new, v);
-                }
-            }
-        }
-        top_new = fmaxf(top_new, __shfl_xor_sync(0xffffffffu, top_new, 1));
-        top_new = fmaxf(top_new, __shfl_xor_sync(0xffffffffu, top_new, 2));
-        const float mref = top_new == -INFINITY ? 0.0f : top_new;
-        const float corr = exp2_fast(m - mref);  // 0 for the first tokens
-        m = top_new;
-        l *= corr;
-        // weights in fixed point; their bytes are the A operand
-        uint4 pa, pb;
-        uint32_t* pw[2] = {reinterpret_cast<uint32_t*>(&pa), reinterpret_cast<uint32_t*>(&pb)};
-        pb = make_uint4(0, 0, 0, 0);
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
+            for (int e = 0; e < 4; ++e) y[e] = unbias(late ? d[1][e] : d[0][e]);
+            const float y0 = odd ? y[0] : fmaf(y[0], 256.0f, y[1]), y1 = odd ? y[2] : fmaf(y[2], 256.0f, y[3]);
+            const float mine = odd ? y1 : y0, other = __shfl_xor_sync(0xffffffffu, odd ? y0 : y1, 1);
+            float x = (odd ? fmaf(other, 256.0f, mine) : fmaf(mine, 256.0f, other)) * (fs * (late ? sk[1] : sk[0]));
+            const int at = 16 * late + 8 * odd + (lane >> 2);
+            if (t0 + at > pos) x = -INFINITY;
+            const float top_new = fmaxf(m, max_redux(x));
+            const float mref = top_new == -INFINITY ? 0.0f : top_new;
+            const float corr = exp2_fast(m - mref);  // 0 for the first tokens
+            m = top_new;
+            const float p = exp2_fast(x - mref);
+            l = fmaf(l, corr, p);
+            // the weight in fixed point; its bytes are the B operand's columns
             constexpr float kOne = ND == 3 ? 16777215.0f : 65535.0f;
-            const float w = svm > 0.0f ? sv[c] / svm * kOne : 0.0f;
-            uint32_t u[2][2];
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const float p = exp2_fast(x[2 * c + i][e] - mref);
-                    l += p;
-                    u[i][e] = ND == 3 ? __float2uint_rn(p * w) : __float_as_uint(p * w + 8388608.0f);
-                }
-            const uint32_t order = jj < 2 ? 0x5410u : 0x1054u;
-#pragma unroll
-            for (int k = 0; k < ND; ++k) {  // byte ND - 1 - k of the four weights
-                const uint32_t sel = ((4u + ND - 1 - k) << 4) | (ND - 1 - k);
-                const uint32_t word = __byte_perm(__byte_perm(u[0][0], u[0][1], sel), __byte_perm(u[1][0], u[1][1], sel), order);
-                if (k < 2)
-                    pw[0][c * 2 + k] = word;
-                else
-                    pw[1][c * 2] = word;
-            }
-        }
-        const float of = svm * (ND == 3 ? 1.0f / 16777215.0f : 1.0f / 65535.0f);
-        const bool turn = __any_sync(0xffffffffu, corr != 1.0f);
-#pragma unroll
-        for (int t = 0; t < NT; t += 2) {
-            if (!EXACT && t * 8 >= hs) break;
-            uint32_t b[4];
-            ldsm4(base + v0 + (mi & 1) * v16 + ((t + (mi >> 1)) * 8 + mr) * 16, b);
+            const float w = p * (svm > 0.0f ? (late ? sv[1] : sv[0]) / svm * kOne : 0.0f);
+            uint32_t* wt = reinterpret_cast<uint32_t*>(weights) + warp * kItem;
+            wt[at] = ND == 3 ? __float2uint_rn(w) : __float_as_uint(w + 8388608.0f);
+            __syncwarp();
+            uint32_t b[2];
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                int d[4] = {kBiasBits, kBiasBits, kBiasBits, kBiasBits}, d3[4] = {kBiasBits, kBiasBits, kBiasBits, kBiasBits};
-                mma_u8(d, pa, b[2 * i], b[2 * i + 1]);
-                if (ND == 3) mma_u8(d3, pb, b[2 * i], b[2 * i + 1]);
-                if (turn) {
-                    o[t + i][0] *= corr;
-                    o[t + i][1] *= corr;
-                }
+                const uint4 u = weights[warp * (kItem / 4) + 4 * i + jj];
+                const int byte = ND - 1 - min(lane >> 2, ND - 1);
+                const uint32_t sel = ((4u + byte) << 4) | byte;
+                b[i] = __byte_perm(__byte_perm(u.x, u.y, sel), __byte_perm(u.z, u.w, sel), 0x5410u);
+                if (lane >> 2 >= ND) b[i] = 0;
+            }
+            const float of = svm * (ND == 3 ? 1.0f / 16777215.0f : 1.0f / 65535.0f);
+            const bool turn = corr != 1.0f;  // alike in all lanes
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    float v = fmaf(unbias(d[e]), 256.0f, unbias(d[2 + e]));
-                    if (ND == 3) v = fmaf(v, 256.0f, unbias(d3[e]));
-                    o[t + i][e] = fmaf(v, of, o[t + i][e]);
+            for (int t = 0; t < NT; t += 2) {
+                if (!EXACT && t * 8 >= hs) break;
+                uint32_t v[4];
+                int e4[4] = {kBiasBits, kBiasBits, kBiasBits, kBiasBits};
+                ldsm4(base + v0 + (mi >> 1) * v16 + (t * 8 + (mi & 1) * 8 + mr) * 16, v);
+                mma_s8u8(e4, v, b[0], b[1]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float& f = o[t + (e >> 1)][e & 1];
+                    if (turn) f *= corr;
+                    f = fmaf(unbias(e4[e]), of, f);
+                }
+            }
+            __syncwarp();  // the weights are read
+        } else {
+            float top_new = m;
+            float x[4][2];
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {  // 16 tokens: tiles 2c and 2c + 1
+                int d[2][NP][4];
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int p = 0; p < NP; ++p)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) d[i][p][e] = kBiasBits;
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) {
+                    if (!EXACT && ks * 32 >= hs) break;
+                    uint32_t b[4];
+                    const int chunk = EXACT ? 2 * ks + (mi & 1) : min(2 * ks + (mi & 1), last_chunk);
+                    ldsm4(base + c * k16 + chunk * kc + ktok * 16, b);
+#pragma unroll
+                    for (int p = 0; p < NP; ++p) {
+                        const uint4 f = qfrag[(ks * NP + p) * 32 + lane];
+                        mma_s8(d[0][p], f, b[0], b[1]);
+                        mma_s8(d[1][p], f, b[2], b[3]);
+                    }
+                }
+                const float f = fs * sk[c];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int t = t0 + 16 * c + 4 * jj + 2 * (i ? 1 - (jj >> 1) : jj >> 1);
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        float v = fmaf(unbias(d[i][0][e]), 256.0f, unbias(d[i][0][2 + e]));
+                        v = fmaf(v, 256.0f, unbias(d[i][1][e]));
+                        v *= f;
+                        if (t + e > pos) v = -INFINITY;
+                        x[2 * c + i][e] = v;
+                        top_new = fmaxf(top_new, v);
+                    }
+                }
+            }
+            top_new = fmaxf(top_new, __shfl_xor_sync(0xffffffffu, top_new, 1));
+            top_new = fmaxf(top_new, __shfl_xor_sync(0xffffffffu, top_new, 2));
+            const float mref = top_new == -INFINITY ? 0.0f : top_new;
+            const float corr = exp2_fast(m - mref);  // 0 for the first tokens
+            m = top_new;
+            l *= corr;
+            // weights in fixed point; their bytes are the A operand
+            uint4 pa, pb;
+            uint32_t* pw[2] = {reinterpret_cast<uint32_t*>(&pa), reinterpret_cast<uint32_t*>(&pb)};
+            pb = make_uint4(0, 0, 0, 0);
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                constexpr float kOne = ND == 3 ? 16777215.0f : 65535.0f;
+                const float w = svm > 0.0f ? sv[c] / svm * kOne : 0.0f;
+                uint32_t u[2][2];
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const float p = exp2_fast(x[2 * c + i][e] - mref);
+                        l += p;
+                        u[i][e] = ND == 3 ? __float2uint_rn(p * w) : __float_as_uint(p * w + 8388608.0f);
+                    }
+                const uint32_t order = jj < 2 ? 0x5410u : 0x1054u;
+#pragma unroll
+                for (int k = 0; k < ND; ++k) {  // byte ND - 1 - k of the four weights
+                    const uint32_t sel = ((4u + ND - 1 - k) << 4) | (ND - 1 - k);
+                    const uint32_t word =
+                        __byte_perm(__byte_perm(u[0][0], u[0][1], sel), __byte_perm(u[1][0], u[1][1], sel), order);
+                    if (k < 2)
+                        pw[0][c * 2 + k] = word;
+                    else
+                        pw[1][c * 2] = word;
+                }
+            }
+            const float of = svm * (ND == 3 ? 1.0f / 16777215.0f : 1.0f / 65535.0f);
+            const bool turn = __any_sync(0xffffffffu, corr != 1.0f);
+#pragma unroll
+            for (int t = 0; t < NT; t += 2) {
+                if (!EXACT && t * 8 >= hs) break;
+                uint32_t b[4];
+                ldsm4(base + v0 + (mi & 1) * v16 + ((t + (mi >> 1)) * 8 + mr) * 16, b);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    int d[4] = {kBiasBits, kBiasBits, kBiasBits, kBiasBits};
+                    int d3[4] = {kBiasBits, kBiasBits, kBiasBits, kBiasBits};
+                    mma_u8(d, pa, b[2 * i], b[2 * i + 1]);
+                    if (ND == 3) mma_u8(d3, pb, b[2 * i], b[2 * i + 1]);
+                    if (turn) {
+                        o[t + i][0] *= corr;
+                        o[t + i][1] *= corr;
+                    }
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        float v = fmaf(unbias(d[e]), 256.0f, unbias(d[2 + e]));
+                        if (ND == 3) v = fmaf(v, 256.0f, unbias(d3[e]));
+                        o[t + i][e] = fmaf(v, of, o[t + i][e]);
+                    }
                 }
             }
         }
@@ -495,50 +608,60 @@ __global__ void __launch_bounds__(kFewThreads, HS <= 128 ? 3 : 1) attend_few_ker
                 sc_slot[1] = sc;
         }
     }
-    l += __shfl_xor_sync(0xffffffffu, l, 1);
-    l += __shfl_xor_sync(0xffffffffu, l, 2);
+    if constexpr (ROWS == 8) {
+        l += __shfl_xor_sync(0xffffffffu, l, 1);
+        l += __shfl_xor_sync(0xffffffffu, l, 2);
+    } else {
+        l = warp_sum(l);
+    }
 
-    // join the warps: [warp][8][hs + 8] over the rings (8 more: a row's stores
+    // join the warps: [warp][ROWS][hs + 8] over the rings (8 more: a row's stores
     // then fall into other banks than its neighbours')
     __syncthreads();
     float* join = reinterpret_cast<float*>(ring_all);
     const int w1 = hs + 8;
     {
-        float* mine = join + (warp * 8 + r8) * w1;
+        float* mine = join + (warp * ROWS + r8) * w1;
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
             if (!EXACT && t * 8 >= hs) break;
-            *reinterpret_cast<float2*>(mine + t * 8 + 2 * jj) = make_float2(o[t][0] + poison, o[t][1] + poison);
+            if constexpr (ROWS == 8) {
+                *reinterpret_cast<float2*>(mine + t * 8 + 2 * jj) = make_float2(o[t][0] + poison, o[t][1] + poison);
+            } else {  // dim 8 t + lane / 4: two digits here, the third by the next lane
+                float v = fmaf(o[t][0], 256.0f, o[t][1]);
+                if (ND == 3) v = fmaf(v, 256.0f, __shfl_down_sync(0xffffffffu, o[t][0], 1));
+                if (jj == 0) mine[t * 8 + (lane >> 2)] = v + poison;
+            }
         }
-        if (jj == 0) {
+        if (ROWS == 8 ? jj == 0 : lane == 0) {
             mine[hs] = m;
             mine[hs + 1] = l;
         }
     }
     __syncthreads();
     const int64_t job = (int64_t)blockIdx.x;
-    float* part = a.part + (job * gridDim.y + split) * 8 * w1;
+    float* part = a.part + (job * gridDim.y + split) * ROWS * w1;
     auto finish = [&](int rr, int d, float v, float mm, float ll) {
         const int row = q.r0 + rr / g, head = h * g + rr % g;
         store_out(a, (int64_t)row * a.ld_out + (int64_t)head * hs + d, v / ll);
         if (a.lse && d == 0) a.lse[(int64_t)row * a.n_heads + head] = (mm + log2f(ll)) * kLn2;
     };
-    const int valid = top + 1 - rt * 8;
+    const int valid = top + 1 - rt * ROWS;
     for (int i = tid; i < valid * hs; i += kFewThreads) {
         const int row8 = i / hs, d = i % hs;
         float mm = -INFINITY, ll = 0.0f, v = 0.0f;
 #pragma unroll
-        for (int w = 0; w < kFewWarps; ++w) mm = fmaxf(mm, join[(w * 8 + row8) * w1 + hs]);
+        for (int w = 0; w < kFewWarps; ++w) mm = fmaxf(mm, join[(w * ROWS + row8) * w1 + hs]);
         const float ref = mm == -INFINITY ? 0.0f : mm;
 #pragma unroll
         for (int w = 0; w < kFewWarps; ++w) {
-            const float* src = join + (w * 8 + row8) * w1;
+            const float* src = join + (w * ROWS + row8) * w1;
             const float c = exp2_fast(src[hs] - ref);
             ll = fmaf(src[hs + 1], c, ll);
             v = fmaf(src[d], c, v);
         }
         if (splits == 1) {
-            finish(rt * 8 + row8, d, v, mm, ll);
+            finish(rt * ROWS + row8, d, v, mm, ll);
         } else {
             __stcg(part + row8 * w1 + d, v);
             if (d == 0) {
@@ -559,14 +682,14 @@ __global__ void __launch_bounds__(kFewThreads, HS <= 128 ? 3 : 1) attend_few_ker
     if (!last_flag) return;
     __threadfence();
     // weights of a row's splits (a warp per row), then the weighted sums
-    const float* all = a.part + job * gridDim.y * 8 * w1;
-    float* weight = join;  // [8][splits], then [8] maxima and [8] sums
-    float *row_max = weight + 8 * splits, *row_sum = row_max + 8;
+    const float* all = a.part + job * gridDim.y * ROWS * w1;
+    float* weight = join;  // [ROWS][splits], then their maxima and sums
+    float *row_max = weight + ROWS * splits, *row_sum = row_max + ROWS;
     for (int row8 = warp; row8 < valid; row8 += kFewWarps) {
         const float* src = all + row8 * w1 + hs;
         float mm = -INFINITY, ll = 0.0f;
         for (int i = lane; i < splits; i += 32) {
-            const float v = __ldcg(src + (int64_t)i * 8 * w1);
+            const float v = __ldcg(src + (int64_t)i * ROWS * w1);
             weight[row8 * splits + i] = v;
             mm = fmaxf(mm, v);
         }
@@ -575,7 +698,7 @@ __global__ void __launch_bounds__(kFewThreads, HS <= 128 ? 3 : 1) attend_few_ker
         for (int i = lane; i < splits; i += 32) {
             const float c = exp2_fast(weight[row8 * splits + i] - ref);
             weight[row8 * splits + i] = c;
-            ll = fmaf(__ldcg(src + (int64_t)i * 8 * w1 + 1), c, ll);
+            ll = fmaf(__ldcg(src + (int64_t)i * ROWS * w1 + 1), c, ll);
         }
         ll = warp_sum(ll);
         if (lane == 0) {
@@ -592,19 +715,19 @@ __global__ void __launch_bounds__(kFewThreads, HS <= 128 ? 3 : 1) attend_few_ker
         for (; k + 8 <= splits; k += 8) {
             float x[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = __ldcg(src + (int64_t)(k + e) * 8 * w1);
+            for (int e = 0; e < 8; ++e) x[e] = __ldcg(src + (int64_t)(k + e) * ROWS * w1);
 #pragma unroll
             for (int e = 0; e < 8; ++e) v = fmaf(x[e], w[k + e], v);
         }
-        for (; k < splits; ++k) v = fmaf(__ldcg(src + (int64_t)k * 8 * w1), w[k], v);
-        finish(rt * 8 + row8, d, v, row_max[row8], row_sum[row8]);
+        for (; k < splits; ++k) v = fmaf(__ldcg(src + (int64_t)k * ROWS * w1), w[k], v);
+        finish(rt * ROWS + row8, d, v, row_max[row8], row_sum[row8]);
     }
 }
 
-template <int ND, int HS, bool EXACT>
+template <int ND, int HS, bool EXACT, int ROWS>
 cudaError_t few_launch(const AttArgs& a, dim3 grid, cudaStream_t st) {
-    auto kern = attend_few_kernel<ND, HS, EXACT>;
-    constexpr int join = kFewWarps * 8 * (HS + 8) * 4;
+    auto kern = attend_few_kernel<ND, HS, EXACT, ROWS>;
+    constexpr int join = kFewWarps * ROWS * (HS + 8) * 4;
     constexpr int smem = few_smem<HS>() > join ? few_smem<HS>() : join;
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e == cudaSuccess)
@@ -623,15 +746,15 @@ cudaError_t few_launch(const AttArgs& a, dim3 grid, cudaStream_t st) {
     return cudaLaunchKernelEx(&cfg, kern, a);
 }
 
-template <int ND>
+template <int ND, int ROWS>
 cudaError_t few_launch(const AttArgs& a, dim3 grid, cudaStream_t st) {
     const int hs = a.c.head_size;
-    if (hs == 64) return few_launch<ND, 64, true>(a, grid, st);
-    if (hs == 128) return few_launch<ND, 128, true>(a, grid, st);
-    if (hs == 256) return few_launch<ND, 256, true>(a, grid, st);
-    if (hs < 64) return few_launch<ND, 64, false>(a, grid, st);
-    if (hs < 128) return few_launch<ND, 128, false>(a, grid, st);
-    return few_launch<ND, 256, false>(a, grid, st);
+    if (hs == 64) return few_launch<ND, 64, true, ROWS>(a, grid, st);
+    if (hs == 128) return few_launch<ND, 128, true, ROWS>(a, grid, st);
+    if (hs == 256) return few_launch<ND, 256, true, ROWS>(a, grid, st);
+    if (hs < 64) return few_launch<ND, 64, false, ROWS>(a, grid, st);
+    if (hs < 128) return few_launch<ND, 128, false, ROWS>(a, grid, st);
+    return few_launch<ND, 256, false, ROWS>(a, grid, st);
 }
 
 // ---------------------------------------------------------------------------
@@ -666,8 +789,15 @@ cudaError_t few_launch(const AttArgs& a, dim3 grid, cudaStream_t st) {
 // out again per granule.  O is rescaled only when a row's maximum has grown by
 // more than 2^13 since its last one: weights are 2^kUnit at that maximum, 2^14 at
 // most, within f16's range.
+//
+// Measured, 1024 rows at the end of 4096 tokens, 32 heads of 128: bf16 132 us
+// (60 GFLOP, 455 TFLOP/s), fp32 153 us; what bounds it is a row tile's chain from
+// scores through softmax to the next product, which two row tiles on an SM hide
+// only in part (tensor pipe and issue slots are both under half busy).  Tiles of
+// 128 tokens with one buffer of scores: bf16 130 us, but f16 with 8 heads to a kv
+// head and pages of 16 176 us against 164, and head size 64 103 us against 98.
 
-constexpr int kManyWarps = 16;  // the last two idle: registers are dealt to warpgroups
+constexpr int kManyWarps = 16;  // whole warpgroups, as registers are dealt to them
 constexpr int kManyThreads = 32 * kManyWarps;
 constexpr float kGrow = 13.0f, kUnit = 1.0f;
 
@@ -875,336 +1005,339 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const __gr
     } else if (warp >= 12) {
         if constexpr (kDeal) regs_down<72>();
         if (warp != 13 && (warp - 12) / 2 < kIssuers && warp % 2 == 0) {
-        // ---------------- MMA issue ----------------
-        // f32 += f16 x f16 (or bf16 x bf16), M 128
-        const uint32_t id_s = (1u << 4) | (kBf16 ? (1u << 7) | (1u << 10) : 0u) | ((uint32_t)(TK >> 3) << 17) | (8u << 24);
-        const uint32_t id_o = (1u << 4) | ((uint32_t)(hs >> 3) << 17) | (8u << 24);
-        const uint64_t dq = smem_desc_sw128(smem_addr(sq)), dk = smem_desc_sw128(smem_addr(sk)),
-                       dv = smem_desc_sw128(smem_addr(sv));
-        const int steps = hs / 16, me = (warp - 12) / 2;
-        bool ok = true;
-        auto wait = [&](uint64_t* bar, uint32_t parity, int code) {
-            ok = ok && __all_sync(0xffffffffu, qwait(bar, parity, a.err, code, abort_flag));
-        };
-        // whether this warp's last use of token tile j is row tile i's
-        auto last_use = [&](int i, int j) { return NS == 2 || i == NQ - 1 || j >= n[NQ - 1]; };
-        auto scores = [&](int i, int j) {  // row tile i, token tile j
-            if (NS == 1 && j >= n[i]) return;
-            wait(&bars->kfull[j % NB], (uint32_t)((j / NB) & 1), DEV_TIMEOUT_FULL);
-            if (!ok) return;
-            tc_fence_after();
-            if (elect_one()) {
-                if (j < n[i]) {
-                    const uint32_t dst = tmem + (i * NS + j % NS) * TK;
-                    const uint64_t kd = dk + (uint32_t)((j % NB) * Lay::kK >> 4);
-#pragma unroll
-                    for (int p = 0; p < PARTS; ++p) {
-                        const uint64_t qd = dq + (uint32_t)((i * Lay::kQ + p * (Lay::kQ / PARTS)) >> 4);
-                        for (int k = 0; k < steps; ++k)  // 64 dims a block of 128-byte rows, 32 bytes a step
-                            mma_f16(dst, qd + (uint32_t)((k >> 2) * (128 * 128) >> 4) + 2 * (k & 3),
-                                    kd + (uint32_t)((k >> 2) * (TK * 128) >> 4) + 2 * (k & 3), id_s, k > 0 || p > 0);
+            // ---------------- MMA issue ----------------
+            // f32 += f16 x f16 (or bf16 x bf16), M 128
+            const uint32_t id_s =
+                (1u << 4) | (kBf16 ? (1u << 7) | (1u << 10) : 0u) | ((uint32_t)(TK >> 3) << 17) | (8u << 24);
+            const uint32_t id_o = (1u << 4) | ((uint32_t)(hs >> 3) << 17) | (8u << 24);
+            const uint64_t dq = smem_desc_sw128(smem_addr(sq)), dk = smem_desc_sw128(smem_addr(sk)),
+                           dv = smem_desc_sw128(smem_addr(sv));
+            const int steps = hs / 16, me = (warp - 12) / 2;
+            bool ok = true;
+            auto wait = [&](uint64_t* bar, uint32_t parity, int code) {
+                ok = ok && __all_sync(0xffffffffu, qwait(bar, parity, a.err, code, abort_flag));
+            };
+            // whether this warp's last use of token tile j is row tile i's
+            auto last_use = [&](int i, int j) { return NS == 2 || i == NQ - 1 || j >= n[NQ - 1]; };
+            auto scores = [&](int i, int j) {  // row tile i, token tile j
+                if (NS == 1 && j >= n[i]) return;
+                wait(&bars->kfull[j % NB], (uint32_t)((j / NB) & 1), DEV_TIMEOUT_FULL);
+                if (!ok) return;
+                tc_fence_after();
+                if (elect_one()) {
+                    if (j < n[i]) {
+                        const uint32_t dst = tmem + (i * NS + j % NS) * TK;
+                        const uint64_t kd = dk + (uint32_t)((j % NB) * Lay::kK >> 4);
+    #pragma unroll
+                        for (int p = 0; p < PARTS; ++p) {
+                            const uint64_t qd = dq + (uint32_t)((i * Lay::kQ + p * (Lay::kQ / PARTS)) >> 4);
+                            for (int k = 0; k < steps; ++k)  // 64 dims a block of 128-byte rows, 32 bytes a step
+                                mma_f16(dst, qd + (uint32_t)((k >> 2) * (128 * 128) >> 4) + 2 * (k & 3),
+                                        kd + (uint32_t)((k >> 2) * (TK * 128) >> 4) + 2 * (k & 3), id_s, k > 0 || p > 0);
+                        }
+                        mma_commit(&bars->sfull[i][j % NS]);
+                        if (last_use(i, j)) mma_commit(&bars->kempty[j % NB]);
+                    } else {  // not a tile of this row tile's
+                        mbar_arrive(&bars->kempty[j % NB]);
                     }
-                    mma_commit(&bars->sfull[i][j % NS]);
-                    if (last_use(i, j)) mma_commit(&bars->kempty[j % NB]);
-                } else {  // not a tile of this row tile's
-                    mbar_arrive(&bars->kempty[j % NB]);
                 }
-            }
-            __syncwarp();
-        };
-        auto values = [&](int i, int j) {
-            if (NS == 1 && j >= n[i]) return;
-            if (j < n[i]) wait(&bars->pfull[i][j % NS], (uint32_t)((j / NS) & 1), DEV_TIMEOUT_FULL);
-            wait(&bars->vfull[j % NB], (uint32_t)((j / NB) & 1), DEV_TIMEOUT_FULL);
-            if (!ok) return;
-            tc_fence_after();
-            if (elect_one()) {
-                if (j < n[i]) {
-                    const uint32_t dst = tmem + NQ * NS * TK + i * HS, src = tmem + (i * NS + j % NS) * TK;
-                    const uint64_t vd = dv + (uint32_t)((j % NB) * Lay::kV >> 4);
-#pragma unroll
-                    for (int k = 0; k < TK / 16; ++k)
-#pragma unroll
-                        for (int p = 0; p < PARTS; ++p)
-                            mma_f16_ts(dst, src + (k >> 1) * 32 + p * 16 + (k & 1) * 8,
-                                       vd + (uint32_t)((k >> 2) * (hs * 128) >> 4) + 2 * (k & 3), id_o,
-                                       j > 0 || k > 0 || p > 0);
-                    mma_commit(&bars->pvdone[i]);
-                    if (last_use(i, j)) {
-                        mma_commit(&bars->vempty[j % NB]);
-                        mma_commit(&bars->tabempty[j & 3]);
+                __syncwarp();
+            };
+            auto values = [&](int i, int j) {
+                if (NS == 1 && j >= n[i]) return;
+                if (j < n[i]) wait(&bars->pfull[i][j % NS], (uint32_t)((j / NS) & 1), DEV_TIMEOUT_FULL);
+                wait(&bars->vfull[j % NB], (uint32_t)((j / NB) & 1), DEV_TIMEOUT_FULL);
+                if (!ok) return;
+                tc_fence_after();
+                if (elect_one()) {
+                    if (j < n[i]) {
+                        const uint32_t dst = tmem + NQ * NS * TK + i * HS, src = tmem + (i * NS + j % NS) * TK;
+                        const uint64_t vd = dv + (uint32_t)((j % NB) * Lay::kV >> 4);
+    #pragma unroll
+                        for (int k = 0; k < TK / 16; ++k)
+    #pragma unroll
+                            for (int p = 0; p < PARTS; ++p)
+                                mma_f16_ts(dst, src + (k >> 1) * 32 + p * 16 + (k & 1) * 8,
+                                           vd + (uint32_t)((k >> 2) * (hs * 128) >> 4) + 2 * (k & 3), id_o,
+                                           j > 0 || k > 0 || p > 0);
+                        mma_commit(&bars->pvdone[i]);
+                        if (last_use(i, j)) {
+                            mma_commit(&bars->vempty[j % NB]);
+                            mma_commit(&bars->tabempty[j & 3]);
+                        }
+                    } else {
+                        mbar_arrive(&bars->vempty[j % NB]);
+                        mbar_arrive(&bars->tabempty[j & 3]);
                     }
-                } else {
-                    mbar_arrive(&bars->vempty[j % NB]);
-                    mbar_arrive(&bars->tabempty[j & 3]);
+                }
+                __syncwarp();
+            };
+            if constexpr (NS == 2) {
+                if (n[me] > 0) wait(&bars->qfull[me], 0, DEV_TIMEOUT_FULL);
+                if (ok) scores(me, 0);
+                for (int j = 0; ok && j < tiles; ++j) {
+                    if (j + 1 < tiles) scores(me, j + 1);
+                    if (ok) values(me, j);
+                }
+            } else {
+    #pragma unroll
+                for (int i = 0; i < NQ; ++i)
+                    if (ok && n[i] > 0) {
+                        wait(&bars->qfull[i], 0, DEV_TIMEOUT_FULL);
+                        if (ok) scores(i, 0);
+                    }
+                for (int j = 0; ok && j < tiles; ++j) {
+    #pragma unroll
+                    for (int i = 0; i < NQ; ++i) {
+                        if (ok) values(i, j);
+                        if (ok) scores(i, j + 1);
+                    }
                 }
             }
+            if (elect_one()) mma_commit(&bars->done[me]);
             __syncwarp();
-        };
-        if constexpr (NS == 2) {
-            if (n[me] > 0) wait(&bars->qfull[me], 0, DEV_TIMEOUT_FULL);
-            if (ok) scores(me, 0);
-            for (int j = 0; ok && j < tiles; ++j) {
-                if (j + 1 < tiles) scores(me, j + 1);
-                if (ok) values(me, j);
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < NQ; ++i)
-                if (ok && n[i] > 0) {
-                    wait(&bars->qfull[i], 0, DEV_TIMEOUT_FULL);
-                    if (ok) scores(i, 0);
-                }
-            for (int j = 0; ok && j < tiles; ++j) {
-#pragma unroll
-                for (int i = 0; i < NQ; ++i) {
-                    if (ok) values(i, j);
-                    if (ok) scores(i, j + 1);
-                }
-            }
-        }
-        if (elect_one()) mma_commit(&bars->done[me]);
-        __syncwarp();
-        mbar_wait(&bars->done[me], 0, a.err, DEV_TIMEOUT_MMA);  // every MMA is done before the memory is freed
+            mbar_wait(&bars->done[me], 0, a.err, DEV_TIMEOUT_MMA);  // every MMA is done before the memory is freed
         } else if (warp == 13) {
-        // ---------------- pages and scales ----------------
-        for (int j = 0; j < tiles; ++j) {
-            const int tok = j * TK + lane * 16;
-            int64_t p = -1;
-            float2 sc = make_float2(NAN, NAN);
-            if (lane < TK / 16 && tok < seen) {
-                p = page_of(a.c, a.b, s, tok >> lp2, a.err);
-                if (p >= 0) sc = __ldg(reinterpret_cast<const float2*>(a.c.scales) + p * H + h);
+            // ---------------- pages and scales ----------------
+            for (int j = 0; j < tiles; ++j) {
+                const int tok = j * TK + lane * 16;
+                int64_t p = -1;
+                float2 sc = make_float2(NAN, NAN);
+                if (lane < TK / 16 && tok < seen) {
+                    p = page_of(a.c, a.b, s, tok >> lp2, a.err);
+                    if (p >= 0) sc = __ldg(reinterpret_cast<const float2*>(a.c.scales) + p * H + h);
+                }
+                const bool fine = sc.y < INFINITY;
+                const float w = fine ? fmaxf(sc.y / svm, 9.094947e-13f) : 1.0f;  // 2^-40 at least
+                const float shift = log2f(w) + kUnit, inv = exp2f(-shift);
+                if (!__all_sync(0xffffffffu, qwait(&bars->tabempty[j & 3], (uint32_t)(((j >> 2) & 1) ^ 1), a.err,
+                                                   DEV_TIMEOUT_EMPTY, abort_flag)))
+                    break;
+                if (lane < TK / 16) {
+                    bars->gran[j & 3][lane] = {sc.x, shift, inv, fine ? 0.0f : NAN};
+                    bars->cell[j & 3][lane] = p >= 0 ? (p * H + h) * (int64_t)(hs * P * 2) : -1;
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bars->tabfull[j & 3]);
             }
-            const bool fine = sc.y < INFINITY;
-            const float w = fine ? fmaxf(sc.y / svm, 9.094947e-13f) : 1.0f;  // 2^-40 at least
-            const float shift = log2f(w) + kUnit, inv = exp2f(-shift);
-            if (!__all_sync(0xffffffffu, qwait(&bars->tabempty[j & 3], (uint32_t)(((j >> 2) & 1) ^ 1), a.err,
-                                               DEV_TIMEOUT_EMPTY, abort_flag)))
-                break;
-            if (lane < TK / 16) {
-                bars->gran[j & 3][lane] = {sc.x, shift, inv, fine ? 0.0f : NAN};
-                bars->cell[j & 3][lane] = p >= 0 ? (p * H + h) * (int64_t)(hs * P * 2) : -1;
-            }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&bars->tabfull[j & 3]);
-        }
         }
     } else {
         // ---------------- softmax ----------------
         if constexpr (kDeal) regs_up<168>();
         if (warp < 4 * NQ && (warp < 4 ? n[0] : n[NQ - 1]) > 0) {
-        const int i = warp >> 2, w4 = warp & 3;
-        const int n_i = i == 0 ? n[0] : n[NQ - 1];
-        // q of this warp's 32 rows
-        const int first = base_row + i * 128 + w4 * 32;
-        if constexpr (PARTS == 1) {
-            // as it is, in 16-byte pieces: a short loop of asynchronous copies (its
-            // unrolled form was bound by fetching instructions that run once)
-            const int per = hs / 8;  // pieces of a row
-#pragma unroll 1
-            for (int pc = lane; pc < 32 * per; pc += 32) {
-                const int rr = pc / per, ck = pc - rr * per, row = w4 * 32 + rr, r = min(first + rr, rows - 1);
-                const uint16_t* src = static_cast<const uint16_t*>(a.q) + (int64_t)(q.r0 + r / g) * a.ld_q +
-                                      (int64_t)(h * g + r % g) * hs + ck * 8;
-                unsigned char* dst = sq + i * Lay::kQ + (ck >> 3) * (128 * 128) + row * 128 + (((ck & 7) ^ (row & 7)) << 4);
-                if (a.q_vec) {
-                    cp_async16(dst, src);
-                } else {
-                    for (int k = 0; k < 8; ++k) reinterpret_cast<uint16_t*>(dst)[k] = __ldg(src + k);
-                }
-            }
-            cp_async_wait();
-            bars->fs[i * 128 + w4 * 32 + lane] = fabsf(a.scale);
-        } else {
-            // scaled and split, a few rows at a time (all their loads before the
-            // first use), 4 dims a lane
-            constexpr int kB = (HS + 127) / 128, kBatch = 8 / kB;
-            int tok = min(first, rows - 1) / g, head = min(first, rows - 1) - tok * g;
-            for (int r0 = 0; r0 < 32; r0 += kBatch) {
-                RawQ<2> raw[kBatch][kB];
-#pragma unroll
-                for (int u = 0; u < kBatch; ++u) {
-                    const int64_t at = (int64_t)(q.r0 + tok) * a.ld_q + (int64_t)(h * g + head) * hs;
-#pragma unroll
-                    for (int b = 0; b < kB; ++b) raw[u][b].load(a, at + min(b * 128 + lane * 4, hs - 4));
-                    if (first + r0 + u + 1 < rows && ++head == g) {
-                        head = 0;
-                        ++tok;
+            const int i = warp >> 2, w4 = warp & 3;
+            const int n_i = i == 0 ? n[0] : n[NQ - 1];
+            // q of this warp's 32 rows
+            const int first = base_row + i * 128 + w4 * 32;
+            if constexpr (PARTS == 1) {
+                // as it is, in 16-byte pieces: a short loop of asynchronous copies (its
+                // unrolled form was bound by fetching instructions that run once)
+                const int per = hs / 8;  // pieces of a row
+    #pragma unroll 1
+                for (int pc = lane; pc < 32 * per; pc += 32) {
+                    const int rr = pc / per, ck = pc - rr * per, row = w4 * 32 + rr, r = min(first + rr, rows - 1);
+                    const uint16_t* src = static_cast<const uint16_t*>(a.q) + (int64_t)(q.r0 + r / g) * a.ld_q +
+                                          (int64_t)(h * g + r % g) * hs + ck * 8;
+                    unsigned char* dst =
+                        sq + i * Lay::kQ + (ck >> 3) * (128 * 128) + row * 128 + (((ck & 7) ^ (row & 7)) << 4);
+                    if (a.q_vec) {
+                        cp_async16(dst, src);
+                    } else {
+                        for (int k = 0; k < 8; ++k) reinterpret_cast<uint16_t*>(dst)[k] = __ldg(src + k);
                     }
                 }
-                float x[kBatch][kB][4];
-#pragma unroll
-                for (int u = 0; u < kBatch; ++u) {
-                    const bool have = first + r0 + u < rows;
-#pragma unroll
-                    for (int b = 0; b < kB; ++b) {
-                        raw[u][b].get(a, x[u][b]);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if (!have || b * 128 + lane * 4 >= hs) x[u][b][e] = 0.0f;
+                cp_async_wait();
+                bars->fs[i * 128 + w4 * 32 + lane] = fabsf(a.scale);
+            } else {
+                // scaled and split, a few rows at a time (all their loads before the
+                // first use), 4 dims a lane
+                constexpr int kB = (HS + 127) / 128, kBatch = 8 / kB;
+                int tok = min(first, rows - 1) / g, head = min(first, rows - 1) - tok * g;
+                for (int r0 = 0; r0 < 32; r0 += kBatch) {
+                    RawQ<2> raw[kBatch][kB];
+    #pragma unroll
+                    for (int u = 0; u < kBatch; ++u) {
+                        const int64_t at = (int64_t)(q.r0 + tok) * a.ld_q + (int64_t)(h * g + head) * hs;
+    #pragma unroll
+                        for (int b = 0; b < kB; ++b) raw[u][b].load(a, at + min(b * 128 + lane * 4, hs - 4));
+                        if (first + r0 + u + 1 < rows && ++head == g) {
+                            head = 0;
+                            ++tok;
+                        }
                     }
-                }
-#pragma unroll
-                for (int u = 0; u < kBatch; ++u) {
-                    const int row = w4 * 32 + r0 + u;
-                    uint32_t m = 0;
-#pragma unroll
-                    for (int b = 0; b < kB; ++b)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) m = max(m, abs_bits(x[u][b][e]));
-                    m = __reduce_max_sync(0xffffffffu, m);
-                    // a power of two that takes the largest into [2^13, 2^14)
-                    int ex = (int)(m >> 23) - 127;
-                    ex = max(-114, min(100, 13 - ex));
-                    const float up = m >= kInfBits ? 0.0f : a.scale < 0.0f ? -lq_exp2i(ex) : lq_exp2i(ex);
-                    if (lane == 0) bars->fs[i * 128 + row] = m >= kInfBits ? NAN : fabsf(a.scale) * lq_exp2i(-ex);
-#pragma unroll
-                    for (int b = 0; b < kB; ++b) {
-                        const int d = b * 128 + lane * 4;
-                        if (d >= hs) continue;
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) x[u][b][e] = up == 0.0f ? 0.0f : x[u][b][e] * up;
-#pragma unroll
-                        for (int p = 0; p < PARTS; ++p) {
-                            const uint32_t w0 = pack_word<__half>(x[u][b]), w1 = pack_word<__half>(x[u][b] + 2);
-                            unsigned char* dst = sq + i * Lay::kQ + p * (Lay::kQ / PARTS) + (d >> 6) * (128 * 128) +
-                                                 row * 128 + ((((d & 63) >> 3) ^ (row & 7)) << 4) + (d & 4) * 2;
-                            *reinterpret_cast<uint2*>(dst) = make_uint2(w0, w1);
-                            if (p + 1 < PARTS) {  // what the first part leaves
-                                float y[4];
-                                unpack_word<__half>(w0, y);
-                                unpack_word<__half>(w1, y + 2);
-#pragma unroll
-                                for (int e = 0; e < 4; ++e) x[u][b][e] -= y[e];
+                    float x[kBatch][kB][4];
+    #pragma unroll
+                    for (int u = 0; u < kBatch; ++u) {
+                        const bool have = first + r0 + u < rows;
+    #pragma unroll
+                        for (int b = 0; b < kB; ++b) {
+                            raw[u][b].get(a, x[u][b]);
+    #pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                if (!have || b * 128 + lane * 4 >= hs) x[u][b][e] = 0.0f;
+                        }
+                    }
+    #pragma unroll
+                    for (int u = 0; u < kBatch; ++u) {
+                        const int row = w4 * 32 + r0 + u;
+                        uint32_t m = 0;
+    #pragma unroll
+                        for (int b = 0; b < kB; ++b)
+    #pragma unroll
+                            for (int e = 0; e < 4; ++e) m = max(m, abs_bits(x[u][b][e]));
+                        m = __reduce_max_sync(0xffffffffu, m);
+                        // a power of two that takes the largest into [2^13, 2^14)
+                        int ex = (int)(m >> 23) - 127;
+                        ex = max(-114, min(100, 13 - ex));
+                        const float up = m >= kInfBits ? 0.0f : a.scale < 0.0f ? -lq_exp2i(ex) : lq_exp2i(ex);
+                        if (lane == 0) bars->fs[i * 128 + row] = m >= kInfBits ? NAN : fabsf(a.scale) * lq_exp2i(-ex);
+    #pragma unroll
+                        for (int b = 0; b < kB; ++b) {
+                            const int d = b * 128 + lane * 4;
+                            if (d >= hs) continue;
+    #pragma unroll
+                            for (int e = 0; e < 4; ++e) x[u][b][e] = up == 0.0f ? 0.0f : x[u][b][e] * up;
+    #pragma unroll
+                            for (int p = 0; p < PARTS; ++p) {
+                                const uint32_t w0 = pack_word<__half>(x[u][b]), w1 = pack_word<__half>(x[u][b] + 2);
+                                unsigned char* dst = sq + i * Lay::kQ + p * (Lay::kQ / PARTS) + (d >> 6) * (128 * 128) +
+                                                     row * 128 + ((((d & 63) >> 3) ^ (row & 7)) << 4) + (d & 4) * 2;
+                                *reinterpret_cast<uint2*>(dst) = make_uint2(w0, w1);
+                                if (p + 1 < PARTS) {  // what the first part leaves
+                                    float y[4];
+                                    unpack_word<__half>(w0, y);
+                                    unpack_word<__half>(w1, y + 2);
+    #pragma unroll
+                                    for (int e = 0; e < 4; ++e) x[u][b][e] -= y[e];
+                                }
                             }
                         }
                     }
                 }
             }
-        }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&bars->qfull[i]);
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars->qfull[i]);
 
-        const int row = w4 * 32 + lane, r = base_row + i * 128 + row;
-        const int pos = r < rows ? q.begin + r / g : -1;
-        const float fs = bars->fs[i * 128 + row];
-                const uint32_t to = tmem + ((uint32_t)(w4 * 32) << 16) + NQ * NS * TK + i * HS;
-        float mref = 0.0f, l = 0.0f, poison = 0.0f;
-        bool ok = true;
-        for (int j = 0; j < n_i; ++j) {
-            ok = __all_sync(0xffffffffu, qwait(&bars->sfull[i][j % NS], (uint32_t)((j / NS) & 1), a.err,
-                                                DEV_TIMEOUT_TFULL, abort_flag));
-            if (!ok) break;
-            tc_fence_after();
-            const uint32_t ts = tmem + ((uint32_t)(w4 * 32) << 16) + (i * NS + j % NS) * TK;
-            const Granule* gr = bars->gran[j & 3];
-            const int left = pos - j * TK;  // the tile's last token that this row sees
-            float x[TK / 32][32];
-#pragma unroll
-            for (int c = 0; c < TK / 32; ++c) tmem_ld<32>(ts + c * 32, reinterpret_cast<int(&)[32]>(x[c]));
-            tmem_ld_wait();
-            if (PARTS == 1 && a.scale < 0.0f) {  // the factors are positive
-#pragma unroll
-                for (int c = 0; c < TK / 32; ++c)
-#pragma unroll
-                    for (int k = 0; k < 32; ++k) x[c][k] = -x[c][k];
-            }
-            if (__any_sync(0xffffffffu, left < TK - 1)) {
-#pragma unroll
-                for (int c = 0; c < TK / 32; ++c)
-#pragma unroll
-                    for (int k = 0; k < 32; ++k)
-                        if (c * 32 + k > left) x[c][k] = -INFINITY;
-            }
-            float m = -INFINITY;
-#pragma unroll
-            for (int e = 0; e < TK / 16; ++e) {
-                const float* y = &x[e / 2][(e & 1) * 16];
-                float t[5];
-#pragma unroll
-                for (int k = 0; k < 5; ++k) t[k] = max3(y[3 * k], y[3 * k + 1], y[3 * k + 2]);
-                m = fmaxf(m, fmaxf(max3(t[0], t[1], t[2]), max3(t[3], t[4], y[15])) * (fs * gr[e].sk));
-            }
-            const bool grown = j == 0 ? m > -INFINITY : m > mref + kGrow;
-            if (__any_sync(0xffffffffu, grown)) {
-                const float next = grown ? m : mref;
-                const float f = exp2_fast(mref - next);
-                mref = next;
-                if (j > 0) {
-                    l *= f;
-                    ok = __all_sync(0xffffffffu, qwait(&bars->pvdone[i], (uint32_t)((j - 1) & 1), a.err, DEV_TIMEOUT_TFULL,
-                                                       abort_flag));
-                    if (!ok) break;
-                    tc_fence_after();
-                    for (int c = 0; c < hs; c += 16) {
-                        int y[16];
-                        tmem_ld<16>(to + c, y);
-                        tmem_ld_wait();
-                        uint32_t z[16];
-#pragma unroll
-                        for (int k = 0; k < 16; ++k) z[k] = __float_as_uint(__int_as_float(y[k]) * f);
-                        tmem_st16(to + c, z);
-                    }
+            const int row = w4 * 32 + lane, r = base_row + i * 128 + row;
+            const int pos = r < rows ? q.begin + r / g : -1;
+            const float fs = bars->fs[i * 128 + row];
+            const uint32_t to = tmem + ((uint32_t)(w4 * 32) << 16) + NQ * NS * TK + i * HS;
+            float mref = 0.0f, l = 0.0f, poison = 0.0f;
+            bool ok = true;
+            for (int j = 0; j < n_i; ++j) {
+                ok = __all_sync(0xffffffffu, qwait(&bars->sfull[i][j % NS], (uint32_t)((j / NS) & 1), a.err,
+                                                    DEV_TIMEOUT_TFULL, abort_flag));
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t ts = tmem + ((uint32_t)(w4 * 32) << 16) + (i * NS + j % NS) * TK;
+                const Granule* gr = bars->gran[j & 3];
+                const int left = pos - j * TK;  // the tile's last token that this row sees
+                float x[TK / 32][32];
+    #pragma unroll
+                for (int c = 0; c < TK / 32; ++c) tmem_ld<32>(ts + c * 32, reinterpret_cast<int(&)[32]>(x[c]));
+                tmem_ld_wait();
+                if (PARTS == 1 && a.scale < 0.0f) {  // the factors are positive
+    #pragma unroll
+                    for (int c = 0; c < TK / 32; ++c)
+    #pragma unroll
+                        for (int k = 0; k < 32; ++k) x[c][k] = -x[c][k];
                 }
-            }
-            uint64_t total[2] = {};
-#pragma unroll
-            for (int c = 0; c < TK / 32; ++c) {
-                uint32_t hi[16], lo[16];
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const Granule gg = gr[2 * c + e];
-                    // a masked -infinity has to stay one: no factor of zero, and
-                    // no NaN from a granule that the row does not see
-                    const bool sees = c * 32 + e * 16 <= left;
-                    float f = sees ? fs * gg.sk : 1e-38f;
-                    if (f == 0.0f) f = 1e-38f;
-                    if (sees) poison += gg.bad;
-                    const uint64_t f2 = f2_pack(f, f), b2 = f2_pack(gg.shift - mref, gg.shift - mref);
-                    uint64_t sum[2];
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) {
-                        const uint64_t z = f2_fma(f2_pack(x[c][e * 16 + 2 * k], x[c][e * 16 + 2 * k + 1]), f2, b2);
-                        const float y[2] = {exp2_fast(f2_lo(z)), exp2_fast(f2_hi(z))};
-                        const uint64_t w = f2_pack(y[0], y[1]);
-                        sum[k & 1] = k < 2 ? w : f2_add(sum[k & 1], w);
-                        hi[e * 8 + k] = pack_word<__half>(y);
-                        if (PARTS == 2) {
-                            float u[2];
-                            unpack_word<__half>(hi[e * 8 + k], u);
-                            u[0] = y[0] - u[0];
-                            u[1] = y[1] - u[1];
-                            lo[e * 8 + k] = pack_word<__half>(u);
+                if (__any_sync(0xffffffffu, left < TK - 1)) {
+    #pragma unroll
+                    for (int c = 0; c < TK / 32; ++c)
+    #pragma unroll
+                        for (int k = 0; k < 32; ++k)
+                            if (c * 32 + k > left) x[c][k] = -INFINITY;
+                }
+                float m = -INFINITY;
+    #pragma unroll
+                for (int e = 0; e < TK / 16; ++e) {
+                    const float* y = &x[e / 2][(e & 1) * 16];
+                    float t[5];
+    #pragma unroll
+                    for (int k = 0; k < 5; ++k) t[k] = max3(y[3 * k], y[3 * k + 1], y[3 * k + 2]);
+                    m = fmaxf(m, fmaxf(max3(t[0], t[1], t[2]), max3(t[3], t[4], y[15])) * (fs * gr[e].sk));
+                }
+                const bool grown = j == 0 ? m > -INFINITY : m > mref + kGrow;
+                if (__any_sync(0xffffffffu, grown)) {
+                    const float next = grown ? m : mref;
+                    const float f = exp2_fast(mref - next);
+                    mref = next;
+                    if (j > 0) {
+                        l *= f;
+                        ok = __all_sync(0xffffffffu, qwait(&bars->pvdone[i], (uint32_t)((j - 1) & 1), a.err,
+                                                           DEV_TIMEOUT_TFULL, abort_flag));
+                        if (!ok) break;
+                        tc_fence_after();
+                        for (int c = 0; c < hs; c += 16) {
+                            int y[16];
+                            tmem_ld<16>(to + c, y);
+                            tmem_ld_wait();
+                            uint32_t z[16];
+    #pragma unroll
+                            for (int k = 0; k < 16; ++k) z[k] = __float_as_uint(__int_as_float(y[k]) * f);
+                            tmem_st16(to + c, z);
                         }
                     }
-                    total[e] = f2_fma(f2_add(sum[0], sum[1]), f2_pack(gg.inv, gg.inv), total[e]);
                 }
-                tmem_st16(ts + c * 32, hi);
-                if (PARTS == 2) tmem_st16(ts + c * 32 + 16, lo);
+                uint64_t total[2] = {};
+    #pragma unroll
+                for (int c = 0; c < TK / 32; ++c) {
+                    uint32_t hi[16], lo[16];
+    #pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const Granule gg = gr[2 * c + e];
+                        // a masked -infinity has to stay one: no factor of zero, and
+                        // no NaN from a granule that the row does not see
+                        const bool sees = c * 32 + e * 16 <= left;
+                        float f = sees ? fs * gg.sk : 1e-38f;
+                        if (f == 0.0f) f = 1e-38f;
+                        if (sees) poison += gg.bad;
+                        const uint64_t f2 = f2_pack(f, f), b2 = f2_pack(gg.shift - mref, gg.shift - mref);
+                        uint64_t sum[2];
+    #pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            const uint64_t z = f2_fma(f2_pack(x[c][e * 16 + 2 * k], x[c][e * 16 + 2 * k + 1]), f2, b2);
+                            const float y[2] = {exp2_fast(f2_lo(z)), exp2_fast(f2_hi(z))};
+                            const uint64_t w = f2_pack(y[0], y[1]);
+                            sum[k & 1] = k < 2 ? w : f2_add(sum[k & 1], w);
+                            hi[e * 8 + k] = pack_word<__half>(y);
+                            if (PARTS == 2) {
+                                float u[2];
+                                unpack_word<__half>(hi[e * 8 + k], u);
+                                u[0] = y[0] - u[0];
+                                u[1] = y[1] - u[1];
+                                lo[e * 8 + k] = pack_word<__half>(u);
+                            }
+                        }
+                        total[e] = f2_fma(f2_add(sum[0], sum[1]), f2_pack(gg.inv, gg.inv), total[e]);
+                    }
+                    tmem_st16(ts + c * 32, hi);
+                    if (PARTS == 2) tmem_st16(ts + c * 32 + 16, lo);
+                }
+                l += (f2_lo(total[0]) + f2_hi(total[0])) + (f2_lo(total[1]) + f2_hi(total[1]));
+                tmem_st_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bars->pfull[i][j % NS]);
             }
-            l += (f2_lo(total[0]) + f2_hi(total[0])) + (f2_lo(total[1]) + f2_hi(total[1]));
-            tmem_st_wait();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&bars->pfull[i][j % NS]);
-        }
-        if (ok)
-            ok = __all_sync(0xffffffffu, qwait(&bars->pvdone[i], (uint32_t)((n_i - 1) & 1), a.err, DEV_TIMEOUT_TFULL, abort_flag));
-        tc_fence_after();
-        if (ok) {
-            const float f = svm * 0.5f / l;  // 2^-kUnit
-            const int64_t at = (int64_t)(q.r0 + r / g) * a.ld_out + (int64_t)(h * g + r % g) * hs;
-            for (int c = 0; c < hs; c += 16) {
-                int y[16];
-                tmem_ld<16>(to + c, y);
-                tmem_ld_wait();
-                if (r < rows) store_row16(a, at + c, y, f, poison);
+            if (ok)
+                ok = __all_sync(0xffffffffu, qwait(&bars->pvdone[i], (uint32_t)((n_i - 1) & 1), a.err,
+                                                   DEV_TIMEOUT_TFULL, abort_flag));
+            tc_fence_after();
+            if (ok) {
+                const float f = svm * 0.5f / l;  // 2^-kUnit
+                const int64_t at = (int64_t)(q.r0 + r / g) * a.ld_out + (int64_t)(h * g + r % g) * hs;
+                for (int c = 0; c < hs; c += 16) {
+                    int y[16];
+                    tmem_ld<16>(to + c, y);
+                    tmem_ld_wait();
+                    if (r < rows) store_row16(a, at + c, y, f, poison);
+                }
+                if (a.lse && r < rows)
+                    a.lse[(int64_t)(q.r0 + r / g) * a.n_heads + h * g + r % g] = (mref + log2f(l)) * kLn2;
             }
-            if (a.lse && r < rows)
-                a.lse[(int64_t)(q.r0 + r / g) * a.n_heads + h * g + r % g] = (mref + log2f(l)) * kLn2;
-        }
         }
     }
     tc_fence_before();
@@ -1284,7 +1417,8 @@ extern "C" int paged_attention(void* out, int64_t ld_out, const void* q, int64_t
     a.err = c->err;
     // few rows: every (sequence, kv head, row tile) is cut into splits of the context
     const int64_t most_rows = (int64_t)batch->max_rows * a.group;
-    a.row_tiles = (int)(((most_rows < kFewRows ? most_rows : kFewRows) + 7) / 8);
+    const int tile_rows = most_rows <= 1 ? 1 : 8;
+    a.row_tiles = (int)(((most_rows < kFewRows ? most_rows : kFewRows) + tile_rows - 1) / tile_rows);
     if (a.row_tiles < 1) a.row_tiles = 1;
     const int64_t jobs = (int64_t)batch->n_seqs * cache->n_kv_heads * a.row_tiles;
     // so many that all fit the GPU's CTA slots at once (a second round costs
@@ -1300,7 +1434,7 @@ extern "C" int paged_attention(void* out, int64_t ld_out, const void* q, int64_t
     if (jobs > INT32_MAX) return lq_fail(LQ_EUNSUPPORTED, "paged_attention: %lld (sequence, kv head) pairs", (long long)jobs);
     void* part = nullptr;
     if (splits > 1) {
-        rc = stream_workspace(c, (size_t)jobs * splits * 8 * (cache->head_size + 8) * sizeof(float), &a.cnt, &part);
+        rc = stream_workspace(c, (size_t)jobs * splits * tile_rows * (cache->head_size + 8) * sizeof(float), &a.cnt, &part);
         if (rc) return rc;
     }
     a.part = static_cast<float*>(part);
@@ -1308,7 +1442,10 @@ extern "C" int paged_attention(void* out, int64_t ld_out, const void* q, int64_t
     a.few_rows = batch->n_seqs == 1 && most_rows > kFewRows && (int64_t)batch->n_rows * a.group > kFewRows ? 0 : kFewRows;
     const dim3 grid((unsigned)jobs, (unsigned)splits);
     cudaError_t e = cudaSuccess;
-    if (a.few_rows) e = type == LQ_F32 ? few_launch<3>(a, grid, stream()) : few_launch<2>(a, grid, stream());
+    if (a.few_rows && tile_rows == 1)
+        e = type == LQ_F32 ? few_launch<3, 1>(a, grid, stream()) : few_launch<2, 1>(a, grid, stream());
+    else if (a.few_rows)
+        e = type == LQ_F32 ? few_launch<3, 8>(a, grid, stream()) : few_launch<2, 8>(a, grid, stream());
     if (e != cudaSuccess) return cuda_fail(e, "paged_attention launch");
     if (most_rows > kFewRows) {
         e = type == LQ_F32   ? many_launch<LQ_F32>(a, stream())
