@@ -43,9 +43,9 @@ struct AttArgs {
     int few_rows;     // (token, head) rows of a sequence and kv head that the first kernel takes
     float scale;      // log2(e) times the caller's
     int row_tiles;    // tiles of 8 (token, head) rows of a sequence and kv head
-    int chunk;        // tokens per split
-    float* part;      // [job][split][rows of a tile][head_size + 8]: out, max, sum
-    int* cnt;         // [job] arrivals
+    int plan;         // contexts are split (0: a CTA takes a whole one)
+    float* part;      // [split of a sequence][kv head, row tile][its rows][head_size + 8]: out, max, sum
+    int* cnt;         // [sequence][kv head, row tile] arrivals
     int* err;
 };
 
@@ -95,6 +95,28 @@ __device__ __forceinline__ void store_out(const AttArgs& a, int64_t i, float v) 
         static_cast<__half*>(a.out)[i] = from_f32<__half>(v);
     else
         static_cast<__nv_bfloat16*>(a.out)[i] = from_f32<__nv_bfloat16>(v);
+}
+
+// 4 neighbouring outputs
+__device__ __forceinline__ void store_out4(const AttArgs& a, int64_t i, const float (&v)[4]) {
+    auto put = [&](auto* p) {
+        using T = std::remove_reference_t<decltype(*p)>;
+        if (reinterpret_cast<uintptr_t>(p) % (4 * sizeof(T)) == 0) {
+            store_n<4, true>(p, v);
+        } else {
+            for (int k = 0; k < 4; ++k) p[k] = from_f32<T>(v[k]);
+        }
+    };
+    if (a.type == LQ_F32)
+        put(static_cast<float*>(a.out) + i);
+    else if (a.type == LQ_F16)
+        put(static_cast<__half*>(a.out) + i);
+    else
+        put(static_cast<__nv_bfloat16*>(a.out) + i);
+}
+
+__device__ __forceinline__ void add4(float4& v, const float4& x, float f) {
+    v = make_float4(fmaf(x.x, f, v.x), fmaf(x.y, f, v.y), fmaf(x.z, f, v.z), fmaf(x.w, f, v.w));
 }
 
 // 16 neighbouring outputs x * f + bad
@@ -198,15 +220,26 @@ __device__ __forceinline__ float unbias(int d) { return __int_as_float(d) - kBia
 // ---------------------------------------------------------------------------
 // Few rows per kv head (decode): bound by the cache's bytes from HBM.
 //
-// One CTA per (sequence, kv head, tile of 8 rows, split of the context); its
+// One CTA per (sequence, kv head, tile of rows, split of the context); its
 // four warps take 32 tokens each in turn, each through a ring of its own of
 // bulk copies, and are joined at the end; the splits of a row are joined by
-// the last CTA to arrive, in split order.  An MMA's 16 rows are the 8 (token,
-// head) rows twice: rows 0-7 hold their first digit, rows 8-15 the second, so
-// a thread finds both digits' dots of its row in its own registers.  A third
-// digit takes a second MMA.
+// the last CTA to arrive, in split order.
 //
-// Tokens and MMA columns: the two 8-column tiles over 16 tokens are dealt so
+// Tiles of 8 rows (several query heads to a kv head, or several tokens): an
+// MMA's 16 rows are the 8 (token, head) rows twice: rows 0-7 hold their first
+// digit, rows 8-15 the second, so a thread finds both digits' dots of its row
+// in its own registers.  A third digit takes a second MMA.
+//
+// One row (a token, and a query head to each kv head): the codes are the MMA's
+// 16 rows, 16 tokens of K or 16 dims of V, and the digits its columns, so that
+// one MMA takes all digits and a lane one token's softmax.  64 sequences of the
+// case below take 78 us so, 120 us as a tile of 8 rows with seven empty.
+//
+// How long a split is follows from the contexts, which only the device knows
+// (a captured call's max_context is that of its longest replay): the least
+// multiple of 128 tokens with which all splits find a CTA slot at once.
+//
+// Tokens and MMA columns of tiles of 8 rows: the two 8-column tiles over 16 tokens are dealt so
 // that a thread's four scores are four neighbouring tokens (the A operand of
 // p . V) and that the eight rows an ldmatrix reads lie in different banks:
 // column 2j + e of the even tile is token 4j + 2x + e with x = j / 2, of the odd
@@ -230,6 +263,46 @@ constexpr int few_smem() {
     return kFewWarps * kSlots * kItem * HS * 2;
 }
 
+struct Split {
+    int s, split, chunk;  // sequence (-1: none), its split, tokens of a split
+};
+
+// The unit-th of at most `units` splits of the batch's sequences, each of which
+// has one at least.  By one warp; a sequence a lane.
+__device__ __forceinline__ Split find_split(const KVBatch& b, int unit, int units, int lane) {
+    auto blocks = [&](int i) {  // of 128 tokens
+        return i < b.n_seqs ? (min(max(__ldg(b.context + i), 0), b.max_context) + 127) / 128 : 0;
+    };
+    asm volatile("prefetch.global.L1 [%0];" ::"l"(b.row_start + min(lane, b.n_seqs)));
+    if (b.n_seqs == 1) return {0, unit, max(2, (blocks(0) + units - 1) / units) * 128};
+    int total = 0;
+    for (int i = lane; i < b.n_seqs; i += 32) total += blocks(i);
+    total = __reduce_add_sync(0xffffffffu, total);
+    int chunk = max(2, (total + units - 1) / units);
+    auto parts = [&](int i) { return i < b.n_seqs ? max(1, (blocks(i) + chunk - 1) / chunk) : 0; };
+    for (;; chunk += max(1, chunk / 8)) {  // ends: a long chunk leaves one split each, fewer than units
+        int n = 0;
+        for (int i = lane; i < b.n_seqs; i += 32) n += parts(i);
+        if (__reduce_add_sync(0xffffffffu, n) <= units) break;
+    }
+    int before = 0;
+    for (int i0 = 0; i0 < b.n_seqs; i0 += 32) {
+        int sum = parts(i0 + lane);
+#pragma unroll
+        for (int o = 1; o < 32; o *= 2) {
+            const int x = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += x;
+        }
+        const int k = __popc(__ballot_sync(0xffffffffu, before + sum <= unit));  // sequences that end before it
+        if (k < 32) {
+            const int past = __shfl_sync(0xffffffffu, sum, max(k - 1, 0));
+            return i0 + k < b.n_seqs ? Split{i0 + k, unit - before - (k > 0 ? past : 0), chunk * 128} : Split{-1, 0, 0};
+        }
+        before += __shfl_sync(0xffffffffu, sum, 31);
+    }
+    return {-1, 0, 0};
+}
+
 // ND: digits of the weights.  ROWS: rows of a tile, 8 or 1
 template <int ND, int HS, bool EXACT, int ROWS>
 __global__ void __launch_bounds__(kFewThreads, HS <= 128 ? 3 : 1) attend_few_kernel(const __grid_constant__ AttArgs a) {
@@ -245,22 +318,27 @@ __global__ void __launch_bounds__(kFewThreads, HS <= 128 ? 3 : 1) attend_few_ker
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int hs = EXACT ? HS : a.c.head_size;
     const int P = a.c.page_size, H = a.c.n_kv_heads, g = a.group;
-    const int rt = blockIdx.x % a.row_tiles, sh = blockIdx.x / a.row_tiles, h = sh % H, s = sh / H;
-    const int split = blockIdx.y;
+    const int rt = blockIdx.x % a.row_tiles, h = blockIdx.x / a.row_tiles;
 
     if (tid < kFewWarps * kSlots) mbar_init(&bars[tid], 1);
     fence_mbar_init();
     pdl_trigger();
     pdl_wait();
+    int s = blockIdx.y, split = 0, chunk = INT32_MAX;
+    if (a.plan) {
+        const Split x = find_split(a.b, blockIdx.y, gridDim.y, lane);
+        if (x.s < 0) return;
+        s = x.s, split = x.split, chunk = x.chunk;
+    }
     const SeqRows q = seq_rows(a.b, s, split == 0 && rt == 0 && h == 0 && tid == 0 ? a.err : nullptr);
     if (split == 0 && rt == 0) zero_rows(a, q, h);
     const int rows = q.n * g;
     if (rows > a.few_rows || rt * ROWS >= rows) return;
     const int top = min(rows, rt * ROWS + ROWS) - 1;            // the tile's last row
     const int seen = q.begin + top / g + 1;               // tokens that it sees
-    const int splits = (seen + a.chunk - 1) / a.chunk;
+    const int splits = a.plan ? (seen + chunk - 1) / chunk : 1;
     if (split >= splits) return;
-    const int ta = split * a.chunk, tb = min(ta + a.chunk, seen);
+    const int ta = a.plan ? split * chunk : 0, tb = a.plan ? min(ta + chunk, seen) : seen;
     int* const err = lane == 0 ? a.err : nullptr;
 
     // the warp's items are kItem tokens at ta + (warp + kFewWarps * j) * kItem; lane L
@@ -639,17 +717,20 @@ __global__ void __launch_bounds__(kFewThreads, HS <= 128 ? 3 : 1) attend_few_ker
         }
     }
     __syncthreads();
-    const int64_t job = (int64_t)blockIdx.x;
-    float* part = a.part + (job * gridDim.y + split) * ROWS * w1;
-    auto finish = [&](int rr, int d, float v, float mm, float ll) {
+    // the split's part, and how far it is to the next one's
+    const int64_t hop = (int64_t)gridDim.x * ROWS * w1;
+    float* part = a.part + blockIdx.y * hop + blockIdx.x * ROWS * w1;
+    // four neighbouring dims of row rr of the sequence
+    auto finish = [&](int rr, int d, float4 v, float mm, float ll) {
         const int row = q.r0 + rr / g, head = h * g + rr % g;
-        store_out(a, (int64_t)row * a.ld_out + (int64_t)head * hs + d, v / ll);
+        store_out4(a, (int64_t)row * a.ld_out + (int64_t)head * hs + d, {v.x / ll, v.y / ll, v.z / ll, v.w / ll});
         if (a.lse && d == 0) a.lse[(int64_t)row * a.n_heads + head] = (mm + log2f(ll)) * kLn2;
     };
-    const int valid = top + 1 - rt * ROWS;
-    for (int i = tid; i < valid * hs; i += kFewThreads) {
-        const int row8 = i / hs, d = i % hs;
-        float mm = -INFINITY, ll = 0.0f, v = 0.0f;
+    const int quads = (top + 1 - rt * ROWS) * (hs / 4);
+    for (int i = tid; i < quads; i += kFewThreads) {
+        const int row8 = i / (hs / 4), d = i % (hs / 4) * 4;
+        float mm = -INFINITY, ll = 0.0f;
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
         for (int w = 0; w < kFewWarps; ++w) mm = fmaxf(mm, join[(w * ROWS + row8) * w1 + hs]);
         const float ref = mm == -INFINITY ? 0.0f : mm;
@@ -658,69 +739,63 @@ __global__ void __launch_bounds__(kFewThreads, HS <= 128 ? 3 : 1) attend_few_ker
             const float* src = join + (w * ROWS + row8) * w1;
             const float c = exp2_fast(src[hs] - ref);
             ll = fmaf(src[hs + 1], c, ll);
-            v = fmaf(src[d], c, v);
+            add4(v, *reinterpret_cast<const float4*>(src + d), c);
         }
         if (splits == 1) {
             finish(rt * ROWS + row8, d, v, mm, ll);
         } else {
-            __stcg(part + row8 * w1 + d, v);
-            if (d == 0) {
-                __stcg(part + row8 * w1 + hs, mm);
-                __stcg(part + row8 * w1 + hs + 1, ll);
-            }
+            __stcg(reinterpret_cast<float4*>(part + row8 * w1 + d), v);
+            if (d == 0) __stcg(reinterpret_cast<float2*>(part + row8 * w1 + hs), make_float2(mm, ll));
         }
     }
     if (splits == 1) return;
     __threadfence();
     __syncthreads();
     if (tid == 0) {
-        const int n = atomicAdd(a.cnt + job, 1);
+        int* cnt = a.cnt + s * (int)gridDim.x + blockIdx.x;
+        const int n = atomicAdd(cnt, 1);
         last_flag = n == splits - 1;
-        if (last_flag) a.cnt[job] = 0;  // as the next launch expects it
+        if (last_flag) *cnt = 0;  // as the next launch expects it
     }
     __syncthreads();
     if (!last_flag) return;
     __threadfence();
-    // weights of a row's splits (a warp per row), then the weighted sums
-    const float* all = a.part + job * gridDim.y * ROWS * w1;
-    float* weight = join;  // [ROWS][splits], then their maxima and sums
-    float *row_max = weight + ROWS * splits, *row_sum = row_max + ROWS;
-    for (int row8 = warp; row8 < valid; row8 += kFewWarps) {
-        const float* src = all + row8 * w1 + hs;
+    // eight splits at a time, all their loads before the first use (one at a time
+    // the join of three splits took 15 us)
+    const float* all = part - split * hop;
+    for (int i = tid; i < quads; i += kFewThreads) {
+        const int row8 = i / (hs / 4), d = i % (hs / 4) * 4;
+        const float* src = all + row8 * w1;
         float mm = -INFINITY, ll = 0.0f;
-        for (int i = lane; i < splits; i += 32) {
-            const float v = __ldcg(src + (int64_t)i * ROWS * w1);
-            weight[row8 * splits + i] = v;
-            mm = fmaxf(mm, v);
-        }
-        mm = warp_max(mm);
-        const float ref = mm == -INFINITY ? 0.0f : mm;
-        for (int i = lane; i < splits; i += 32) {
-            const float c = exp2_fast(weight[row8 * splits + i] - ref);
-            weight[row8 * splits + i] = c;
-            ll = fmaf(__ldcg(src + (int64_t)i * ROWS * w1 + 1), c, ll);
-        }
-        ll = warp_sum(ll);
-        if (lane == 0) {
-            row_max[row8] = mm;
-            row_sum[row8] = ll;
-        }
-    }
-    __syncthreads();
-    for (int i = tid; i < valid * hs; i += kFewThreads) {
-        const int row8 = i / hs, d = i % hs;
-        const float *src = all + row8 * w1 + d, *w = weight + row8 * splits;
-        float v = 0.0f;
-        int k = 0;
-        for (; k + 8 <= splits; k += 8) {
-            float x[8];
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 1
+        for (int k = 0; k < splits; k += 8) {
+            float4 x[8];
+            float2 ml[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = __ldcg(src + (int64_t)(k + e) * ROWS * w1);
+            for (int e = 0; e < 8; ++e) {
+                x[e] = v;
+                ml[e] = make_float2(-INFINITY, 0.0f);
+                if (k + e < splits) {
+                    x[e] = __ldcg(reinterpret_cast<const float4*>(src + (k + e) * hop + d));
+                    ml[e] = __ldcg(reinterpret_cast<const float2*>(src + (k + e) * hop + hs));
+                }
+            }
+            const float was = mm;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v = fmaf(x[e], w[k + e], v);
+            for (int e = 0; e < 8; ++e) mm = fmaxf(mm, ml[e].x);
+            const float ref = mm == -INFINITY ? 0.0f : mm, c = exp2_fast(was - ref);
+            ll *= c;
+            v = make_float4(v.x * c, v.y * c, v.z * c, v.w * c);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                if (k + e >= splits) break;
+                const float f = exp2_fast(ml[e].x - ref);
+                ll = fmaf(ml[e].y, f, ll);
+                add4(v, x[e], f);
+            }
         }
-        for (; k < splits; ++k) v = fmaf(__ldcg(src + (int64_t)k * ROWS * w1), w[k], v);
-        finish(rt * ROWS + row8, d, v, row_max[row8], row_sum[row8]);
+        finish(rt * ROWS + row8, d, v, mm, ll);
     }
 }
 
@@ -1420,27 +1495,24 @@ extern "C" int paged_attention(void* out, int64_t ld_out, const void* q, int64_t
     const int tile_rows = most_rows <= 1 ? 1 : 8;
     a.row_tiles = (int)(((most_rows < kFewRows ? most_rows : kFewRows) + tile_rows - 1) / tile_rows);
     if (a.row_tiles < 1) a.row_tiles = 1;
-    const int64_t jobs = (int64_t)batch->n_seqs * cache->n_kv_heads * a.row_tiles;
-    // so many that all fit the GPU's CTA slots at once (a second round costs
-    // more than uneven contexts: 16 sequences of the 70B shape 27 us in one, 35 us
-    // in two), 256 tokens at least (two steps of every warp)
-    const int64_t slots = 3 * c->num_sms;
-    int64_t splits = jobs <= kWsCounters ? slots / jobs : 1;
-    if (splits < 1) splits = 1;
-    a.chunk = (int)(((batch->max_context + splits - 1) / splits + 127) / 128 * 128);
-    if (a.chunk < 256) a.chunk = 256;
-    splits = (batch->max_context + a.chunk - 1) / a.chunk;
-    if (splits < 1) splits = 1;
-    if (jobs > INT32_MAX) return lq_fail(LQ_EUNSUPPORTED, "paged_attention: %lld (sequence, kv head) pairs", (long long)jobs);
+    // Splits of contexts, as many as find a CTA slot each (three CTAs to an SM,
+    // one beyond 128 dims): a second round costs more than uneven contexts (16
+    // sequences of the 70B shape 27 us in one, 35 us in two).
+    const int64_t x = (int64_t)cache->n_kv_heads * a.row_tiles;
+    const int64_t slots = (cache->head_size <= 128 ? 3 : 1) * c->num_sms;
+    const int64_t most_splits = (int64_t)batch->n_seqs * ((batch->max_context + 255) / 256);
+    int64_t units = slots / x < most_splits ? slots / x : most_splits;
+    a.plan = units > batch->n_seqs;
+    if (!a.plan) units = batch->n_seqs;
     void* part = nullptr;
-    if (splits > 1) {
-        rc = stream_workspace(c, (size_t)jobs * splits * tile_rows * (cache->head_size + 8) * sizeof(float), &a.cnt, &part);
+    if (a.plan) {
+        rc = stream_workspace(c, (size_t)(units * x * tile_rows * (cache->head_size + 8)) * sizeof(float), &a.cnt, &part);
         if (rc) return rc;
     }
     a.part = static_cast<float*>(part);
     // one sequence with many rows leaves nothing to the first kernel
     a.few_rows = batch->n_seqs == 1 && most_rows > kFewRows && (int64_t)batch->n_rows * a.group > kFewRows ? 0 : kFewRows;
-    const dim3 grid((unsigned)jobs, (unsigned)splits);
+    const dim3 grid((unsigned)x, (unsigned)units);
     cudaError_t e = cudaSuccess;
     if (a.few_rows && tile_rows == 1)
         e = type == LQ_F32 ? few_launch<3, 1>(a, grid, stream()) : few_launch<2, 1>(a, grid, stream());

@@ -450,3 +450,26 @@ def test_append_then_attend(cuda, dtype):
         qv, out, lse = run_attention(torch, q_rot, codes, scales, b, dtype, hs)
         want, wlse, tol, ltol = attention(qv, codes, scales, b, dtype, 1 / math.sqrt(hs))
         assert np.all(np.abs(out - want) <= tol) and np.all(np.abs(lse - wlse) <= ltol)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("seqs,kv_heads,group", [(1, 1, 1), (33, 1, 1), (70, 2, 1), (70, 1, 6), (300, 1, 1), (300, 1, 2), (500, 1, 1)])
+def test_attend_bound_far_above_the_contexts(cuda, dtype, seqs, kv_heads, group):
+    """Many sequences, idle and long ones among them, and a max_context that none
+    comes near: how they are split follows from the contexts themselves."""
+    rng = np.random.default_rng(seqs)
+    ctx = [int(x) for x in rng.integers(0, 400, seqs)]
+    ctx[seqs // 2] = 3000
+    rows = [int(x) for x in rng.integers(0, 2, seqs)]
+    rows[seqs // 2] = 1
+    batch = Batch(rng, rows, ctx, 64)
+    codes, scales = random_cache(rng, batch.n_pages, kv_heads, 64, 64)
+    q = rng.standard_normal((batch.n_rows, kv_heads * group, 64)) * 2
+    for bound in (3000, 100000):
+        qv, out, lse = run_attention(cuda, q, codes, scales, batch, dtype, 64, 0.125,
+                                     dev=batch.device(cuda, max_context=bound))
+        want, wlse, tol, ltol = attention(qv, codes, scales, batch, dtype, 0.125)
+        assert np.all(np.abs(out - want) <= tol), (np.abs(out - want) / np.maximum(tol, 1e-30)).max()
+        empty = np.isinf(wlse)
+        assert np.array_equal(empty, np.isneginf(lse)) and not out[empty].any()
+        assert np.all(np.abs(lse[~empty] - wlse[~empty]) <= ltol[~empty])
