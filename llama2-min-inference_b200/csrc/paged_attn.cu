@@ -115,10 +115,6 @@ __device__ __forceinline__ void store_out4(const AttArgs& a, int64_t i, const fl
         put(static_cast<__nv_bfloat16*>(a.out) + i);
 }
 
-__device__ __forceinline__ void add4(float4& v, const float4& x, float f) {
-    v = make_float4(fmaf(x.x, f, v.x), fmaf(x.y, f, v.y), fmaf(x.z, f, v.z), fmaf(x.w, f, v.w));
-}
-
 // 16 neighbouring outputs x * f + bad
 __device__ __forceinline__ void store_row16(const AttArgs& a, int64_t i, const int (&x)[16], float f, float bad) {
     float v[16];
@@ -720,17 +716,21 @@ __global__ void __launch_bounds__(kFewThreads, HS <= 128 ? 3 : 1) attend_few_ker
     // the split's part, and how far it is to the next one's
     const int64_t hop = (int64_t)gridDim.x * ROWS * w1;
     float* part = a.part + blockIdx.y * hop + blockIdx.x * ROWS * w1;
-    // four neighbouring dims of row rr of the sequence
-    auto finish = [&](int rr, int d, float4 v, float mm, float ll) {
+    // W neighbouring dims of a row to a thread: one row has a thread for each dim
+    constexpr int W = ROWS == 8 ? 4 : 1;
+    auto finish = [&](int rr, int d, const float (&v)[W], float mm, float ll) {
         const int row = q.r0 + rr / g, head = h * g + rr % g;
-        store_out4(a, (int64_t)row * a.ld_out + (int64_t)head * hs + d, {v.x / ll, v.y / ll, v.z / ll, v.w / ll});
+        const int64_t at = (int64_t)row * a.ld_out + (int64_t)head * hs + d;
+        if constexpr (W == 4)
+            store_out4(a, at, {v[0] / ll, v[1] / ll, v[2] / ll, v[3] / ll});
+        else
+            store_out(a, at, v[0] / ll);
         if (a.lse && d == 0) a.lse[(int64_t)row * a.n_heads + head] = (mm + log2f(ll)) * kLn2;
     };
-    const int quads = (top + 1 - rt * ROWS) * (hs / 4);
-    for (int i = tid; i < quads; i += kFewThreads) {
-        const int row8 = i / (hs / 4), d = i % (hs / 4) * 4;
-        float mm = -INFINITY, ll = 0.0f;
-        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    const int shares = (top + 1 - rt * ROWS) * (hs / W);
+    for (int i = tid; i < shares; i += kFewThreads) {
+        const int row8 = i / (hs / W), d = i % (hs / W) * W;
+        float mm = -INFINITY, ll = 0.0f, v[W] = {};
 #pragma unroll
         for (int w = 0; w < kFewWarps; ++w) mm = fmaxf(mm, join[(w * ROWS + row8) * w1 + hs]);
         const float ref = mm == -INFINITY ? 0.0f : mm;
@@ -739,13 +739,23 @@ __global__ void __launch_bounds__(kFewThreads, HS <= 128 ? 3 : 1) attend_few_ker
             const float* src = join + (w * ROWS + row8) * w1;
             const float c = exp2_fast(src[hs] - ref);
             ll = fmaf(src[hs + 1], c, ll);
-            add4(v, *reinterpret_cast<const float4*>(src + d), c);
+            float x[W];
+            if constexpr (W == 4)
+                load_n<4, true>(src + d, x);
+            else
+                x[0] = src[d];
+#pragma unroll
+            for (int e = 0; e < W; ++e) v[e] = fmaf(x[e], c, v[e]);
         }
         if (splits == 1) {
             finish(rt * ROWS + row8, d, v, mm, ll);
         } else {
-            __stcg(reinterpret_cast<float4*>(part + row8 * w1 + d), v);
-            if (d == 0) __stcg(reinterpret_cast<float2*>(part + row8 * w1 + hs), make_float2(mm, ll));
+            float* to = part + row8 * w1;
+            if constexpr (W == 4)
+                __stcg(reinterpret_cast<float4*>(to + d), make_float4(v[0], v[1], v[2], v[3]));
+            else
+                __stcg(to + d, v[0]);
+            if (d == 0) __stcg(reinterpret_cast<float2*>(to + hs), make_float2(mm, ll));
         }
     }
     if (splits == 1) return;
@@ -761,24 +771,30 @@ __global__ void __launch_bounds__(kFewThreads, HS <= 128 ? 3 : 1) attend_few_ker
     if (!last_flag) return;
     __threadfence();
     // eight splits at a time, all their loads before the first use (one at a time
-    // the join of three splits took 15 us)
+    // the join of three splits of 8 rows took 15 us)
     const float* all = part - split * hop;
-    for (int i = tid; i < quads; i += kFewThreads) {
-        const int row8 = i / (hs / 4), d = i % (hs / 4) * 4;
+    for (int i = tid; i < shares; i += kFewThreads) {
+        const int row8 = i / (hs / W), d = i % (hs / W) * W;
         const float* src = all + row8 * w1;
-        float mm = -INFINITY, ll = 0.0f;
-        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        float mm = -INFINITY, ll = 0.0f, v[W] = {};
 #pragma unroll 1
         for (int k = 0; k < splits; k += 8) {
-            float4 x[8];
+            float x[8][W];
             float2 ml[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                x[e] = v;
                 ml[e] = make_float2(-INFINITY, 0.0f);
+#pragma unroll
+                for (int c = 0; c < W; ++c) x[e][c] = 0.0f;
                 if (k + e < splits) {
-                    x[e] = __ldcg(reinterpret_cast<const float4*>(src + (k + e) * hop + d));
-                    ml[e] = __ldcg(reinterpret_cast<const float2*>(src + (k + e) * hop + hs));
+                    const float* from = src + (k + e) * hop;
+                    if constexpr (W == 4) {
+                        const float4 y = __ldcg(reinterpret_cast<const float4*>(from + d));
+                        x[e][0] = y.x, x[e][1] = y.y, x[e][2] = y.z, x[e][3] = y.w;
+                    } else {
+                        x[e][0] = __ldcg(from + d);
+                    }
+                    ml[e] = __ldcg(reinterpret_cast<const float2*>(from + hs));
                 }
             }
             const float was = mm;
@@ -786,13 +802,14 @@ __global__ void __launch_bounds__(kFewThreads, HS <= 128 ? 3 : 1) attend_few_ker
             for (int e = 0; e < 8; ++e) mm = fmaxf(mm, ml[e].x);
             const float ref = mm == -INFINITY ? 0.0f : mm, c = exp2_fast(was - ref);
             ll *= c;
-            v = make_float4(v.x * c, v.y * c, v.z * c, v.w * c);
+#pragma unroll
+            for (int z = 0; z < W; ++z) v[z] *= c;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                if (k + e >= splits) break;
                 const float f = exp2_fast(ml[e].x - ref);
                 ll = fmaf(ml[e].y, f, ll);
-                add4(v, x[e], f);
+#pragma unroll
+                for (int z = 0; z < W; ++z) v[z] = fmaf(x[e][z], f, v[z]);
             }
         }
         finish(rt * ROWS + row8, d, v, mm, ll);
