@@ -254,6 +254,9 @@ constexpr int kItem = 32;   // tokens of one step of a warp
 constexpr int kSlots = 2;   // its ring
 constexpr int kFewRows = 32;  // (token, head) rows of a sequence up to which it is taken
 
+// CTAs on an SM: what registers and the rings allow
+constexpr int few_ctas(int hs, int rows) { return hs > 128 ? 1 : hs <= 64 && rows == 1 ? 5 : 3; }
+
 template <int HS>
 constexpr int few_smem() {
     return kFewWarps * kSlots * kItem * HS * 2;
@@ -301,7 +304,7 @@ __device__ __forceinline__ Split find_split(const KVBatch& b, int unit, int unit
 
 // ND: digits of the weights.  ROWS: rows of a tile, 8 or 1
 template <int ND, int HS, bool EXACT, int ROWS>
-__global__ void __launch_bounds__(kFewThreads, HS <= 128 ? 3 : 1) attend_few_kernel(const __grid_constant__ AttArgs a) {
+__global__ void __launch_bounds__(kFewThreads, few_ctas(HS, ROWS)) attend_few_kernel(const __grid_constant__ AttArgs a) {
     constexpr int KS = HS / 32;       // k steps of q . K
     constexpr int NP = 2;             // MMAs of a tile of q . K: two digits, the third
     constexpr int NT = HS / 8;        // column tiles of p . V
@@ -1516,7 +1519,7 @@ extern "C" int paged_attention(void* out, int64_t ld_out, const void* q, int64_t
     // one beyond 128 dims): a second round costs more than uneven contexts (16
     // sequences of the 70B shape 27 us in one, 35 us in two).
     const int64_t x = (int64_t)cache->n_kv_heads * a.row_tiles;
-    const int64_t slots = (cache->head_size <= 128 ? 3 : 1) * c->num_sms;
+    const int64_t slots = few_ctas(cache->head_size, tile_rows) * c->num_sms;
     const int64_t most_splits = (int64_t)batch->n_seqs * ((batch->max_context + 255) / 256);
     int64_t units = slots / x < most_splits ? slots / x : most_splits;
     a.plan = units > batch->n_seqs;
