@@ -66,6 +66,29 @@ __device__ __forceinline__ int find_seq(int n, int at, int lane, F key) {
     return s;
 }
 
+// 8 dims by their four pairs' (cos, sin): u and v are the pairs' first and second
+// dims (halves), or 4 dims each
+__device__ __forceinline__ void turn8(bool halves, const float4& t0, const float4& t1, float (&u)[4], float (&v)[4]) {
+    const float c[4] = {t0.x, t0.z, t1.x, t1.z}, n[4] = {t0.y, t0.w, t1.y, t1.w};
+    if (halves) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float p = u[k], r = v[k];
+            u[k] = p * c[k] - r * n[k];
+            v[k] = p * n[k] + r * c[k];
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const float p = u[2 * k], r = u[2 * k + 1], p2 = v[2 * k], r2 = v[2 * k + 1];
+            u[2 * k] = p * c[k] - r * n[k];
+            u[2 * k + 1] = p * n[k] + r * c[k];
+            v[2 * k] = p2 * c[k + 2] - r2 * n[k + 2];
+            v[2 * k + 1] = p2 * n[k + 2] + r2 * c[k + 2];
+        }
+    }
+}
+
 constexpr int kNoRope = 2;  // MODE: LQ_ROPE_*, or this, or -1 for whichever at run time
 
 // A warp's share of a row of queries: 8 dims a lane, 256 neighbouring ones at a
@@ -98,25 +121,7 @@ __device__ __forceinline__ void rotate_queries(const AppendArgs& a, int unit, in
         t1 = tab[d / 4 + 1];
     }
     auto turned = [&](float (&u)[4], float (&v)[4]) {
-        if (!turn) return;
-        const float c[4] = {t0.x, t0.z, t1.x, t1.z}, n[4] = {t0.y, t0.w, t1.y, t1.w};
-        if (halves) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const float p = u[k], r = v[k];
-                u[k] = p * c[k] - r * n[k];
-                v[k] = p * n[k] + r * c[k];
-            }
-        } else {
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                const float p = u[2 * k], r = u[2 * k + 1], p2 = v[2 * k], r2 = v[2 * k + 1];
-                u[2 * k] = p * c[k] - r * n[k];
-                u[2 * k + 1] = p * n[k] + r * c[k];
-                v[2 * k] = p2 * c[k + 2] - r2 * n[k + 2];
-                v[2 * k + 1] = p2 * n[k + 2] + r2 * c[k + 2];
-            }
-        }
+        if (turn) turn8(halves, t0, t1, u, v);
     };
     if (fixed) {
         const int o0 = halves ? d / 2 - d : 0, o1 = halves ? o0 + hs / 2 : 4;
@@ -321,32 +326,41 @@ __global__ void __launch_bounds__(kAppendThreads, 4) append_kernel(const __grid_
     const T* vr = static_cast<const T*>(a.r.v) + (int64_t)row0 * a.r.ld_v + (int64_t)h * hs;
     const float* tab0 = a.r.rope ? a.r.rope + (int64_t)t0 * hs : nullptr;
 
-    // K: 4 dims of a token at a time (a word of codes), hw of them per token.
-    // V: 4 tokens of a dim (a word), words wf .. w1 - 1 hold new tokens.
-    const int hw = hs / 4, nk = nt * hw, wf = off / 4, w1 = (off + nt + 3) / 4, nv = (w1 - wf) * hs;
-    const Walk k0(tid, threads, hw), v0(tid, threads, hs);
-    const int mode = MODE < 0 ? a.r.rope_mode : MODE;
+    // K: 8 dims of a token at a time, as in rotate_queries.  V: 4 tokens of 4 dims,
+    // a word of codes for each dim; words wf .. w1 - 1 hold new tokens, and four
+    // neighbouring threads take the words of 16 tokens.
+    const int hw = hs / 8, nk = nt * hw, wf = off / 4, w1 = (off + nt + 3) / 4, g0 = wf / 4, nv = ((w1 + 3) / 4 - g0) * hs;
+    const Walk k0(tid, threads, hw), v0(tid / 4, threads / 4, hs / 4);
     const bool turn = MODE < 0 ? tab0 != nullptr : MODE != kNoRope;
-    auto load_k = [&](const Walk& i, float (&k)[4]) {
-        rotated4<T, VEC>(kr + i.q * a.r.ld_k, turn ? tab0 + i.q * hs : nullptr, hs, mode, 4 * i.r, k);
+    const bool halves = MODE < 0 ? turn && a.r.rope_mode == LQ_ROPE_HALVES : MODE == LQ_ROPE_HALVES;
+    auto dims = [&](const Walk& i, int& e0, int& e1) {
+        e0 = halves ? 4 * i.r : 8 * i.r;
+        e1 = halves ? e0 + hs / 2 : e0 + 4;
     };
-    auto load_v = [&](const Walk& i, float (&x)[4]) {
-        const int t = 4 * (wf + i.q) - off;
-        const T* p = vr + t * a.r.ld_v + i.r;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = t + e >= 0 && t + e < nt ? to_f32(p[e * a.r.ld_v]) : 0.0f;
+    auto load_k = [&](const Walk& i, float (&u)[4], float (&v)[4]) {
+        int e0, e1;
+        dims(i, e0, e1);
+        const T* row = kr + i.q * a.r.ld_k;
+        load_n<4, VEC>(row + e0, u);
+        load_n<4, VEC>(row + e1, v);
+        if (turn) {
+            const float4* t = reinterpret_cast<const float4*>(tab0 + i.q * hs) + 2 * i.r;
+            turn8(halves, t[0], t[1], u, v);
+        }
     };
     uint32_t mk = 0, mv = 0;
     Walk ki = k0, vi = v0;
 #pragma unroll 4
     for (int i = tid; i < nk; i += threads, ki.next()) {
-        float k[4], v[4];
-        load_k(ki, k);
-        load_n<4, VEC>(vr + ki.q * a.r.ld_v + 4 * ki.r, v);
+        float u[4], v[4], x[4], y[4];
+        load_k(ki, u, v);
+        const T* row = vr + ki.q * a.r.ld_v + 8 * ki.r;
+        load_n<4, VEC>(row, x);
+        load_n<4, VEC>(row + 4, y);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            mk = max(mk, abs_bits(k[e]));
-            mv = max(mv, abs_bits(v[e]));
+            mk = max(mk, max(abs_bits(u[e]), abs_bits(v[e])));
+            mv = max(mv, max(abs_bits(x[e]), abs_bits(y[e])));
         }
     }
     float old_k = 0.0f, old_v = 0.0f;  // a page whose first token arrives now starts afresh
@@ -377,7 +391,7 @@ __global__ void __launch_bounds__(kAppendThreads, 4) append_kernel(const __grid_
     const bool grow_k = off > 0 && sk != old_k, grow_v = off > 0 && sv != old_v;
     if (grow_k) {
         const float ratio = qk.bad ? 0.0f : old_k / sk;
-        for (int i = tid; i < off * hw; i += threads) {
+        for (int i = tid; i < off * (hs / 4); i += threads) {
             const int t = i % off, w = i / off;  // word w (4 dims) of token t
             uint32_t* p = reinterpret_cast<uint32_t*>(kc + ((int64_t)(w / 4) * P + t) * 16) + (w & 3);
             *p = again(*p, ratio);
@@ -391,49 +405,69 @@ __global__ void __launch_bounds__(kAppendThreads, 4) append_kernel(const __grid_
             *p = again(*p, ratio_v);
         }
     }
-    auto store_k = [&](const Walk& i, float (&k)[4]) {
-        const int d = 4 * i.r;
+    auto store_k = [&](int t, int d, float (&k)[4]) {
         const uint32_t c = qk(k[0], k[1], k[2], k[3]);
-        *reinterpret_cast<uint32_t*>(kc + ((d >> 4) * P + off + i.q) * 16 + (d & 15)) = c;
+        *reinterpret_cast<uint32_t*>(kc + ((d >> 4) * P + off + t) * 16 + (d & 15)) = c;
         if (a.r.k_out) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) k[e] = (float)code_of(c >> (8 * e)) * sk;
-            store_n<4, VEC>(static_cast<T*>(a.r.k_out) + (int64_t)(row0 + i.q) * a.r.ld_kv_out + (int64_t)h * hs + d, k);
-        }
-    };
-    auto store_v = [&](const Walk& i, const float (&x)[4]) {
-        const int w = wf + i.q;
-        uint32_t* p = reinterpret_cast<uint32_t*>(vc + ((w >> 2) * hs + i.r) * 16) + (w & 3);
-        const uint32_t c = qv(x[0], x[1], x[2], x[3]);
-        // a word at either end: earlier tokens kept or rescaled, later bytes kept
-        const int lo = max(off - 4 * w, 0), hi = min(off + nt - 4 * w, 4);  // its new bytes
-        uint32_t word = c;
-        if (lo > 0 || hi < 4) {
-            uint32_t was = *p;
-            if (grow_v && lo > 0) was = again(was, ratio_v, lo);
-            const uint32_t mask = (hi >= 4 ? 0xFFFFFFFFu : (1u << (8 * hi)) - 1u) & ~((1u << (8 * lo)) - 1u);
-            word = (c & mask) | (was & ~mask);
-        }
-        *p = word;
-        if (a.r.v_out) {
-            T* out = static_cast<T*>(a.r.v_out) + (row0 + 4 * w - off) * a.r.ld_kv_out + (int64_t)h * hs + i.r;
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (e >= lo && e < hi) out[e * a.r.ld_kv_out] = from_f32<T>((float)code_of(c >> (8 * e)) * sv);
+            store_n<4, VEC>(static_cast<T*>(a.r.k_out) + (int64_t)(row0 + t) * a.r.ld_kv_out + (int64_t)h * hs + d, k);
         }
     };
     ki = k0;
-#pragma unroll 4
-    for (int i = tid; i < nk; i += threads, ki.next()) {
-        float k[4];
-        load_k(ki, k);
-        store_k(ki, k);
-    }
 #pragma unroll 2
+    for (int i = tid; i < nk; i += threads, ki.next()) {
+        float u[4], v[4];
+        load_k(ki, u, v);
+        int e0, e1;
+        dims(ki, e0, e1);
+        store_k(ki.q, e0, u);
+        store_k(ki.q, e1, v);
+    }
+#pragma unroll 1
     for (int i = tid; i < nv; i += threads, vi.next()) {
-        float x[4];
-        load_v(vi, x);
-        store_v(vi, x);
+        const int w = 4 * (g0 + vi.q) + (tid & 3), d = 4 * vi.r, t = 4 * w - off;
+        if (w < wf || w >= w1) continue;
+        const T* x = vr + t * a.r.ld_v + d;
+        float v[4][4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[e][k] = 0.0f;
+            if (t + e >= 0 && t + e < nt) load_n<4, VEC>(x + e * a.r.ld_v, v[e]);
+        }
+        uint32_t c[4];  // by token
+#pragma unroll
+        for (int e = 0; e < 4; ++e) c[e] = qv(v[e][0], v[e][1], v[e][2], v[e][3]);
+        const uint32_t a0 = __byte_perm(c[0], c[1], 0x5140), a1 = __byte_perm(c[2], c[3], 0x5140);
+        const uint32_t b0 = __byte_perm(c[0], c[1], 0x7362), b1 = __byte_perm(c[2], c[3], 0x7362);
+        uint32_t word[4] = {__byte_perm(a0, a1, 0x5410), __byte_perm(a0, a1, 0x7632), __byte_perm(b0, b1, 0x5410),
+                            __byte_perm(b0, b1, 0x7632)};  // by dim
+        // a word at either end: earlier tokens kept or rescaled, later bytes kept
+        const int lo = max(-t, 0), hi = min(nt - t, 4);  // its new bytes
+        uint32_t* p = reinterpret_cast<uint32_t*>(vc + ((w >> 2) * hs + d) * 16) + (w & 3);
+        if (lo > 0 || hi < 4) {
+            const uint32_t mask = (hi >= 4 ? 0xFFFFFFFFu : (1u << (8 * hi)) - 1u) & ~((1u << (8 * lo)) - 1u);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                uint32_t was = p[4 * k];
+                if (grow_v && lo > 0) was = again(was, ratio_v, lo);
+                word[k] = (word[k] & mask) | (was & ~mask);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) p[4 * k] = word[k];
+        if (a.r.v_out) {
+            T* out = static_cast<T*>(a.r.v_out) + (row0 + t) * a.r.ld_kv_out + (int64_t)h * hs + d;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (e < lo || e >= hi) continue;
+                float o[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) o[k] = (float)code_of(c[e] >> (8 * k)) * sv;
+                store_n<4, VEC>(out + e * a.r.ld_kv_out, o);
+            }
+        }
     }
 }
 
