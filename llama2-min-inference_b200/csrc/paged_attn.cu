@@ -901,7 +901,7 @@ struct Granule {  // 16 tokens
 };
 
 struct ManyBars {
-    uint64_t qfull[2], kfull[4], kempty[4], vfull[4], vempty[4], sfull[2][2], pfull[2][2], pvdone[2], done[2];
+    uint64_t qfull[2], kfull[4], kempty[4], vfull[4], vempty[4], sfull[2][2], pfull[2][2], pvdone[2], last[2], done[2];
     uint64_t tabfull[4], tabempty[4];
     uint32_t tmem_base;
     int abort_flag;
@@ -997,6 +997,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const __gr
                 mbar_init(&bars->pfull[i][b], 4);
             }
             mbar_init(&bars->pvdone[i], 1);
+            mbar_init(&bars->last[i], 1);
             mbar_init(&bars->done[i], 1);
         }
         for (int i = 0; i < 4; ++i) {
@@ -1155,7 +1156,9 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const __gr
                                 mma_f16_ts(dst, src + (k >> 1) * 32 + p * 16 + (k & 1) * 8,
                                            vd + (uint32_t)((k >> 2) * (hs * 128) >> 4) + 2 * (k & 3), id_o,
                                            j > 0 || k > 0 || p > 0);
-                        mma_commit(&bars->pvdone[i]);
+                        // the last tile's on a barrier of its own: softmax may come to it
+                        // before the tile before it is done, whose phase has the other parity
+                        mma_commit(j == n[i] - 1 ? &bars->last[i] : &bars->pvdone[i]);
                         if (last_use(i, j)) {
                             mma_commit(&bars->vempty[j % NB]);
                             mma_commit(&bars->tabempty[j & 3]);
@@ -1359,7 +1362,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const __gr
                     const float next = grown ? m : mref;
                     const float f = exp2_fast(mref - next);
                     mref = next;
-                    if (j > 0) {
+                    if (j > 0) {  // the product before last is done: these scores were issued after it
                         l *= f;
                         ok = __all_sync(0xffffffffu, qwait(&bars->pvdone[i], (uint32_t)((j - 1) & 1), a.err,
                                                            DEV_TIMEOUT_TFULL, abort_flag));
@@ -1418,8 +1421,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const __gr
                 if (lane == 0) mbar_arrive(&bars->pfull[i][j % NS]);
             }
             if (ok)
-                ok = __all_sync(0xffffffffu, qwait(&bars->pvdone[i], (uint32_t)((n_i - 1) & 1), a.err,
-                                                   DEV_TIMEOUT_TFULL, abort_flag));
+                ok = __all_sync(0xffffffffu, qwait(&bars->last[i], 0, a.err, DEV_TIMEOUT_TFULL, abort_flag));
             tc_fence_after();
             if (ok) {
                 const float f = svm * 0.5f / l;  // 2^-kUnit

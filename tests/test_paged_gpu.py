@@ -473,3 +473,34 @@ def test_attend_bound_far_above_the_contexts(cuda, dtype, seqs, kv_heads, group)
         empty = np.isinf(wlse)
         assert np.array_equal(empty, np.isneginf(lse)) and not out[empty].any()
         assert np.all(np.abs(lse[~empty] - wlse[~empty]) <= ltol[~empty])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("group,hs,page", [(2, 128, 64), (1, 64, 16), (3, 128, 16)])
+def test_prompts_same_bits_many_times(cuda, dtype, group, hs, page):
+    """Prompts that end in the middle of tiles, over and over with the GPU busy:
+    every launch gives the first one's bits, which are right."""
+    rng = np.random.default_rng(group)
+    rows, ctx = [300, 1, 129, 64], [700, 900, 129, 65]
+    batch = Batch(rng, rows, ctx, page)
+    codes, scales = random_cache(rng, batch.n_pages, 4, hs, page)
+    heads = 4 * group
+    q = rng.standard_normal((batch.n_rows, heads, hs)) * 2
+    tc, ts = cuda.from_numpy(codes).cuda(), cuda.from_numpy(scales).cuda()
+    c = cache_struct(tc, ts, 4, hs, page)
+    b, keep = batch.device(cuda)
+    qt = cuda.from_numpy(q.reshape(batch.n_rows, heads * hs)).cuda().to(torch_type(cuda, dtype))
+    outs = [cuda.empty_like(qt) for _ in range(9)]
+    wrong = cuda.zeros(1, device="cuda", dtype=cuda.int64)
+    for n in range(40):
+        for out in outs[n > 0:]:
+            lq.paged_attention(out.data_ptr(), qt.data_ptr(), heads, c, b, KINDS[dtype], hs**-0.5)
+        lq.sync()
+        for out in outs[1:]:
+            wrong += (out != outs[0]).sum()
+        cuda.cuda.synchronize()
+    assert int(wrong) == 0
+    qv = qt.double().cpu().numpy().reshape(-1, heads, hs)
+    want, _, tol, _ = attention(qv, codes, scales, batch, dtype, hs**-0.5)
+    got = outs[0].double().cpu().numpy().reshape(want.shape)
+    assert np.all(np.abs(got - want) <= tol)
