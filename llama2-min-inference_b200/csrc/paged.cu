@@ -297,10 +297,10 @@ template <typename T, bool VEC, int MODE>
 __global__ void __launch_bounds__(kAppendThreads, 4) append_kernel(const __grid_constant__ AppendArgs a) {
     pdl_trigger();
     pdl_wait();
-    constexpr int threads = kAppendThreads;
+    const int threads = blockDim.x;
     const int tid = threadIdx.x, lane = tid & 31;
     if (blockIdx.x >= a.kv_blocks) {
-        rotate_queries<T, VEC, MODE>(a, (blockIdx.x - a.kv_blocks) * kAppendWarps + (tid >> 5), lane);
+        rotate_queries<T, VEC, MODE>(a, (blockIdx.x - a.kv_blocks) * (threads / 32) + (tid >> 5), lane);
         return;
     }
     const int hs = a.c.head_size, P = a.c.page_size, H = a.c.n_kv_heads;
@@ -350,7 +350,7 @@ __global__ void __launch_bounds__(kAppendThreads, 4) append_kernel(const __grid_
     };
     uint32_t mk = 0, mv = 0;
     Walk ki = k0, vi = v0;
-#pragma unroll 4
+#pragma unroll 2
     for (int i = tid; i < nk; i += threads, ki.next()) {
         float u[4], v[4], x[4], y[4];
         load_k(ki, u, v);
@@ -376,8 +376,7 @@ __global__ void __launch_bounds__(kAppendThreads, 4) append_kernel(const __grid_
         wv[tid >> 5] = mv;
     }
     __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kAppendWarps; ++w) {
+    for (int w = 0; w < threads / 32; ++w) {
         mk = max(mk, wk[w]);
         mv = max(mv, wv[w]);
     }
@@ -481,13 +480,19 @@ cudaError_t append_t(AppendArgs& a, int sms, cudaStream_t st) {
     const bool one = a.b.max_rows <= 1;
     int64_t kv = one ? (int64_t)a.b.n_seqs * ((a.c.n_kv_heads + kAppendWarps - 1) / kAppendWarps)
                      : ((int64_t)a.b.n_rows / a.c.page_size + 2 * a.b.n_seqs) * a.c.n_kv_heads;
+    // Threads for a page: no more than fill the GPU (768 an SM, of the 1024 that
+    // registers allow), since a block's start costs every warp as much as some
+    // hundred elements.  2424 pages of 16 tokens: 64 threads 47 us, 256 58 us;
+    // 576 pages of 32 tokens: 25 us and 17 us.
+    int threads = kAppendThreads;
+    while (!one && threads > 32 && kv * (threads / 2) >= (int64_t)sms * 768) threads /= 2;
     // a row of queries is cut into 256-dim parts until there are 8 warps per SM
     int64_t q_blocks = 0;
     a.q_parts = 1;
     if (r.q) {
         const int most = (r.n_heads * a.c.head_size + 255) / 256, want = 8 * sms / a.b.n_rows;
         a.q_parts = want < 1 ? 1 : want < most ? want : most;
-        q_blocks = ((int64_t)a.b.n_rows * a.q_parts + kAppendWarps - 1) / kAppendWarps;
+        q_blocks = ((int64_t)a.b.n_rows * a.q_parts + threads / 32 - 1) / (threads / 32);
     }
     if (kv + q_blocks > INT32_MAX) return cudaErrorInvalidConfiguration;
     a.kv_blocks = (int)kv;
@@ -496,7 +501,7 @@ cudaError_t append_t(AppendArgs& a, int sms, cudaStream_t st) {
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(kv + q_blocks));
-    cfg.blockDim = dim3(kAppendThreads);
+    cfg.blockDim = dim3(threads);
     cfg.stream = st;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
