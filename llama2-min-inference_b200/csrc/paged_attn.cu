@@ -1465,15 +1465,18 @@ cudaError_t many_launch_t(const AttArgs& a, cudaStream_t st) {
     return cudaLaunchKernelEx(&cfg, kern, a);
 }
 
-// Two row tiles of 128 for the usual head sizes, whose kernels have their
-// addresses at compile time; one for any other (their accumulators and operands
-// would not fit twice at the largest).
+// Two row tiles of 128 up to 128 dims, one beyond (their accumulators and
+// operands would not fit twice); 64 and 128 dims with their addresses at compile
+// time.
 template <int TYPE>
 cudaError_t many_launch(const AttArgs& a, cudaStream_t st) {
     constexpr bool f32 = TYPE == LQ_F32;
     constexpr int TK = f32 ? 128 : 64, NS = f32 ? 1 : 2;
-    if (a.c.head_size == 64) return many_launch_t<64, TYPE, 2, TK, NS, f32 ? 2 : 4, true>(a, st);
-    if (a.c.head_size == 128) return many_launch_t<128, TYPE, 2, TK, NS, f32 ? 1 : 3, true>(a, st);
+    const int hs = a.c.head_size;
+    if (hs == 64) return many_launch_t<64, TYPE, 2, TK, NS, f32 ? 2 : 4, true>(a, st);
+    if (hs == 128) return many_launch_t<128, TYPE, 2, TK, NS, f32 ? 1 : 3, true>(a, st);
+    if (hs < 64) return many_launch_t<64, TYPE, 2, TK, NS, f32 ? 2 : 4, false>(a, st);
+    if (hs < 128) return many_launch_t<128, TYPE, 2, TK, NS, f32 ? 1 : 3, false>(a, st);
     return many_launch_t<256, TYPE, 1, f32 ? 64 : 128, 1, 1, false>(a, st);
 }
 

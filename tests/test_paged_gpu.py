@@ -504,3 +504,10 @@ def test_prompts_same_bits_many_times(cuda, dtype, group, hs, page):
     want, _, tol, _ = attention(qv, codes, scales, batch, dtype, hs**-0.5)
     got = outs[0].double().cpu().numpy().reshape(want.shape)
     assert np.all(np.abs(got - want) <= tol)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("hs", [16, 32, 48, 80, 96, 112, 144, 240])
+def test_attend_prompt_head_sizes(cuda, dtype, hs):
+    """Prompts at head sizes between the usual ones."""
+    check_attention(cuda, np.random.default_rng(hs), [150, 40], [333, 41], 2, 2, hs, 32, dtype)
