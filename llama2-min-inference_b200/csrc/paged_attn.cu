@@ -866,10 +866,10 @@ cudaError_t few_launch(const AttArgs& a, dim3 grid, cudaStream_t st) {
 //                    scores from tensor memory, writes its weights over them
 //                    as the A operand of the second product, 2 x (32 columns
 //                    of scores -> 16 of f16 pairs, the second ones for fp32)
-//   warps 8-11       convert codes: global -> registers (a tile ahead) -> f16 in
+//   4 or 8 warps     convert codes: global -> registers (a tile ahead) -> f16 in
 //                    shared memory (128-byte swizzle)
-//   warp 12 (and 14) issue the MMAs
-//   warp 13          looks up pages and scales, up to four tiles ahead
+//   then 4 warps     the first (and the third) issue the MMAs, the second looks
+//                    up pages and scales, up to four tiles ahead
 //
 // The 16-bit types keep two buffers of scores per row tile, of 64 tokens each:
 // the next scores are computed while softmax is at these, and each row tile
@@ -892,8 +892,11 @@ cudaError_t few_launch(const AttArgs& a, dim3 grid, cudaStream_t st) {
 // 128 tokens with one buffer of scores: bf16 130 us, but f16 with 8 heads to a kv
 // head and pages of 16 176 us against 164, and head size 64 103 us against 98.
 
-constexpr int kManyWarps = 16;  // whole warpgroups, as registers are dealt to them
-constexpr int kManyThreads = 32 * kManyWarps;
+// Converting warps: codes to 16 bits are two or three instructions each, and with
+// four warps they held up the 16-bit types (132 us in the case below, 85 us without
+// any conversion).
+constexpr int many_converters(int ns) { return ns == 2 ? 8 : 4; }
+constexpr int many_threads(int ns) { return 32 * (8 + many_converters(ns) + 4); }
 constexpr float kGrow = 13.0f, kUnit = 1.0f;
 
 struct Granule {  // 16 tokens
@@ -955,13 +958,13 @@ __device__ __forceinline__ void put_codes(unsigned char* block, int row, int pai
 }
 
 template <int HS, int TYPE, int NQ, int TK, int NS, int NB, bool EXACT>
-__global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const __grid_constant__ AttArgs a) {
+__global__ void __launch_bounds__(many_threads(NS), 1) attend_many_kernel(const __grid_constant__ AttArgs a) {
     using Lay = ManyLayout<HS, TYPE, NQ, TK, NS, NB>;
     constexpr int kIssuers = NS == 2 ? NQ : 1;  // warps that issue MMAs: one per row tile, or one for all
     constexpr int PARTS = Lay::kParts;
     constexpr bool kBf16 = TYPE == LQ_BF16;
-    constexpr int kPieces = HS / 16;  // 16-byte pieces of K (and of V) per converting thread and 128 tokens
-    constexpr int kLoads = kPieces * TK / 128;
+    constexpr int kConv = many_converters(NS), kIssue = 8 + kConv;  // converting warps; the first issuing warp
+    constexpr int kLoads = HS / 16 * TK / (32 * kConv);  // 16-byte pieces of K (and of V) per converting thread
     extern __shared__ __align__(1024) unsigned char raw[];
     unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
     unsigned char *sq = sm, *sk = sq + NQ * Lay::kQ, *sv = sk + NB * Lay::kK;
@@ -1003,8 +1006,8 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const __gr
         for (int i = 0; i < 4; ++i) {
             mbar_init(&bars->tabfull[i], 1);
             mbar_init(&bars->tabempty[i], kIssuers);
-            mbar_init(&bars->kfull[i], 4);
-            mbar_init(&bars->vfull[i], 4);
+            mbar_init(&bars->kfull[i], kConv);
+            mbar_init(&bars->vfull[i], kConv);
             mbar_init(&bars->kempty[i], kIssuers);
             mbar_init(&bars->vempty[i], kIssuers);
         }
@@ -1012,11 +1015,11 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const __gr
         bars->peak = 0;
         fence_mbar_init();
     }
-    if (warp == 12) tmem_alloc<1, 512>(&bars->tmem_base);
+    if (warp == kIssue) tmem_alloc<1, 512>(&bars->tmem_base);
     const int lp2 = __ffs(P) - 1;
     const int32_t* pages = a.b.pages + (int64_t)s * a.b.max_pages;
     uint32_t pk = 0;
-    for (int lp = tid; lp << lp2 < seen && lp < a.b.max_pages; lp += kManyThreads) {
+    for (int lp = tid; lp << lp2 < seen && lp < a.b.max_pages; lp += many_threads(NS)) {
         const int p = __ldg(pages + lp);
         if (p < 0 || p >= a.c.n_pages) continue;  // reported below
         const uint32_t v = abs_bits(__ldg(a.c.scales + ((int64_t)p * H + h) * 2 + 1));
@@ -1032,22 +1035,25 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const __gr
     const float svm = bars->peak ? __uint_as_float(bars->peak) : 1.0f;
     const int8_t* codes = static_cast<const int8_t*>(a.c.codes);
 
-    // 512 threads hold 65536 registers; 128 scores a thread take a share of 168
-    constexpr bool kDeal = NS == 1;  // 2 x 128 x 168 + 128 x 104 + 128 x 72
-    if (warp >= 8 && warp < 12) {
+    // 512 threads have 128 registers each; 128 scores a thread take a larger share,
+    // dealt to warpgroups within that sum
+    constexpr bool kDeal = NS == 1;
+    constexpr int kSoftRegs = 168, kConvRegs = 104, kIssueRegs = 72;
+    static_assert(!kDeal || 8 * kSoftRegs + kConv * kConvRegs + 4 * kIssueRegs <= (12 + kConv) * 128, "registers");
+    if (warp >= 8 && warp < kIssue) {
         // ---------------- conversion ----------------
-        if constexpr (kDeal) regs_down<104>();
-        const int t = tid - 256;  // 0..127
+        if constexpr (kDeal) regs_down<kConvRegs>();
+        const int t = tid - 256;
         uint4 kr[kLoads], vr[kLoads];
-        // K: token t (two threads a token for TK of 64, half the dims each)
-        const int kt = TK == 128 ? t : t & 63, kc0 = TK == 128 ? 0 : (t >> 6);
-        constexpr int kcs = TK == 128 ? 1 : 2;
-        // V: the tile's pieces t, t + 128, ...: piece tc * hs + d is 16 tokens of dim d
+        // K: token t % TK, every kcs-th piece of its dims
+        constexpr int kcs = 32 * kConv / TK;
+        const int kt = t % TK, kc0 = t / TK;
+        // V: every 32 * kConv-th piece of the tile: piece tc * hs + d is 16 tokens of dim d
         int pd[kLoads], ptc[kLoads];
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
-            ptc[i] = (t + 128 * i) / hs;
-            pd[i] = (t + 128 * i) - ptc[i] * hs;
+            ptc[i] = (t + 32 * kConv * i) / hs;
+            pd[i] = (t + 32 * kConv * i) - ptc[i] * hs;
         }
         bool ok = true;
         auto load_k = [&](int j) {
@@ -1098,9 +1104,9 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const __gr
             if (lane == 0) mbar_arrive(&bars->vfull[buf]);
             if (j + 1 < tiles) load_v(j + 1);
         }
-    } else if (warp >= 12) {
-        if constexpr (kDeal) regs_down<72>();
-        if (warp != 13 && (warp - 12) / 2 < kIssuers && warp % 2 == 0) {
+    } else if (warp >= kIssue) {
+        if constexpr (kDeal) regs_down<kIssueRegs>();
+        if ((warp - kIssue) / 2 < kIssuers && warp % 2 == 0) {
             // ---------------- MMA issue ----------------
             // f32 += f16 x f16 (or bf16 x bf16), M 128
             const uint32_t id_s =
@@ -1108,7 +1114,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const __gr
             const uint32_t id_o = (1u << 4) | ((uint32_t)(hs >> 3) << 17) | (8u << 24);
             const uint64_t dq = smem_desc_sw128(smem_addr(sq)), dk = smem_desc_sw128(smem_addr(sk)),
                            dv = smem_desc_sw128(smem_addr(sv));
-            const int steps = hs / 16, me = (warp - 12) / 2;
+            const int steps = hs / 16, me = (warp - kIssue) / 2;
             bool ok = true;
             auto wait = [&](uint64_t* bar, uint32_t parity, int code) {
                 ok = ok && __all_sync(0xffffffffu, qwait(bar, parity, a.err, code, abort_flag));
@@ -1195,7 +1201,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const __gr
             if (elect_one()) mma_commit(&bars->done[me]);
             __syncwarp();
             mbar_wait(&bars->done[me], 0, a.err, DEV_TIMEOUT_MMA);  // every MMA is done before the memory is freed
-        } else if (warp == 13) {
+        } else if (warp == kIssue + 1) {
             // ---------------- pages and scales ----------------
             for (int j = 0; j < tiles; ++j) {
                 const int tok = j * TK + lane * 16;
@@ -1221,7 +1227,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const __gr
         }
     } else {
         // ---------------- softmax ----------------
-        if constexpr (kDeal) regs_up<168>();
+        if constexpr (kDeal) regs_up<kSoftRegs>();
         if (warp < 4 * NQ && (warp < 4 ? n[0] : n[NQ - 1]) > 0) {
             const int i = warp >> 2, w4 = warp & 3;
             const int n_i = i == 0 ? n[0] : n[NQ - 1];
@@ -1439,7 +1445,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) attend_many_kernel(const __gr
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 12) {
+    if (warp == kIssue) {
         tc_fence_after();
         tmem_free<1, 512>(tmem);
     }
@@ -1457,7 +1463,7 @@ cudaError_t many_launch_t(const AttArgs& a, cudaStream_t st) {
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)x, (unsigned)a.c.n_kv_heads, (unsigned)a.b.n_seqs);
-    cfg.blockDim = dim3(kManyThreads);
+    cfg.blockDim = dim3(many_threads(NS));
     cfg.dynamicSmemBytes = Lay::kSmem;
     cfg.stream = st;
     cfg.attrs = attr;
