@@ -1130,7 +1130,7 @@ __global__ void __launch_bounds__(many_threads(NS), 1) attend_many_kernel(const 
                     if (j < n[i]) {
                         const uint32_t dst = tmem + (i * NS + j % NS) * TK;
                         const uint64_t kd = dk + (uint32_t)((j % NB) * Lay::kK >> 4);
-    #pragma unroll
+#pragma unroll
                         for (int p = 0; p < PARTS; ++p) {
                             const uint64_t qd = dq + (uint32_t)((i * Lay::kQ + p * (Lay::kQ / PARTS)) >> 4);
                             for (int k = 0; k < steps; ++k)  // 64 dims a block of 128-byte rows, 32 bytes a step
@@ -1155,9 +1155,9 @@ __global__ void __launch_bounds__(many_threads(NS), 1) attend_many_kernel(const 
                     if (j < n[i]) {
                         const uint32_t dst = tmem + NQ * NS * TK + i * HS, src = tmem + (i * NS + j % NS) * TK;
                         const uint64_t vd = dv + (uint32_t)((j % NB) * Lay::kV >> 4);
-    #pragma unroll
+#pragma unroll
                         for (int k = 0; k < TK / 16; ++k)
-    #pragma unroll
+#pragma unroll
                             for (int p = 0; p < PARTS; ++p)
                                 mma_f16_ts(dst, src + (k >> 1) * 32 + p * 16 + (k & 1) * 8,
                                            vd + (uint32_t)((k >> 2) * (hs * 128) >> 4) + 2 * (k & 3), id_o,
@@ -1184,14 +1184,14 @@ __global__ void __launch_bounds__(many_threads(NS), 1) attend_many_kernel(const 
                     if (ok) values(me, j);
                 }
             } else {
-    #pragma unroll
+#pragma unroll
                 for (int i = 0; i < NQ; ++i)
                     if (ok && n[i] > 0) {
                         wait(&bars->qfull[i], 0, DEV_TIMEOUT_FULL);
                         if (ok) scores(i, 0);
                     }
                 for (int j = 0; ok && j < tiles; ++j) {
-    #pragma unroll
+#pragma unroll
                     for (int i = 0; i < NQ; ++i) {
                         if (ok) values(i, j);
                         if (ok) scores(i, j + 1);
@@ -1203,23 +1203,39 @@ __global__ void __launch_bounds__(many_threads(NS), 1) attend_many_kernel(const 
             mbar_wait(&bars->done[me], 0, a.err, DEV_TIMEOUT_MMA);  // every MMA is done before the memory is freed
         } else if (warp == kIssue + 1) {
             // ---------------- pages and scales ----------------
-            for (int j = 0; j < tiles; ++j) {
-                const int tok = j * TK + lane * 16;
-                int64_t p = -1;
-                float2 sc = make_float2(NAN, NAN);
-                if (lane < TK / 16 && tok < seen) {
-                    p = page_of(a.c, a.b, s, tok >> lp2, a.err);
-                    if (p >= 0) sc = __ldg(reinterpret_cast<const float2*>(a.c.scales) + p * H + h);
+            // a granule a lane, the next 32 looked up while these are handed out: two
+            // dependent loads from memory for each tile took longer than its products
+            constexpr int kGran = TK / 16, kRound = 32 / kGran;  // granules of a tile, tiles of a round
+            int64_t p = -1, p_next = -1;
+            float2 sc = make_float2(NAN, NAN), sc_next = sc;
+            auto look_up = [&](int j) {  // tiles j .. j + kRound - 1
+                const int tok = (j * kGran + lane) * 16;
+                p_next = -1;
+                sc_next = make_float2(NAN, NAN);
+                if (tok < seen) {
+                    p_next = page_of(a.c, a.b, s, tok >> lp2, a.err);
+                    if (p_next >= 0) sc_next = __ldg(reinterpret_cast<const float2*>(a.c.scales) + p_next * H + h);
                 }
-                const bool fine = sc.y < INFINITY;
-                const float w = fine ? fmaxf(sc.y / svm, 9.094947e-13f) : 1.0f;  // 2^-40 at least
-                const float shift = log2f(w) + kUnit, inv = exp2f(-shift);
+            };
+            Granule gr = {};
+            look_up(0);
+            for (int j = 0; j < tiles; ++j) {
+                if (j % kRound == 0) {
+                    p = p_next;
+                    sc = sc_next;
+                    look_up(j + kRound);
+                    const bool fine = sc.y < INFINITY;
+                    const float w = fine ? fmaxf(sc.y / svm, 9.094947e-13f) : 1.0f;  // 2^-40 at least
+                    const float shift = log2f(w) + kUnit;
+                    gr = {sc.x, shift, exp2f(-shift), fine ? 0.0f : NAN};
+                }
                 if (!__all_sync(0xffffffffu, qwait(&bars->tabempty[j & 3], (uint32_t)(((j >> 2) & 1) ^ 1), a.err,
                                                    DEV_TIMEOUT_EMPTY, abort_flag)))
                     break;
-                if (lane < TK / 16) {
-                    bars->gran[j & 3][lane] = {sc.x, shift, inv, fine ? 0.0f : NAN};
-                    bars->cell[j & 3][lane] = p >= 0 ? (p * H + h) * (int64_t)(hs * P * 2) : -1;
+                const int i = lane - j % kRound * kGran;
+                if (i >= 0 && i < kGran) {
+                    bars->gran[j & 3][i] = gr;
+                    bars->cell[j & 3][i] = p >= 0 ? (p * H + h) * (int64_t)(hs * P * 2) : -1;
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&bars->tabfull[j & 3]);
@@ -1237,7 +1253,7 @@ __global__ void __launch_bounds__(many_threads(NS), 1) attend_many_kernel(const 
                 // as it is, in 16-byte pieces: a short loop of asynchronous copies (its
                 // unrolled form was bound by fetching instructions that run once)
                 const int per = hs / 8;  // pieces of a row
-    #pragma unroll 1
+#pragma unroll 1
                 for (int pc = lane; pc < 32 * per; pc += 32) {
                     const int rr = pc / per, ck = pc - rr * per, row = w4 * 32 + rr, r = min(first + rr, rows - 1);
                     const uint16_t* src = static_cast<const uint16_t*>(a.q) + (int64_t)(q.r0 + r / g) * a.ld_q +
@@ -1259,10 +1275,10 @@ __global__ void __launch_bounds__(many_threads(NS), 1) attend_many_kernel(const 
                 int tok = min(first, rows - 1) / g, head = min(first, rows - 1) - tok * g;
                 for (int r0 = 0; r0 < 32; r0 += kBatch) {
                     RawQ<2> raw[kBatch][kB];
-    #pragma unroll
+#pragma unroll
                     for (int u = 0; u < kBatch; ++u) {
                         const int64_t at = (int64_t)(q.r0 + tok) * a.ld_q + (int64_t)(h * g + head) * hs;
-    #pragma unroll
+#pragma unroll
                         for (int b = 0; b < kB; ++b) raw[u][b].load(a, at + min(b * 128 + lane * 4, hs - 4));
                         if (first + r0 + u + 1 < rows && ++head == g) {
                             head = 0;
@@ -1270,24 +1286,24 @@ __global__ void __launch_bounds__(many_threads(NS), 1) attend_many_kernel(const 
                         }
                     }
                     float x[kBatch][kB][4];
-    #pragma unroll
+#pragma unroll
                     for (int u = 0; u < kBatch; ++u) {
                         const bool have = first + r0 + u < rows;
-    #pragma unroll
+#pragma unroll
                         for (int b = 0; b < kB; ++b) {
                             raw[u][b].get(a, x[u][b]);
-    #pragma unroll
+#pragma unroll
                             for (int e = 0; e < 4; ++e)
                                 if (!have || b * 128 + lane * 4 >= hs) x[u][b][e] = 0.0f;
                         }
                     }
-    #pragma unroll
+#pragma unroll
                     for (int u = 0; u < kBatch; ++u) {
                         const int row = w4 * 32 + r0 + u;
                         uint32_t m = 0;
-    #pragma unroll
+#pragma unroll
                         for (int b = 0; b < kB; ++b)
-    #pragma unroll
+#pragma unroll
                             for (int e = 0; e < 4; ++e) m = max(m, abs_bits(x[u][b][e]));
                         m = __reduce_max_sync(0xffffffffu, m);
                         // a power of two that takes the largest into [2^13, 2^14)
@@ -1295,13 +1311,13 @@ __global__ void __launch_bounds__(many_threads(NS), 1) attend_many_kernel(const 
                         ex = max(-114, min(100, 13 - ex));
                         const float up = m >= kInfBits ? 0.0f : a.scale < 0.0f ? -lq_exp2i(ex) : lq_exp2i(ex);
                         if (lane == 0) bars->fs[i * 128 + row] = m >= kInfBits ? NAN : fabsf(a.scale) * lq_exp2i(-ex);
-    #pragma unroll
+#pragma unroll
                         for (int b = 0; b < kB; ++b) {
                             const int d = b * 128 + lane * 4;
                             if (d >= hs) continue;
-    #pragma unroll
+#pragma unroll
                             for (int e = 0; e < 4; ++e) x[u][b][e] = up == 0.0f ? 0.0f : x[u][b][e] * up;
-    #pragma unroll
+#pragma unroll
                             for (int p = 0; p < PARTS; ++p) {
                                 const uint32_t w0 = pack_word<__half>(x[u][b]), w1 = pack_word<__half>(x[u][b] + 2);
                                 unsigned char* dst = sq + i * Lay::kQ + p * (Lay::kQ / PARTS) + (d >> 6) * (128 * 128) +
@@ -1311,7 +1327,7 @@ __global__ void __launch_bounds__(many_threads(NS), 1) attend_many_kernel(const 
                                     float y[4];
                                     unpack_word<__half>(w0, y);
                                     unpack_word<__half>(w1, y + 2);
-    #pragma unroll
+#pragma unroll
                                     for (int e = 0; e < 4; ++e) x[u][b][e] -= y[e];
                                 }
                             }
@@ -1338,28 +1354,28 @@ __global__ void __launch_bounds__(many_threads(NS), 1) attend_many_kernel(const 
                 const Granule* gr = bars->gran[j & 3];
                 const int left = pos - j * TK;  // the tile's last token that this row sees
                 float x[TK / 32][32];
-    #pragma unroll
+#pragma unroll
                 for (int c = 0; c < TK / 32; ++c) tmem_ld<32>(ts + c * 32, reinterpret_cast<int(&)[32]>(x[c]));
                 tmem_ld_wait();
                 if (PARTS == 1 && a.scale < 0.0f) {  // the factors are positive
-    #pragma unroll
+#pragma unroll
                     for (int c = 0; c < TK / 32; ++c)
-    #pragma unroll
+#pragma unroll
                         for (int k = 0; k < 32; ++k) x[c][k] = -x[c][k];
                 }
                 if (__any_sync(0xffffffffu, left < TK - 1)) {
-    #pragma unroll
+#pragma unroll
                     for (int c = 0; c < TK / 32; ++c)
-    #pragma unroll
+#pragma unroll
                         for (int k = 0; k < 32; ++k)
                             if (c * 32 + k > left) x[c][k] = -INFINITY;
                 }
                 float m = -INFINITY;
-    #pragma unroll
+#pragma unroll
                 for (int e = 0; e < TK / 16; ++e) {
                     const float* y = &x[e / 2][(e & 1) * 16];
                     float t[5];
-    #pragma unroll
+#pragma unroll
                     for (int k = 0; k < 5; ++k) t[k] = max3(y[3 * k], y[3 * k + 1], y[3 * k + 2]);
                     m = fmaxf(m, fmaxf(max3(t[0], t[1], t[2]), max3(t[3], t[4], y[15])) * (fs * gr[e].sk));
                 }
@@ -1379,17 +1395,17 @@ __global__ void __launch_bounds__(many_threads(NS), 1) attend_many_kernel(const 
                             tmem_ld<16>(to + c, y);
                             tmem_ld_wait();
                             uint32_t z[16];
-    #pragma unroll
+#pragma unroll
                             for (int k = 0; k < 16; ++k) z[k] = __float_as_uint(__int_as_float(y[k]) * f);
                             tmem_st16(to + c, z);
                         }
                     }
                 }
                 uint64_t total[2] = {};
-    #pragma unroll
+#pragma unroll
                 for (int c = 0; c < TK / 32; ++c) {
                     uint32_t hi[16], lo[16];
-    #pragma unroll
+#pragma unroll
                     for (int e = 0; e < 2; ++e) {
                         const Granule gg = gr[2 * c + e];
                         // a masked -infinity has to stay one: no factor of zero, and
@@ -1400,7 +1416,7 @@ __global__ void __launch_bounds__(many_threads(NS), 1) attend_many_kernel(const 
                         if (sees) poison += gg.bad;
                         const uint64_t f2 = f2_pack(f, f), b2 = f2_pack(gg.shift - mref, gg.shift - mref);
                         uint64_t sum[2];
-    #pragma unroll
+#pragma unroll
                         for (int k = 0; k < 8; ++k) {
                             const uint64_t z = f2_fma(f2_pack(x[c][e * 16 + 2 * k], x[c][e * 16 + 2 * k + 1]), f2, b2);
                             const float y[2] = {exp2_fast(f2_lo(z)), exp2_fast(f2_hi(z))};
