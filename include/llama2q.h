@@ -98,7 +98,10 @@ int lq_sync(void);
  * operator kernel start (and start streaming its weights) while the previous
  * kernel on the stream is still finishing — programmatic dependent launch.
  * Activations are still read only after that kernel completes.  Set it only
- * when no kernel queued before an operator writes that operator's weights. */
+ * when no kernel queued before an operator writes that operator's weights.
+ * The token-scaled products and the paged cache need no flag: their kernels
+ * always start early and read nothing until the previous one is complete
+ * (weights are fetched into L2 before). */
 #define LQ_LAUNCH_PDL 1
 int lq_set_launch_flags(int flags);
 
@@ -236,8 +239,8 @@ typedef struct KVRows {
     const void* k;
     const void* v;
     void* q_out;        /* rotated queries; may be q itself */
-    void* k_out;        /* code * scale of the new rows as the cache now holds them; may be null */
-    void* v_out;
+    void* k_out;        /* code * scale of the new rows as the cache now holds them; may be */
+    void* v_out;        /* null; not k's or v's memory, which is read twice */
     int64_t ld_q, ld_k, ld_v, ld_q_out;
     int64_t ld_kv_out;  /* of k_out and v_out */
     int32_t n_heads;    /* query heads */

@@ -241,12 +241,11 @@ __device__ __forceinline__ float unbias(int d) { return __int_as_float(d) - kBia
 // column 2j + e of the even tile is token 4j + 2x + e with x = j / 2, of the odd
 // tile with x = 1 - j / 2.
 //
-// Measured, 128 dims: 64 sequences of up to 1100 tokens, 40 heads, fp32 120 us
-// (458 MB, 3.8 TB/s; 16-bit rows 91 us); 16 of up to 4000, 8 kv heads of 8 query
-// heads each, bf16 33 us (86 MB, 2.6 TB/s); one of 2048, 32 heads, fp32 14.5 us,
-// of which 10 us are a launch, the queries, one ring and the join.  What holds the
-// long ones is a step's chain (scores, maximum, weights, products, their unpacking)
-// and its issue slots, with twelve warps on an SM at 168 registers a thread.
+// Measured, 128 dims: 64 sequences of up to 1100 tokens, 40 heads, fp32 78 us (458
+// MB, 5.9 TB/s); 16 of up to 4000, 8 kv heads of 8 query heads each, bf16 24 us (86
+// MB, 3.6 TB/s), fp32 28 us; 16 of 8192 each 53 us (5.1 TB/s); one of 2048, 32
+// heads, fp32 10.7 us.  What holds the short ones is the chain lengths, pages,
+// codes, and the two joins: 5 us with one split to a sequence, 8 us with more.
 
 constexpr int kFewWarps = 4;
 constexpr int kFewThreads = 32 * kFewWarps;
@@ -885,15 +884,16 @@ cudaError_t few_launch(const AttArgs& a, dim3 grid, cudaStream_t st) {
 // more than 2^13 since its last one: weights are 2^kUnit at that maximum, 2^14 at
 // most, within f16's range.
 //
-// Measured, 1024 rows at the end of 4096 tokens, 32 heads of 128: bf16 132 us
-// (60 GFLOP, 455 TFLOP/s), fp32 153 us; what bounds it is a row tile's chain from
-// scores through softmax to the next product, which two row tiles on an SM hide
-// only in part (tensor pipe and issue slots are both under half busy).  Tiles of
-// 128 tokens with one buffer of scores: bf16 130 us, but f16 with 8 heads to a kv
-// head and pages of 16 176 us against 164, and head size 64 103 us against 98.
+// Measured, 1024 rows at the end of 4096 tokens, 32 heads of 128: bf16 117 us
+// (60 GFLOP, 515 TFLOP/s), fp32 152 us.  What bounds it is the conversion (93 us
+// without it), then a row tile's chain from scores through softmax to the next
+// product, which two row tiles on an SM hide only in part (tensor pipe and issue
+// slots are both under half busy).  Tiles of 128 tokens with one buffer of scores
+// were level in bf16, and slower in f16 with 8 heads to a kv head and pages of 16
+// (176 us against 164) and at head size 64 (103 us against 98).
 
 // Converting warps: codes to 16 bits are two or three instructions each, and with
-// four warps they held up the 16-bit types (132 us in the case below, 85 us without
+// four warps they held up the 16-bit types (132 us in the case above, 85 us without
 // any conversion).
 constexpr int many_converters(int ns) { return ns == 2 ? 8 : 4; }
 constexpr int many_threads(int ns) { return 32 * (8 + many_converters(ns) + 4); }
