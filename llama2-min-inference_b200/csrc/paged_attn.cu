@@ -761,17 +761,17 @@ __global__ void __launch_bounds__(kFewThreads, few_ctas(HS, ROWS)) attend_few_ke
         }
     }
     if (splits == 1) return;
-    __threadfence();
     __syncthreads();
     if (tid == 0) {
+        __threadfence();  // for the whole CTA: its stores were before the barrier
         int* cnt = a.cnt + s * (int)gridDim.x + blockIdx.x;
         const int n = atomicAdd(cnt, 1);
         last_flag = n == splits - 1;
         if (last_flag) *cnt = 0;  // as the next launch expects it
+        __threadfence();
     }
     __syncthreads();
     if (!last_flag) return;
-    __threadfence();
     // eight splits at a time, all their loads before the first use (one at a time
     // the join of three splits of 8 rows took 15 us)
     const float* all = part - split * hop;
