@@ -8,12 +8,16 @@
 //           65536), the digits signed bytes.  The digits' dots with the codes are
 //           exact; the score is (65536 D1 + 256 D2 + D3) * qs * scale * s_K[page].
 //           (Two digits would do for outputs of 16 bits, but not for lse.)
-//   p . V:  p * s_V[page] / max s_V of the 32 tokens is in [0, 1] and becomes 24
-//           bits (16 for the 16-bit types), whose bytes are unsigned digits.
+//   p . V:  p * s_V[page], relative to the largest of it among 32 tokens, is in
+//           [0, 1] and becomes 32 bits, whose bytes are unsigned digits; the
+//           largest joins the product's factor.
 //
-// A product's error so is 2^-24 of the row's largest term (2^-17 in p . V of the
-// 16-bit types, whose results carry 2^-9 or 2^-12), as the rounding of an fp32
-// sum.  Softmax statistics and the output's accumulator are fp32.
+// A term of q . K so is off by 2^-24 of the row's largest |q|, a weight by 2^-33 of
+// the largest p * s_V of its own 32 tokens and not of the row's: a key that takes
+// nearly all of the sum (an attention sink, whose V may be near zero) leaves the
+// thousands around it their bits.  (16 bits relative to the row's running maximum
+// lost 5% to 27% of such an output.)  Softmax statistics and the output's
+// accumulator are fp32.
 #include <cmath>
 
 #include "lq_ctx.h"
@@ -224,7 +228,7 @@ __device__ __forceinline__ float unbias(int d) { return __int_as_float(d) - kBia
 // Tiles of 8 rows (several query heads to a kv head, or several tokens): an
 // MMA's 16 rows are the 8 (token, head) rows twice: rows 0-7 hold their first
 // digit, rows 8-15 the second, so a thread finds both digits' dots of its row
-// in its own registers.  A third digit takes a second MMA.
+// in its own registers.  The third and the weights' fourth take a second MMA.
 //
 // One row (a token, and a query head to each kv head): the codes are the MMA's
 // 16 rows, 16 tokens of K or 16 dims of V, and the digits its columns, so that
@@ -242,8 +246,8 @@ __device__ __forceinline__ float unbias(int d) { return __int_as_float(d) - kBia
 // tile with x = 1 - j / 2.
 //
 // Measured, 128 dims: 64 sequences of up to 1100 tokens, 40 heads, fp32 78 us (458
-// MB, 5.9 TB/s); 16 of up to 4000, 8 kv heads of 8 query heads each, bf16 24 us (86
-// MB, 3.6 TB/s), fp32 28 us; 16 of 8192 each 53 us (5.1 TB/s); one of 2048, 32
+// MB, 5.9 TB/s); 16 of up to 4000, 8 kv heads of 8 query heads each, 26 us (86
+// MB, 3.3 TB/s); 16 of 8192 each 53 us (5.1 TB/s); one of 2048, 32
 // heads, fp32 10.7 us.  What holds the short ones is the chain lengths, pages,
 // codes, and the two joins: 5 us with one split to a sequence, 8 us with more.
 
@@ -251,6 +255,7 @@ constexpr int kFewWarps = 4;
 constexpr int kFewThreads = 32 * kFewWarps;
 constexpr int kItem = 32;   // tokens of one step of a warp
 constexpr int kSlots = 2;   // its ring
+constexpr float kLeast = 7.9e-31f;  // 2^-100: below it, a weight (of at most 1) counts as zero
 constexpr int kFewRows = 32;  // (token, head) rows of a sequence up to which it is taken
 
 // CTAs on an SM: what registers and the rings allow
@@ -301,8 +306,8 @@ __device__ __forceinline__ Split find_split(const KVBatch& b, int unit, int unit
     return {-1, 0, 0};
 }
 
-// ND: digits of the weights.  ROWS: rows of a tile, 8 or 1
-template <int ND, int HS, bool EXACT, int ROWS>
+// PARTS: 2 for fp32, 1 for the 16-bit types.  ROWS: rows of a tile, 8 or 1
+template <int PARTS, int HS, bool EXACT, int ROWS>
 __global__ void __launch_bounds__(kFewThreads, few_ctas(HS, ROWS)) attend_few_kernel(const __grid_constant__ AttArgs a) {
     constexpr int KS = HS / 32;       // k steps of q . K
     constexpr int NP = 2;             // MMAs of a tile of q . K: two digits, the third
@@ -403,7 +408,7 @@ __global__ void __launch_bounds__(kFewThreads, few_ctas(HS, ROWS)) attend_few_ke
 #pragma unroll
             for (int e = 0; e < 4; ++e) x[b][e] = 0.0f;
             if (have && d < hs) {
-                RawQ<ND - 1> raw;
+                RawQ<PARTS> raw;
                 raw.load(a, base + d);
                 raw.get(a, x[b]);
             }
@@ -507,7 +512,13 @@ __global__ void __launch_bounds__(kFewThreads, few_ctas(HS, ROWS)) attend_few_ke
                 if (t0 + 16 * c <= pos && (c == 0 || two)) poison = NAN;
                 sv[c] = 0.0f;
             }
+        // a page that the row does not see has no say in what its weights are relative to
+        if (P < kItem) {
+            if (t0 > pos) sv[0] = 0.0f;
+            if (t0 + 16 > pos) sv[1] = 0.0f;
+        }
         const float svm = fmaxf(sv[0], sv[1]);
+        constexpr float kOne = 4294967040.0f;  // the largest weight: 2^32 less an ulp
         if constexpr (ROWS == 1) {
             // scores: the codes of 16 tokens are the A operand, q's digits the
             // columns 0-2 and, again, 4-6.  A lane so finds one digit pair or third
@@ -537,28 +548,33 @@ __global__ void __launch_bounds__(kFewThreads, few_ctas(HS, ROWS)) attend_few_ke
             float x = (odd ? fmaf(other, 256.0f, mine) : fmaf(mine, 256.0f, other)) * (fs * (late ? sk[1] : sk[0]));
             const int at = 16 * late + 8 * odd + (lane >> 2);
             if (t0 + at > pos) x = -INFINITY;
-            const float top_new = fmaxf(m, max_redux(x));
+            const float top = max_redux(x), top_new = fmaxf(m, top);
             const float mref = top_new == -INFINITY ? 0.0f : top_new;
             const float corr = exp2_fast(m - mref);  // 0 for the first tokens
+            const float rise = exp2_fast(top - mref);
             m = top_new;
-            const float p = exp2_fast(x - mref);
-            l = fmaf(l, corr, p);
+            const float p = exp2_fast(x - (top == -INFINITY ? 0.0f : top));
+            l = fmaf(l, corr, p * rise);
             // the weight in fixed point; its bytes are the B operand's columns
-            constexpr float kOne = ND == 3 ? 16777215.0f : 65535.0f;
-            const float w = p * (svm > 0.0f ? (late ? sv[1] : sv[0]) / svm * kOne : 0.0f);
+            float w = p, of = svm * rise * (1.0f / kOne);
+            if (P < kItem) {  // two pages
+                w = svm > 0.0f ? p * ((late ? sv[1] : sv[0]) / svm) : 0.0f;
+                const float most = max_redux(w);
+                w = most > kLeast ? w / most : 0.0f;
+                of *= most;
+            }
             uint32_t* wt = reinterpret_cast<uint32_t*>(weights) + warp * kItem;
-            wt[at] = ND == 3 ? __float2uint_rn(w) : __float_as_uint(w + 8388608.0f);
+            wt[at] = __float2uint_rn(w * kOne);
             __syncwarp();
             uint32_t b[2];
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const uint4 u = weights[warp * (kItem / 4) + 4 * i + jj];
-                const int byte = ND - 1 - min(lane >> 2, ND - 1);
+                const int byte = 3 - min(lane >> 2, 3);
                 const uint32_t sel = ((4u + byte) << 4) | byte;
                 b[i] = __byte_perm(__byte_perm(u.x, u.y, sel), __byte_perm(u.z, u.w, sel), 0x5410u);
-                if (lane >> 2 >= ND) b[i] = 0;
+                if (lane >> 2 >= 4) b[i] = 0;
             }
-            const float of = svm * (ND == 3 ? 1.0f / 16777215.0f : 1.0f / 65535.0f);
             const bool turn = corr != 1.0f;  // alike in all lanes
 #pragma unroll
             for (int t = 0; t < NT; t += 2) {
@@ -576,7 +592,7 @@ __global__ void __launch_bounds__(kFewThreads, few_ctas(HS, ROWS)) attend_few_ke
             }
             __syncwarp();  // the weights are read
         } else {
-            float top_new = m;
+            float top = -INFINITY;
             float x[4][2];
 #pragma unroll
             for (int c = 0; c < 2; ++c) {  // 16 tokens: tiles 2c and 2c + 1
@@ -611,46 +627,64 @@ __global__ void __launch_bounds__(kFewThreads, few_ctas(HS, ROWS)) attend_few_ke
                         v *= f;
                         if (t + e > pos) v = -INFINITY;
                         x[2 * c + i][e] = v;
-                        top_new = fmaxf(top_new, v);
+                        top = fmaxf(top, v);
                     }
                 }
             }
-            top_new = fmaxf(top_new, __shfl_xor_sync(0xffffffffu, top_new, 1));
-            top_new = fmaxf(top_new, __shfl_xor_sync(0xffffffffu, top_new, 2));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            const float top_new = fmaxf(m, top), top_ref = top == -INFINITY ? 0.0f : top;
             const float mref = top_new == -INFINITY ? 0.0f : top_new;
             const float corr = exp2_fast(m - mref);  // 0 for the first tokens
+            const float rise = exp2_fast(top - mref);
             m = top_new;
-            l *= corr;
+            float sum = 0.0f, of = svm * rise * (1.0f / kOne);
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    x[t][e] = exp2_fast(x[t][e] - top_ref);
+                    sum += x[t][e];
+                }
+            l = fmaf(l, corr, sum * rise);
+            if (P < kItem) {  // two pages
+                float most = 0.0f;
+#pragma unroll
+                for (int t = 0; t < 4; ++t) {
+                    const float w = svm > 0.0f ? sv[t / 2] / svm : 0.0f;
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        x[t][e] *= w;
+                        most = fmaxf(most, x[t][e]);
+                    }
+                }
+                most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+                most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+#pragma unroll
+                for (int t = 0; t < 4; ++t)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) x[t][e] = most > kLeast ? x[t][e] / most : 0.0f;
+                of *= most;
+            }
             // weights in fixed point; their bytes are the A operand
             uint4 pa, pb;
             uint32_t* pw[2] = {reinterpret_cast<uint32_t*>(&pa), reinterpret_cast<uint32_t*>(&pb)};
-            pb = make_uint4(0, 0, 0, 0);
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                constexpr float kOne = ND == 3 ? 16777215.0f : 65535.0f;
-                const float w = svm > 0.0f ? sv[c] / svm * kOne : 0.0f;
                 uint32_t u[2][2];
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const float p = exp2_fast(x[2 * c + i][e] - mref);
-                        l += p;
-                        u[i][e] = ND == 3 ? __float2uint_rn(p * w) : __float_as_uint(p * w + 8388608.0f);
-                    }
+                    for (int e = 0; e < 2; ++e) u[i][e] = __float2uint_rn(x[2 * c + i][e] * kOne);
                 const uint32_t order = jj < 2 ? 0x5410u : 0x1054u;
 #pragma unroll
-                for (int k = 0; k < ND; ++k) {  // byte ND - 1 - k of the four weights
-                    const uint32_t sel = ((4u + ND - 1 - k) << 4) | (ND - 1 - k);
+                for (int k = 0; k < 4; ++k) {  // byte 3 - k of the four weights
+                    const uint32_t sel = ((7u - k) << 4) | (3u - k);
                     const uint32_t word =
                         __byte_perm(__byte_perm(u[0][0], u[0][1], sel), __byte_perm(u[1][0], u[1][1], sel), order);
-                    if (k < 2)
-                        pw[0][c * 2 + k] = word;
-                    else
-                        pw[1][c * 2] = word;
+                    pw[k / 2][c * 2 + k % 2] = word;
                 }
             }
-            const float of = svm * (ND == 3 ? 1.0f / 16777215.0f : 1.0f / 65535.0f);
             const bool turn = __any_sync(0xffffffffu, corr != 1.0f);
 #pragma unroll
             for (int t = 0; t < NT; t += 2) {
@@ -662,7 +696,7 @@ __global__ void __launch_bounds__(kFewThreads, few_ctas(HS, ROWS)) attend_few_ke
                     int d[4] = {kBiasBits, kBiasBits, kBiasBits, kBiasBits};
                     int d3[4] = {kBiasBits, kBiasBits, kBiasBits, kBiasBits};
                     mma_u8(d, pa, b[2 * i], b[2 * i + 1]);
-                    if (ND == 3) mma_u8(d3, pb, b[2 * i], b[2 * i + 1]);
+                    mma_u8(d3, pb, b[2 * i], b[2 * i + 1]);
                     if (turn) {
                         o[t + i][0] *= corr;
                         o[t + i][1] *= corr;
@@ -670,7 +704,8 @@ __global__ void __launch_bounds__(kFewThreads, few_ctas(HS, ROWS)) attend_few_ke
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
                         float v = fmaf(unbias(d[e]), 256.0f, unbias(d[2 + e]));
-                        if (ND == 3) v = fmaf(v, 256.0f, unbias(d3[e]));
+                        v = fmaf(v, 256.0f, unbias(d3[e]));
+                        v = fmaf(v, 256.0f, unbias(d3[2 + e]));
                         o[t + i][e] = fmaf(v, of, o[t + i][e]);
                     }
                 }
@@ -703,9 +738,9 @@ __global__ void __launch_bounds__(kFewThreads, few_ctas(HS, ROWS)) attend_few_ke
             if (!EXACT && t * 8 >= hs) break;
             if constexpr (ROWS == 8) {
                 *reinterpret_cast<float2*>(mine + t * 8 + 2 * jj) = make_float2(o[t][0] + poison, o[t][1] + poison);
-            } else {  // dim 8 t + lane / 4: two digits here, the third by the next lane
+            } else {  // dim 8 t + lane / 4: two digits here, the others by the next lane
                 float v = fmaf(o[t][0], 256.0f, o[t][1]);
-                if (ND == 3) v = fmaf(v, 256.0f, __shfl_down_sync(0xffffffffu, o[t][0], 1));
+                v = fmaf(v, 65536.0f, __shfl_down_sync(0xffffffffu, v, 1));
                 if (jj == 0) mine[t * 8 + (lane >> 2)] = v + poison;
             }
         }
@@ -818,9 +853,9 @@ __global__ void __launch_bounds__(kFewThreads, few_ctas(HS, ROWS)) attend_few_ke
     }
 }
 
-template <int ND, int HS, bool EXACT, int ROWS>
+template <int PARTS, int HS, bool EXACT, int ROWS>
 cudaError_t few_launch(const AttArgs& a, dim3 grid, cudaStream_t st) {
-    auto kern = attend_few_kernel<ND, HS, EXACT, ROWS>;
+    auto kern = attend_few_kernel<PARTS, HS, EXACT, ROWS>;
     constexpr int join = kFewWarps * ROWS * (HS + 8) * 4;
     constexpr int smem = few_smem<HS>() > join ? few_smem<HS>() : join;
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
@@ -840,15 +875,15 @@ cudaError_t few_launch(const AttArgs& a, dim3 grid, cudaStream_t st) {
     return cudaLaunchKernelEx(&cfg, kern, a);
 }
 
-template <int ND, int ROWS>
+template <int PARTS, int ROWS>
 cudaError_t few_launch(const AttArgs& a, dim3 grid, cudaStream_t st) {
     const int hs = a.c.head_size;
-    if (hs == 64) return few_launch<ND, 64, true, ROWS>(a, grid, st);
-    if (hs == 128) return few_launch<ND, 128, true, ROWS>(a, grid, st);
-    if (hs == 256) return few_launch<ND, 256, true, ROWS>(a, grid, st);
-    if (hs < 64) return few_launch<ND, 64, false, ROWS>(a, grid, st);
-    if (hs < 128) return few_launch<ND, 128, false, ROWS>(a, grid, st);
-    return few_launch<ND, 256, false, ROWS>(a, grid, st);
+    if (hs == 64) return few_launch<PARTS, 64, true, ROWS>(a, grid, st);
+    if (hs == 128) return few_launch<PARTS, 128, true, ROWS>(a, grid, st);
+    if (hs == 256) return few_launch<PARTS, 256, true, ROWS>(a, grid, st);
+    if (hs < 64) return few_launch<PARTS, 64, false, ROWS>(a, grid, st);
+    if (hs < 128) return few_launch<PARTS, 128, false, ROWS>(a, grid, st);
+    return few_launch<PARTS, 256, false, ROWS>(a, grid, st);
 }
 
 // ---------------------------------------------------------------------------
@@ -1562,9 +1597,9 @@ extern "C" int paged_attention(void* out, int64_t ld_out, const void* q, int64_t
     const dim3 grid((unsigned)x, (unsigned)units);
     cudaError_t e = cudaSuccess;
     if (a.few_rows && tile_rows == 1)
-        e = type == LQ_F32 ? few_launch<3, 1>(a, grid, stream()) : few_launch<2, 1>(a, grid, stream());
+        e = type == LQ_F32 ? few_launch<2, 1>(a, grid, stream()) : few_launch<1, 1>(a, grid, stream());
     else if (a.few_rows)
-        e = type == LQ_F32 ? few_launch<3, 8>(a, grid, stream()) : few_launch<2, 8>(a, grid, stream());
+        e = type == LQ_F32 ? few_launch<2, 8>(a, grid, stream()) : few_launch<1, 8>(a, grid, stream());
     if (e != cudaSuccess) return cuda_fail(e, "paged_attention launch");
     if (most_rows > kFewRows) {
         e = type == LQ_F32   ? many_launch<LQ_F32>(a, stream())

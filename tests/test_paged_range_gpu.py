@@ -1,0 +1,148 @@
+"""paged_attention where weights, page scales and queries span many orders of
+magnitude: an attention sink over thousands of small weights, pages whose value
+scales lie up to 2^30 apart, seen and unseen ones."""
+import math
+
+import numpy as np
+import pytest
+
+from paged_ref import HALF_ULP, Batch, attention, k_index, random_cache, sequence_kv, v_index
+from test_paged_gpu import run_attention
+
+pytestmark = pytest.mark.gpu
+
+
+def sink_cache(rng, batch, kv_heads, hs, page, where):
+    """Keys that one direction of q tells apart: dim 0 of token `where` of every
+    sequence holds 127, of the others -8 to 8; the rest is small.  The sink's
+    values are zero, the others' all of one sign."""
+    codes, scales = random_cache(rng, batch.n_pages, kv_heads, hs, page)
+    k = rng.integers(-3, 4, (batch.n_pages, kv_heads, page, hs)).astype(np.int8)
+    k[..., 0] = rng.integers(-8, 9, k.shape[:-1])
+    v = rng.integers(20, 101, k.shape).astype(np.int8)
+    for s in range(len(batch.rows)):
+        p = int(batch.pages[s, where // page])
+        k[p, :, where % page, 0] = 127
+        v[p, :, where % page] = 0
+    codes[:, :, 0][:, :, k_index(hs, page)] = k
+    codes[:, :, 1][:, :, v_index(hs, page)] = v
+    scales[:] = np.float32(1 / 127)
+    return codes, scales
+
+
+def bound(q, codes, scales, batch, dtype, scale, step, floor):
+    """out in 64 bits, and what its error may be: scores as in paged_ref.attention;
+    every weight off by `step` of itself, and those of 32 neighbouring tokens by
+    `floor` of the row's largest p * s_V (the others are measured against
+    something smaller); the last rounding."""
+    eq = 2.0**-22 if dtype == "f32" else 2.0**-14
+    n, heads, hs = q.shape
+    g = heads // codes.shape[1]
+    out, tol = np.zeros(q.shape), np.zeros(q.shape)
+    for s in range(len(batch.rows)):
+        for h in range(codes.shape[1]):
+            k, v, sk, sv = sequence_kv(codes, scales, batch, s, h, hs)
+            kv, vv = k * sk[:, None], v * sv[:, None]
+            size = np.abs(k).sum(1) * sk * abs(scale)
+            for i in range(batch.rows[s]):
+                row, m = batch.row_start[s] + i, batch.ctx[s] - batch.rows[s] + i + 1
+                for e in range(h * g, h * g + g):
+                    x = q[row, e]
+                    sc = kv[:m] @ x * scale
+                    ds = (size[:m] * np.abs(x).max() * eq
+                          + 4 * 2.0**-24 * abs(scale) * (np.abs(kv[:m]) @ np.abs(x))).max()
+                    p = np.exp(sc - sc.max())
+                    p /= p.sum()
+                    out[row, e] = p @ vv[:m]
+                    mag = p @ np.abs(vv[:m])
+                    tol[row, e] = ((2 * (ds + 2.0**-20) + step) * 2 * mag + 32 * 127 * floor * (p * sv[:m]).max()
+                                   + 2 * HALF_ULP[dtype] * np.abs(out[row, e]) + 1e-30)
+    return out, tol
+
+
+# the type's range: from here on values round to infinity; half the distance of its smallest values
+LARGEST = {"f32": 2.0**128, "f16": 65520.0, "bf16": 2.0**128}
+SMALL = {"f32": 2.0**-150, "f16": 2.0**-25, "bf16": 2.0**-134}
+
+
+def agree(out, want, tol, dtype):
+    """Within tol, where the type's range allows: past it a value rounds to
+    infinity, below its normal numbers to a multiple of the smallest."""
+    tol = tol + SMALL[dtype]
+    over = np.abs(want) >= LARGEST[dtype]
+    assert np.all(np.isinf(out[over]) | (np.abs(want[over]) - tol[over] < LARGEST[dtype]))
+    assert np.all(np.sign(out[over]) == np.sign(want[over]))
+    err = np.abs(out[~over] - want[~over])
+    near = np.isinf(out[~over]) & (np.abs(want[~over]) + tol[~over] >= LARGEST[dtype])
+    assert np.all((err <= tol[~over]) | near), np.nanmax(err / tol[~over])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("name,seqs,rows,ctx,kv_heads,group", [
+    ("split, one row", 1, 1, 4000, 2, 1), ("split, eight rows", 1, 2, 4000, 1, 4),
+    ("whole contexts, one row", 60, 1, 1100, 8, 1), ("whole contexts, eight rows", 30, 1, 1100, 16, 2),
+])
+def test_attend_sink(cuda, dtype, page, name, seqs, rows, ctx, kv_heads, group):
+    """One key takes most of the sum and gives nothing to the output, which is what
+    thousands of others 11 to 13 nats lower leave."""
+    check_sink(cuda, dtype, page, seqs, rows, ctx, kv_heads, group)
+
+
+def check_sink(cuda, dtype, page, seqs, rows, ctx, kv_heads, group):
+    hs = 64
+    rng = np.random.default_rng(ctx + page)
+    batch = Batch(rng, [rows] * seqs, [ctx] * seqs, page)
+    codes, scales = sink_cache(rng, batch, kv_heads, hs, page, 5)
+    q = rng.standard_normal((batch.n_rows, kv_heads * group, hs)) * 0.1
+    q[..., 0] = 12 * math.sqrt(hs)  # the sink's key is 1 there, the others' about 0
+    qv, out, _ = run_attention(cuda, q, codes, scales, batch, dtype, hs, 1 / math.sqrt(hs))
+    # a weight's own form: 24 or 32 fixed bits in blocks of 32, or one or two f16
+    step, floor = (2.0**-21, 2.0**-31) if dtype == "f32" else (2.0**-11, 2.0**-24)
+    want, tol = bound(qv, codes, scales, batch, dtype, 1 / math.sqrt(hs), step, floor)
+    agree(out, want, tol, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("group", [1, 4])
+@pytest.mark.parametrize("order", ["falling", "rising", "mixed"])
+def test_attend_page_scales_apart(cuda, dtype, group, order):
+    """Two pages in one step of 32 tokens, their value scales 2^0 to 2^30 apart;
+    contexts that end in the first, the second or later: what a row does not see
+    has no say, and a page it hardly attends to takes nothing from the others."""
+    rng = np.random.default_rng(group)
+    hs, page, kv_heads = 64, 16, 2
+    ctx = [1, 5, 16, 17, 20, 32, 33, 50, 64, 80, 100]
+    batch = Batch(rng, [1] * len(ctx), ctx, page)
+    codes, scales = random_cache(rng, batch.n_pages, kv_heads, hs, page)
+    spread(rng, batch, scales, order)
+    q = rng.standard_normal((batch.n_rows, kv_heads * group, hs)) * 2
+    # the slots past a context's last page: a page of the largest scale, unseen
+    qv, out, lse = run_attention(cuda, q, codes, scales, batch, dtype, hs, 0.125)
+    want, wlse, tol, ltol = attention(qv, codes, scales, batch, dtype, 0.125)
+    agree(out, want, tol, dtype)
+    assert np.all(np.abs(lse - wlse) <= ltol)
+
+
+def spread(rng, batch, scales, order):
+    for s, c in enumerate(batch.ctx):
+        n = -(-c // batch.page)
+        k = {"falling": -np.arange(n) * 30 // max(n - 1, 1), "rising": np.arange(n) * 30 // max(n - 1, 1),
+             "mixed": rng.permutation(n) * 30 // max(n - 1, 1)}[order]
+        p = batch.pages[s, :n].astype(np.int64)
+        scales[p, :, 1] = (2.0 ** (k - 15))[:, None] * (1 + rng.random((n, scales.shape[1])))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_attend_unseen_half_of_a_step(cuda, dtype):
+    """Rows of one tile that see one or both of two pages: the second's scale,
+    2^30 times the first's, is nothing to rows before it."""
+    rng = np.random.default_rng(3)
+    hs, page = 64, 16
+    batch = Batch(rng, [8], [20], page)  # positions 12 .. 19
+    codes, scales = random_cache(rng, batch.n_pages, 1, hs, page)
+    scales[int(batch.pages[0, 1]), :, 1] = 2.0**25
+    q = rng.standard_normal((8, 1, hs)) * 2
+    qv, out, _ = run_attention(cuda, q, codes, scales, batch, dtype, hs, 0.125)
+    want, _, tol, _ = attention(qv, codes, scales, batch, dtype, 0.125)
+    agree(out, want, tol, dtype)
