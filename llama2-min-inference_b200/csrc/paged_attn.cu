@@ -1,8 +1,9 @@
 // paged_attention: causal attention of ragged rows over the paged int8 cache.
 //
-// Both products run on integer tensor-core instructions over the cache's
-// codes as they lie, so that no code is ever converted.  The other operand is
-// written in fixed point, as int8 digits:
+// Two kernels.  Prompts' codes become 16-bit floats for tcgen05 (below, with what
+// that costs in accuracy).  For few rows both products run on integer tensor-core
+// instructions over the cache's codes as they lie, so that no code is converted.
+// The other operand is written in fixed point, as int8 digits:
 //
 //   q . K:  a row of q is qs * (65536 d1 + 256 d2 + d3), qs = max|q| / (127 *
 //           65536), the digits signed bytes.  The digits' dots with the codes are
@@ -913,14 +914,17 @@ cudaError_t few_launch(const AttArgs& a, dim3 grid, cudaStream_t st) {
 // is in softmax.
 //
 // s_K multiplies scores by 16-token granules (one FMA with the exponent's
-// shift); s_V enters as its logarithm: a weight's exponent gets log2(s_V / max
-// s_V over the context), so O needs no second scaling, and the sum divides it
-// out again per granule.  O is rescaled only when a row's maximum has grown by
-// more than 2^13 since its last one: weights are 2^kUnit at that maximum, 2^14 at
-// most, within f16's range.
+// shift); s_V enters as its logarithm: a weight's exponent gets log2(s_V / the
+// first s_V of the sequence), so O needs no second scaling, and the sum divides it
+// out again per granule.  The maximum that a row follows is that of score plus
+// logarithm, over what the row sees: the weights that count are the ones with bits,
+// however far apart the pages' scales lie, and pages that a row does not see or
+// hardly attends to take none.  O is rescaled only when that maximum has grown by
+// more than 2^kGrow since its last one: weights are 2^kUnit at that maximum, 2^14 at
+// most, and have 11 bits, down to 2^-31 of the largest (fp32: 22, down to 2^-36).
 //
 // Measured, 1024 rows at the end of 4096 tokens, 32 heads of 128: bf16 117 us
-// (60 GFLOP, 515 TFLOP/s), fp32 152 us.  What bounds it is the conversion (93 us
+// (60 GFLOP, 515 TFLOP/s), fp32 161 us.  What bounds it is the conversion (93 us
 // without it), then a row tile's chain from scores through softmax to the next
 // product, which two row tiles on an SM hide only in part (tensor pipe and issue
 // slots are both under half busy).  Tiles of 128 tokens with one buffer of scores
@@ -932,10 +936,18 @@ cudaError_t few_launch(const AttArgs& a, dim3 grid, cudaStream_t st) {
 // any conversion).
 constexpr int many_converters(int ns) { return ns == 2 ? 8 : 4; }
 constexpr int many_threads(int ns) { return 32 * (8 + many_converters(ns) + 4); }
-constexpr float kGrow = 13.0f, kUnit = 1.0f;
+// A row's maximum may grow by 2^kGrow before O is rescaled.  Their sum is 14, of f16's
+// 16 bits upwards (a score of some 10^7 rounds by a bit); what kGrow leaves to kUnit is
+// what small weights keep.  fp32 with 11 + 3 160 us, 6 + 8 159 us, 4 + 10 154 us in the case
+// above; f16 with 8 heads to a kv head 177, 161 and 159 us.
+constexpr float grow_bits(int parts) { return parts == 2 ? 3.0f : 8.0f; }
+// s_V relative to the sequence's first: beyond 2^kFar either way it counts as that,
+// and as no less than 2^-kBelow of the largest so far, so that a weight's share of the sum
+// (its product with `inv`) stays a normal number
+constexpr float kFar = 100.0f, kBelow = 80.0f;
 
 struct Granule {  // 16 tokens
-    float sk, shift, inv, bad;  // s_K, log2(weight) + kUnit, 1 / (weight * 2^kUnit), NaN where s_V is not finite
+    float sk, shift, inv, bad;  // s_K, log2(s_V / first), 2^-shift, NaN where s_V is not finite
 };
 
 struct ManyBars {
@@ -943,7 +955,7 @@ struct ManyBars {
     uint64_t tabfull[4], tabempty[4];
     uint32_t tmem_base;
     int abort_flag;
-    uint32_t peak;       // bits of the largest finite s_V of the context
+    float first;         // the s_V that the others are relative to
     Granule gran[4][8];  // by tile, four deep
     int64_t cell[4][8];  // the granules' pages: byte offset of the head's codes, or -1
     float fs[256];       // rows' factors of the scores
@@ -998,6 +1010,7 @@ __global__ void __launch_bounds__(many_threads(NS), 1) attend_many_kernel(const 
     constexpr int kIssuers = NS == 2 ? NQ : 1;  // warps that issue MMAs: one per row tile, or one for all
     constexpr int PARTS = Lay::kParts;
     constexpr bool kBf16 = TYPE == LQ_BF16;
+    constexpr float kGrow = grow_bits(PARTS), kUnit = 14.0f - kGrow;
     constexpr int kConv = many_converters(NS), kIssue = 8 + kConv;  // converting warps; the first issuing warp
     constexpr int kLoads = HS / 16 * TK / (32 * kConv);  // 16-byte pieces of K (and of V) per converting thread
     extern __shared__ __align__(1024) unsigned char raw[];
@@ -1047,27 +1060,14 @@ __global__ void __launch_bounds__(many_threads(NS), 1) attend_many_kernel(const 
             mbar_init(&bars->vempty[i], kIssuers);
         }
         bars->abort_flag = 0;
-        bars->peak = 0;
         fence_mbar_init();
     }
     if (warp == kIssue) tmem_alloc<1, 512>(&bars->tmem_base);
     const int lp2 = __ffs(P) - 1;
-    const int32_t* pages = a.b.pages + (int64_t)s * a.b.max_pages;
-    uint32_t pk = 0;
-    for (int lp = tid; lp << lp2 < seen && lp < a.b.max_pages; lp += many_threads(NS)) {
-        const int p = __ldg(pages + lp);
-        if (p < 0 || p >= a.c.n_pages) continue;  // reported below
-        const uint32_t v = abs_bits(__ldg(a.c.scales + ((int64_t)p * H + h) * 2 + 1));
-        if (v < kInfBits) pk = max(pk, v);
-    }
-    pk = __reduce_max_sync(0xffffffffu, pk);
     tc_fence_before();
-    __syncthreads();
-    if (lane == 0 && pk) atomicMax(&bars->peak, pk);
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = bars->tmem_base;
-    const float svm = bars->peak ? __uint_as_float(bars->peak) : 1.0f;
     const int8_t* codes = static_cast<const int8_t*>(a.c.codes);
 
     // 512 threads have 128 registers each; 128 scores a thread take a larger share,
@@ -1253,6 +1253,7 @@ __global__ void __launch_bounds__(many_threads(NS), 1) attend_many_kernel(const 
                 }
             };
             Granule gr = {};
+            float first = 1.0f, most = -kFar;
             look_up(0);
             for (int j = 0; j < tiles; ++j) {
                 if (j % kRound == 0) {
@@ -1260,8 +1261,20 @@ __global__ void __launch_bounds__(many_threads(NS), 1) attend_many_kernel(const 
                     sc = sc_next;
                     look_up(j + kRound);
                     const bool fine = sc.y < INFINITY;
-                    const float w = fine ? fmaxf(sc.y / svm, 9.094947e-13f) : 1.0f;  // 2^-40 at least
-                    const float shift = log2f(w) + kUnit;
+                    if (j == 0) {
+                        const uint32_t some = __ballot_sync(0xffffffffu, fine && sc.y > 0.0f);
+                        if (some) first = __shfl_sync(0xffffffffu, sc.y, __ffs(some) - 1);
+                        if (lane == 0) bars->first = first;
+                    }
+                    float shift = fine ? fminf(fmaxf(log2f(sc.y / first), -kFar), kFar) : -kFar, up = shift;
+#pragma unroll
+                    for (int o = 1; o < 32; o *= 2) {  // the largest up to this granule
+                        const float x = __shfl_up_sync(0xffffffffu, up, o);
+                        if (lane >= o) up = fmaxf(up, x);
+                    }
+                    up = fmaxf(up, most);
+                    most = __shfl_sync(0xffffffffu, up, 31);
+                    shift = fmaxf(shift, up - kBelow);
                     gr = {sc.x, shift, exp2f(-shift), fine ? 0.0f : NAN};
                 }
                 if (!__all_sync(0xffffffffu, qwait(&bars->tabempty[j & 3], (uint32_t)(((j >> 2) & 1) ^ 1), a.err,
@@ -1412,19 +1425,24 @@ __global__ void __launch_bounds__(many_threads(NS), 1) attend_many_kernel(const 
                     float t[5];
 #pragma unroll
                     for (int k = 0; k < 5; ++k) t[k] = max3(y[3 * k], y[3 * k + 1], y[3 * k + 2]);
-                    m = fmaxf(m, fmaxf(max3(t[0], t[1], t[2]), max3(t[3], t[4], y[15])) * (fs * gr[e].sk));
+                    m = fmaxf(m, fmaf(fmaxf(max3(t[0], t[1], t[2]), max3(t[3], t[4], y[15])), fs * gr[e].sk, gr[e].shift));
                 }
-                const bool grown = j == 0 ? m > -INFINITY : m > mref + kGrow;
+                const bool grown = j == 0 ? m > -INFINITY : m > mref + (kUnit + kGrow);
                 if (__any_sync(0xffffffffu, grown)) {
-                    const float next = grown ? m : mref;
+                    const float next = grown ? m - kUnit : mref;
                     const float f = exp2_fast(mref - next);
                     mref = next;
-                    if (j > 0) {  // the product before last is done: these scores were issued after it
+                    if (j > 0) {
                         l *= f;
-                        ok = __all_sync(0xffffffffu, qwait(&bars->pvdone[i], (uint32_t)((j - 1) & 1), a.err,
-                                                           DEV_TIMEOUT_TFULL, abort_flag));
-                        if (!ok) break;
+                        if constexpr (NS == 2) {  // else the scores were issued after the product before them
+                            ok = __all_sync(0xffffffffu, qwait(&bars->pvdone[i], (uint32_t)((j - 1) & 1), a.err,
+                                                               DEV_TIMEOUT_TFULL, abort_flag));
+                            if (!ok) break;
+                        }
                         tc_fence_after();
+                        // a short loop: it runs rarely, and fetching its instructions took
+                        // longer than they do (fp32 170 us unrolled, 162 us)
+#pragma unroll 1
                         for (int c = 0; c < hs; c += 16) {
                             int y[16];
                             tmem_ld<16>(to + c, y);
@@ -1446,8 +1464,8 @@ __global__ void __launch_bounds__(many_threads(NS), 1) attend_many_kernel(const 
                         // a masked -infinity has to stay one: no factor of zero, and
                         // no NaN from a granule that the row does not see
                         const bool sees = c * 32 + e * 16 <= left;
-                        float f = sees ? fs * gg.sk : 1e-38f;
-                        if (f == 0.0f) f = 1e-38f;
+                        float f = sees ? fs * gg.sk : 1.4e-45f;
+                        if (f == 0.0f) f = 1.4e-45f;
                         if (sees) poison += gg.bad;
                         const uint64_t f2 = f2_pack(f, f), b2 = f2_pack(gg.shift - mref, gg.shift - mref);
                         uint64_t sum[2];
@@ -1481,7 +1499,7 @@ __global__ void __launch_bounds__(many_threads(NS), 1) attend_many_kernel(const 
                 ok = __all_sync(0xffffffffu, qwait(&bars->last[i], 0, a.err, DEV_TIMEOUT_TFULL, abort_flag));
             tc_fence_after();
             if (ok) {
-                const float f = svm * 0.5f / l;  // 2^-kUnit
+                const float f = bars->first / l;
                 const int64_t at = (int64_t)(q.r0 + r / g) * a.ld_out + (int64_t)(h * g + r % g) * hs;
                 for (int c = 0; c < hs; c += 16) {
                     int y[16];

@@ -30,11 +30,11 @@ def sink_cache(rng, batch, kv_heads, hs, page, where):
     return codes, scales
 
 
-def bound(q, codes, scales, batch, dtype, scale, step, floor):
+def bound(q, codes, scales, batch, dtype, scale, step, floor, every):
     """out in 64 bits, and what its error may be: scores as in paged_ref.attention;
-    every weight off by `step` of itself, and those of 32 neighbouring tokens by
-    `floor` of the row's largest p * s_V (the others are measured against
-    something smaller); the last rounding."""
+    every weight off by `step` of itself, and `every` weight, or those of 32
+    neighbouring tokens (the others are measured against something smaller), by
+    `floor` of the row's largest p * s_V; the last rounding."""
     eq = 2.0**-22 if dtype == "f32" else 2.0**-14
     n, heads, hs = q.shape
     g = heads // codes.shape[1]
@@ -55,7 +55,8 @@ def bound(q, codes, scales, batch, dtype, scale, step, floor):
                     p /= p.sum()
                     out[row, e] = p @ vv[:m]
                     mag = p @ np.abs(vv[:m])
-                    tol[row, e] = ((2 * (ds + 2.0**-20) + step) * 2 * mag + 32 * 127 * floor * (p * sv[:m]).max()
+                    count = np.abs(v[:m]).sum(0) if every else 32 * 127
+                    tol[row, e] = ((2 * (ds + 2.0**-20) + step) * 2 * mag + count * floor * (p * sv[:m]).max()
                                    + 2 * HALF_ULP[dtype] * np.abs(out[row, e]) + 1e-30)
     return out, tol
 
@@ -89,17 +90,19 @@ def test_attend_sink(cuda, dtype, page, name, seqs, rows, ctx, kv_heads, group):
     check_sink(cuda, dtype, page, seqs, rows, ctx, kv_heads, group)
 
 
-def check_sink(cuda, dtype, page, seqs, rows, ctx, kv_heads, group):
-    hs = 64
+def check_sink(cuda, dtype, page, seqs, rows, ctx, kv_heads, group, hs=64, where=5):
     rng = np.random.default_rng(ctx + page)
     batch = Batch(rng, [rows] * seqs, [ctx] * seqs, page)
-    codes, scales = sink_cache(rng, batch, kv_heads, hs, page, 5)
+    codes, scales = sink_cache(rng, batch, kv_heads, hs, page, where)
     q = rng.standard_normal((batch.n_rows, kv_heads * group, hs)) * 0.1
     q[..., 0] = 12 * math.sqrt(hs)  # the sink's key is 1 there, the others' about 0
     qv, out, _ = run_attention(cuda, q, codes, scales, batch, dtype, hs, 1 / math.sqrt(hs))
-    # a weight's own form: 24 or 32 fixed bits in blocks of 32, or one or two f16
-    step, floor = (2.0**-21, 2.0**-31) if dtype == "f32" else (2.0**-11, 2.0**-24)
-    want, tol = bound(qv, codes, scales, batch, dtype, 1 / math.sqrt(hs), step, floor)
+    # a weight's own form: 24 or more fixed bits in blocks of 32, or one or two f16,
+    # whose smallest step is 2^-24 where the largest weight is 2^6 (fp32: 2^11) or more
+    many = rows * group > 32
+    step = 2.0**-21 if dtype == "f32" else 2.0**-11
+    floor = (2.0**-36, 2.0**-31)[dtype != "f32"] if many else (2.0**-31, 2.0**-24)[dtype != "f32"]
+    want, tol = bound(qv, codes, scales, batch, dtype, 1 / math.sqrt(hs), step, floor, many)
     agree(out, want, tol, dtype)
 
 
@@ -146,3 +149,47 @@ def test_attend_unseen_half_of_a_step(cuda, dtype):
     qv, out, _ = run_attention(cuda, q, codes, scales, batch, dtype, hs, 0.125)
     want, _, tol, _ = attention(qv, codes, scales, batch, dtype, 0.125)
     agree(out, want, tol, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows,ctx,group,hs,page,where", [
+    (40, 4000, 1, 64, 16, 5), (40, 3000, 4, 64, 64, 2900), (300, 700, 1, 64, 32, 0), (40, 1500, 1, 128, 64, 700),
+    (40, 1500, 1, 192, 16, 700)])
+def test_attend_sink_prompt(cuda, dtype, rows, ctx, group, hs, page, where):
+    """The same from a prompt's rows, the sink at the start, within and near the end."""
+    check_sink(cuda, dtype, page, 1, rows, ctx, 1, group, hs, where)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("order", ["falling", "rising", "mixed"])
+@pytest.mark.parametrize("group,hs,page", [(1, 64, 16), (2, 128, 64), (1, 192, 32)])
+def test_attend_page_scales_apart_prompt(cuda, dtype, order, group, hs, page):
+    """Value scales 2^0 to 2^30 apart before, behind and at the rows' positions."""
+    rng = np.random.default_rng(hs)
+    batch = Batch(rng, [100, 40, 150], [100, 333, 260], page)
+    codes, scales = random_cache(rng, batch.n_pages, 2, hs, page)
+    spread(rng, batch, scales, order)
+    q = rng.standard_normal((batch.n_rows, 2 * group, hs)) * 2
+    qv, out, lse = run_attention(cuda, q, codes, scales, batch, dtype, hs, hs**-0.5)
+    want, wlse, tol, ltol = attention(qv, codes, scales, batch, dtype, hs**-0.5)
+    agree(out, want, tol, dtype)
+    assert np.all(np.abs(lse - wlse) <= ltol)
+
+
+@pytest.mark.parametrize("rows,ctx", [([60], [200]), ([9, 200], [9, 200])])
+def test_attend_prompt_blind_to_later_pages(cuda, rows, ctx):
+    """Rows before a page have the same bits whatever that page's scales are."""
+    rng = np.random.default_rng(7)
+    hs, page = 64, 16
+    batch = Batch(rng, rows, ctx, page)
+    codes, scales = random_cache(rng, batch.n_pages, 1, hs, page)
+    q = rng.standard_normal((batch.n_rows, 1, hs)) * 2
+    last = int(batch.pages[-1, (ctx[-1] - 1) // page])  # positions 192 .. 199
+    for dtype in ("f32", "f16", "bf16"):
+        outs = []
+        for factor in (1.0, 2.0**20, np.nan):
+            other = scales.copy()
+            other[last] *= np.float32(factor)
+            outs.append(run_attention(cuda, q, codes, other, batch, dtype, hs, 0.125)[1:])
+        for out, lse in outs[1:]:
+            assert np.array_equal(out[:-8], outs[0][0][:-8]) and np.array_equal(lse[:-8], outs[0][1][:-8])
