@@ -5,6 +5,7 @@
 #include <cstdlib>
 #include <cstring>
 #include <mutex>
+#include <new>
 
 #include "lq_ctx.h"
 #include "lq_host.h"
@@ -93,44 +94,93 @@ int ensure_scratch(DevCtx* c, size_t bytes) {
     return LQ_OK;
 }
 
-// the workspace of the library's stream, with room for partial_bytes
+namespace {
+
+// zeroed counters and room for the partial results; allowed inside a capture,
+// of which nothing here becomes a part
+cudaError_t workspace_memory(size_t bytes, size_t head, void** out) {
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    cudaError_t e = cudaThreadExchangeStreamCaptureMode(&mode);
+    if (e != cudaSuccess) return e;
+    void* p = nullptr;
+    cudaStream_t st = nullptr;
+    e = cudaMalloc(&p, bytes);
+    if (e == cudaSuccess) e = cudaStreamCreateWithFlags(&st, cudaStreamNonBlocking);
+    if (e == cudaSuccess) e = cudaMemsetAsync(p, 0, head, st);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+    if (st) cudaStreamDestroy(st);
+    if (e != cudaSuccess && p) cudaFree(p);
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    *out = p;
+    return e;
+}
+
+void CUDART_CB workspace_released(void* w) { static_cast<DevCtx::Workspace*>(w)->held.store(0); }
+
+}  // namespace
+
+// A workspace with room for partial_bytes: the library's stream's, or, while that
+// stream is captured, one that belongs to the graph until the graph (and what was
+// instantiated from it) is destroyed.  A graph may be replayed on any stream, beside
+// calls on the stream it was captured on and beside other graphs.
 int stream_workspace(DevCtx* c, size_t partial_bytes, int** counters, void** partials) {
     constexpr size_t kHead = kWsCounters * sizeof(int);
-    DevCtx::Workspace* w = nullptr;
-    for (int i = 0; i < c->n_ws; ++i)
-        if (c->ws[i].stream == g_stream) w = &c->ws[i];
-    if (!w || w->bytes < kHead + partial_bytes) {
-        cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
-        if (cudaStreamIsCapturing(g_stream, &cs) == cudaSuccess && cs != cudaStreamCaptureStatusNone)
-            return lq_fail(LQ_EINVAL,
-                           "workspace of %zu bytes needed inside a graph capture: make one call of this size on this "
-                           "stream before capturing",
-                           partial_bytes);
-        if (!w && c->n_ws == c->cap_ws) {
-            const int cap = c->cap_ws ? 2 * c->cap_ws : 16;
-            void* m = realloc(c->ws, cap * sizeof(DevCtx::Workspace));
-            if (!m) return lq_fail(LQ_ENOMEM, "workspace table");
-            c->ws = static_cast<DevCtx::Workspace*>(m);
-            c->cap_ws = cap;
+    const size_t need = kHead + partial_bytes;
+    cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
+    unsigned long long id = 0;  // of a capture: not 0
+    cudaGraph_t graph = nullptr;
+    cudaError_t e = cudaStreamGetCaptureInfo(g_stream, &cs, &id, &graph);
+    if (e != cudaSuccess) return cuda_fail(e, "workspace");
+    const bool captured = cs == cudaStreamCaptureStatusActive;
+    if (!captured) id = 0;
+    DevCtx::Workspace *w = nullptr, *grows = nullptr;
+    for (DevCtx::Workspace* i = c->ws; i && !w; i = i->next)
+        if (i->held.load() && i->stream == g_stream && i->capture == id) {
+            if (i->bytes >= need)
+                w = i;
+            else
+                grows = i;
         }
-        // at least twice the old size: what growth leaves behind adds up to one workspace
-        size_t bytes = kHead + partial_bytes;
-        if (w && bytes < 2 * w->bytes) bytes = 2 * w->bytes;
-        if (bytes < (size_t)1 << 22) bytes = (size_t)1 << 22;
-        void* p = nullptr;
-        cudaError_t e = cudaMalloc(&p, bytes);
-        if (e == cudaSuccess) e = cudaMemset(p, 0, kHead);
-        if (e == cudaSuccess) e = cudaStreamSynchronize(nullptr);
-        if (e != cudaSuccess) {
-            if (p) cudaFree(p);
-            return cuda_fail(e, "workspace allocation");
-        }
+    if (!w) {
+        for (DevCtx::Workspace* i = c->ws; captured && i && !w; i = i->next)
+            if (!i->held.load() && i->bytes >= need) w = i;  // a destroyed graph's
         if (!w) {
-            w = &c->ws[c->n_ws++];
-            w->stream = g_stream;
+            // a stream's grows to at least twice the old size: what it leaves to launches
+            // in flight adds up to one workspace
+            size_t bytes = need;
+            if (!captured && grows && bytes < 2 * grows->bytes) bytes = 2 * grows->bytes;
+            const size_t least = captured ? (size_t)1 << 20 : (size_t)1 << 22;
+            if (bytes < least) bytes = least;
+            void* p = nullptr;
+            e = workspace_memory(bytes, kHead, &p);
+            if (e != cudaSuccess) return cuda_fail(e, "workspace allocation");
+            w = captured || !grows ? new (std::nothrow) DevCtx::Workspace : grows;
+            if (!w) {
+                cudaFree(p);
+                return lq_fail(LQ_ENOMEM, "workspace table");
+            }
+            w->p = p;
+            w->bytes = bytes;
+            if (w != grows) {
+                w->next = c->ws;
+                c->ws = w;
+            }
         }
-        w->p = p;
-        w->bytes = bytes;
+        w->stream = g_stream;
+        w->capture = id;
+        if (captured) {
+            cudaUserObject_t owner = nullptr;
+            e = cudaUserObjectCreate(&owner, w, workspace_released, 1, cudaUserObjectNoDestructorSync);
+            if (e != cudaSuccess) return cuda_fail(e, "workspace of a graph");
+            w->held.store(1);
+            e = cudaGraphRetainUserObject(graph, owner, 1, cudaGraphUserObjectMove);
+            if (e != cudaSuccess) {
+                cudaUserObjectRelease(owner, 1);
+                return cuda_fail(e, "workspace of a graph");
+            }
+        } else {
+            w->held.store(1);
+        }
     }
     *counters = static_cast<int*>(w->p);
     *partials = static_cast<char*>(w->p) + kHead;
@@ -238,8 +288,9 @@ int lq_sync(void) {
     if (!c) return lq_fail(LQ_ECUDA, "no CUDA device context (no device, or first use inside a graph capture)");
     const int a = check_device_error(c->err, g_stream);
     if (a) {  // a call that gave up may have left its arrival counters
-        for (int i = 0; i < c->n_ws; ++i)
-            if (c->ws[i].stream == g_stream) cudaMemsetAsync(c->ws[i].p, 0, kWsCounters * sizeof(int), g_stream);
+        for (DevCtx::Workspace* w = c->ws; w; w = w->next)
+            if (w->held.load() && w->capture == 0 && w->stream == g_stream)
+                cudaMemsetAsync(w->p, 0, kWsCounters * sizeof(int), g_stream);
     }
     const int b = noalloc_check_error(g_stream);  // always read (and clear) both words
     return a ? a : b;

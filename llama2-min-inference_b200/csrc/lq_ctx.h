@@ -4,6 +4,7 @@
 #include <cstdint>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <vector>
 
 #include "lq_host.h"
@@ -36,17 +37,17 @@ struct DevCtx {
         uint64_t used;
     };
     std::vector<CallGraph> graphs;
-    // workspaces of the token-scaled products and the paged attention, one per
-    // stream: kWsCounters arrival counters (zero between launches), then
-    // partial results.  One that grows leaves the old one allocated: captured
-    // graphs may hold it.
+    // workspaces of the paged attention, one per stream and one per captured graph:
+    // kWsCounters arrival counters (zero between launches), then partial results
     struct Workspace {
         cudaStream_t stream;
+        unsigned long long capture;  // the capture's id; 0: calls outside captures
+        std::atomic<int> held{0};    // 0: its graph is gone
         void* p;
         size_t bytes;
+        Workspace* next;
     };
     Workspace* ws = nullptr;
-    int n_ws = 0, cap_ws = 0;
     cudaStream_t capture = nullptr;  // private stream the graphs are captured on
     uint64_t tick = 0;
 };
