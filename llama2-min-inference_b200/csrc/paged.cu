@@ -585,6 +585,7 @@ int kv_append(const PagedKV* cache, const KVBatch* batch, const KVRows* rows) {
     AppendArgs a;
     a.c = *cache;
     a.b = *batch;
+    if (a.b.max_rows > a.b.n_rows) a.b.max_rows = a.b.n_rows;
     a.r = *rows;
     a.err = c->err;
     if (rows->q && rows->n_heads == 0) a.r.q = nullptr;

@@ -1579,6 +1579,7 @@ extern "C" int paged_attention(void* out, int64_t ld_out, const void* q, int64_t
     AttArgs a = {};
     a.c = *cache;
     a.b = *batch;
+    if (a.b.max_rows > a.b.n_rows) a.b.max_rows = a.b.n_rows;  // a bound, however far above: grids follow it
     a.q = q;
     a.out = out;
     a.lse = lse;
@@ -1591,7 +1592,7 @@ extern "C" int paged_attention(void* out, int64_t ld_out, const void* q, int64_t
     a.scale = scale * kLog2e;
     a.err = c->err;
     // few rows: every (sequence, kv head, row tile) is cut into splits of the context
-    const int64_t most_rows = (int64_t)batch->max_rows * a.group;
+    const int64_t most_rows = (int64_t)a.b.max_rows * a.group;
     const int tile_rows = most_rows <= 1 ? 1 : 8;
     a.row_tiles = (int)(((most_rows < kFewRows ? most_rows : kFewRows) + tile_rows - 1) / tile_rows);
     if (a.row_tiles < 1) a.row_tiles = 1;
