@@ -100,7 +100,8 @@ __device__ __forceinline__ uint32_t pack8(uint32_t a, uint32_t b, uint32_t c, ui
 // quotient (three roundings of a value up to 127), so where it is further than
 // 2^-13 from a half both round to the same integer; a word with one that is
 // not (one in a thousand) is divided.  Adding 1.5 * 2^23 leaves the rounded
-// integer in the low bits.
+// integer in the low bits.  A scale below fp32's normal numbers has few bits (190 of its smallest
+// steps over 127 round to one step), so those quotients are kept to 127.
 struct Quant8 {
     float s, inv;
     bool bad;  // the scale is NaN: codes 0
@@ -120,7 +121,7 @@ struct Quant8 {
         if (near > 0.5f - 1.220703125e-4f || inv == 0.0f) {
             if (bad) return 0u;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[e] = (uint32_t)__float2int_rn(x[e] / s);
+            for (int e = 0; e < 4; ++e) o[e] = (uint32_t)max(-127, min(127, __float2int_rn(x[e] / s)));
         }
         return pack8(o[0], o[1], o[2], o[3]);
     }
