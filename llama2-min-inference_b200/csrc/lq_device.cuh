@@ -125,6 +125,13 @@ __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;"
 __device__ __forceinline__ void pdl_trigger() {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
+// A load, after pdl_wait, of what the kernel before may have written.  Not the
+// read-only path (__ldg, const __restrict__): its data must not change while the kernel
+// runs, and with an early launch it runs while the one before still writes.
+template <typename T>
+__device__ __forceinline__ T ld_after(const T* p) {
+    return *p;
+}
 
 __device__ __forceinline__ void named_bar_sync(int id, int nthreads) {
     asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(nthreads) : "memory");

@@ -21,9 +21,9 @@ struct SeqRows {
 };
 
 __device__ __forceinline__ SeqRows seq_rows(const KVBatch& b, int s, int* err) {
-    const int a = __ldg(b.row_start + s), e = __ldg(b.row_start + s + 1);
+    const int a = ld_after(b.row_start + s), e = ld_after(b.row_start + s + 1);
     SeqRows q;
-    q.ctx = __ldg(b.context + s);
+    q.ctx = ld_after(b.context + s);
     q.first = q.r0 = a;
     q.n = e - a;
     if (a < 0 || e < a || e > b.n_rows || e - a > b.max_rows) {
@@ -47,7 +47,7 @@ __device__ __forceinline__ SeqRows seq_rows(const KVBatch& b, int s, int* err) {
 // the physical page of logical page lp, or -1 (recorded) when there is none
 __device__ __forceinline__ int64_t page_of(const PagedKV& c, const KVBatch& b, int s, int lp, int* err) {
     if (lp < b.max_pages) {
-        const int p = __ldg(b.pages + (int64_t)s * b.max_pages + lp);
+        const int p = ld_after(b.pages + (int64_t)s * b.max_pages + lp);
         if (p >= 0 && p < c.n_pages) return p;
     }
     set_err(err, DEV_BAD_PAGE);

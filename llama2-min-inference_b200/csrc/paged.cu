@@ -98,7 +98,7 @@ template <typename T, bool VEC, int MODE>
 __device__ __forceinline__ void rotate_queries(const AppendArgs& a, int unit, int lane) {
     const int hs = a.c.head_size, row = unit / a.q_parts, part = unit - row * a.q_parts;
     if (row >= a.b.n_rows) return;
-    const int s = find_seq(a.b.n_seqs, row, lane, [&](int i) { return __ldg(a.b.row_start + i); });
+    const int s = find_seq(a.b.n_seqs, row, lane, [&](int i) { return ld_after(a.b.row_start + i); });
     if (s < 0) return;
     const SeqRows q = seq_rows(a.b, s, lane == 0 ? a.err : nullptr);
     if (row < q.r0 || row >= q.r0 + q.n) return;
@@ -305,11 +305,11 @@ __global__ void __launch_bounds__(kAppendThreads, 4) append_kernel(const __grid_
     }
     const int hs = a.c.head_size, P = a.c.page_size, H = a.c.n_kv_heads;
     const int job = blockIdx.x / H, h = blockIdx.x % H;
-    const int s = find_seq(a.b.n_seqs, job, lane, [&](int i) { return __ldg(a.b.row_start + i) / P + 2 * i; });
+    const int s = find_seq(a.b.n_seqs, job, lane, [&](int i) { return ld_after(a.b.row_start + i) / P + 2 * i; });
     if (s < 0) return;
     const SeqRows q = seq_rows(a.b, s, tid == 0 ? a.err : nullptr);
     if (q.n <= 0) return;
-    const int lp = q.begin / P + (job - (__ldg(a.b.row_start + s) / P + 2 * s));
+    const int lp = q.begin / P + (job - (ld_after(a.b.row_start + s) / P + 2 * s));
     const int t0 = max(q.begin, lp * P), t1 = min(q.ctx, lp * P + P);  // the page's new tokens
     if (t0 >= t1) return;
     if (a.r.rope && t1 > a.r.rope_rows) {

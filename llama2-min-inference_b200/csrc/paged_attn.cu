@@ -62,20 +62,20 @@ struct RawQ {
         if constexpr (PARTS == 2) {
             const float* p = static_cast<const float*>(a.q) + i;
             if (a.q_vec) {
-                const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
+                const uint4 v = ld_after(reinterpret_cast<const uint4*>(p));
                 w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
             } else {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) w[e] = __float_as_uint(__ldg(p + e));
+                for (int e = 0; e < 4; ++e) w[e] = __float_as_uint(ld_after(p + e));
             }
         } else {
             const uint16_t* p = static_cast<const uint16_t*>(a.q) + i;
             if (a.q_vec) {
-                const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
+                const uint2 v = ld_after(reinterpret_cast<const uint2*>(p));
                 w[0] = v.x, w[1] = v.y;
             } else {
-                w[0] = __ldg(p) | (uint32_t)__ldg(p + 1) << 16;
-                w[1] = __ldg(p + 2) | (uint32_t)__ldg(p + 3) << 16;
+                w[0] = ld_after(p) | (uint32_t)ld_after(p + 1) << 16;
+                w[1] = ld_after(p + 2) | (uint32_t)ld_after(p + 3) << 16;
             }
         }
     }
@@ -275,7 +275,7 @@ struct Split {
 // has one at least.  By one warp; a sequence a lane.
 __device__ __forceinline__ Split find_split(const KVBatch& b, int unit, int units, int lane) {
     auto blocks = [&](int i) {  // of 128 tokens
-        return i < b.n_seqs ? (min(max(__ldg(b.context + i), 0), b.max_context) + 127) / 128 : 0;
+        return i < b.n_seqs ? (min(max(ld_after(b.context + i), 0), b.max_context) + 127) / 128 : 0;
     };
     asm volatile("prefetch.global.L1 [%0];" ::"l"(b.row_start + min(lane, b.n_seqs)));
     if (b.n_seqs == 1) return {0, unit, max(2, (blocks(0) + units - 1) / units) * 128};
@@ -385,7 +385,7 @@ __global__ void __launch_bounds__(kFewThreads, few_ctas(HS, ROWS)) attend_few_ke
         // the scales of the item's pages, by lane 0 (and 1): used one step later
         const int64_t pl = lane == 1 ? p1 : p0;
         float2 sc = make_float2(NAN, NAN);
-        if (lane < 2 && pl >= 0) sc = __ldg(reinterpret_cast<const float2*>(a.c.scales) + pl * H + h);
+        if (lane < 2 && pl >= 0) sc = ld_after(reinterpret_cast<const float2*>(a.c.scales) + pl * H + h);
         return sc;
     };
     __syncthreads();  // barriers are ready
@@ -1099,7 +1099,7 @@ __global__ void __launch_bounds__(many_threads(NS), 1) attend_many_kernel(const 
 #pragma unroll
             for (int i = 0; i < kLoads; ++i) {
                 const int c = kc0 + i * kcs;
-                kr[i] = at >= 0 && c * 16 < hs ? __ldg(src + c * P) : make_uint4(0, 0, 0, 0);
+                kr[i] = at >= 0 && c * 16 < hs ? ld_after(src + c * P) : make_uint4(0, 0, 0, 0);
             }
         };
         auto load_v = [&](int j) {  // after load_k(j)
@@ -1108,7 +1108,7 @@ __global__ void __launch_bounds__(many_threads(NS), 1) attend_many_kernel(const 
                 const int64_t at = ok && ptc[i] < TK / 16 ? bars->cell[j & 3][ptc[i]] : -1;
                 const uint4* src = reinterpret_cast<const uint4*>(codes + at) + (hs >> 4) * P +
                                    (((j * TK + ptc[i] * 16) & (P - 1)) >> 4) * hs + pd[i];
-                vr[i] = at >= 0 ? __ldg(src) : make_uint4(0, 0, 0, 0);
+                vr[i] = at >= 0 ? ld_after(src) : make_uint4(0, 0, 0, 0);
             }
         };
         load_k(0);
@@ -1249,7 +1249,7 @@ __global__ void __launch_bounds__(many_threads(NS), 1) attend_many_kernel(const 
                 sc_next = make_float2(NAN, NAN);
                 if (tok < seen) {
                     p_next = page_of(a.c, a.b, s, tok >> lp2, a.err);
-                    if (p_next >= 0) sc_next = __ldg(reinterpret_cast<const float2*>(a.c.scales) + p_next * H + h);
+                    if (p_next >= 0) sc_next = ld_after(reinterpret_cast<const float2*>(a.c.scales) + p_next * H + h);
                 }
             };
             Granule gr = {};
@@ -1311,7 +1311,7 @@ __global__ void __launch_bounds__(many_threads(NS), 1) attend_many_kernel(const 
                     if (a.q_vec) {
                         cp_async16(dst, src);
                     } else {
-                        for (int k = 0; k < 8; ++k) reinterpret_cast<uint16_t*>(dst)[k] = __ldg(src + k);
+                        for (int k = 0; k < 8; ++k) reinterpret_cast<uint16_t*>(dst)[k] = ld_after(src + k);
                     }
                 }
                 cp_async_wait();

@@ -19,7 +19,7 @@ namespace {
 
 template <typename T, bool VEC, int KEEP>
 __global__ void __maxnreg__(40)
-    quantize_rows_kernel(const T* __restrict__ x, int64_t ld, int n, int8_t* __restrict__ q, int pitch, float* __restrict__ s) {
+    quantize_rows_kernel(const T* x, int64_t ld, int n, int8_t* __restrict__ q, int pitch, float* __restrict__ s) {
     constexpr int E = 16 / sizeof(T);  // elements of a piece; their codes are E bytes
     constexpr int W = E / 4;           // elements of a word
     pdl_trigger();
@@ -188,8 +188,8 @@ __device__ __forceinline__ void store_columns(T* y, int64_t ld, const int (&acc)
 template <int CH>
 __device__ __forceinline__ void store_columns(const RowsArgs& a, int tok, int ch, const int (&v)[CH], int lane) {
     const int n = min(CH, a.rows - tok);
-    const float xsv = lane < n ? __ldg(a.xs + tok + lane) : 0.0f;
-    const float wsv = ch < a.d ? __ldg(a.ws + ch) : 0.0f;
+    const float xsv = lane < n ? ld_after(a.xs + tok + lane) : 0.0f;
+    const float wsv = ch < a.d ? ld_after(a.ws + ch) : 0.0f;
     const int64_t at = (int64_t)tok * a.ld + ch;
     if (a.type == LQ_F32)
         store_columns<CH>(static_cast<float*>(a.y) + at, a.ld, v, xsv, wsv, n, ch < a.d);
