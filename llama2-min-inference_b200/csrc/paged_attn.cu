@@ -1024,7 +1024,6 @@ __global__ void __launch_bounds__(many_threads(NS), 1) attend_many_kernel(const 
     const int tile = gridDim.x - 1 - blockIdx.x;  // long ones first
     const int h = blockIdx.y, s = blockIdx.z;
 
-    pdl_trigger();
     pdl_wait();
     const SeqRows q = seq_rows(a.b, s, a.few_rows == 0 && tile == 0 && h == 0 && tid == 0 ? a.err : nullptr);
     const int rows = q.n * g, base_row = tile * NQ * 128;
@@ -1068,6 +1067,9 @@ __global__ void __launch_bounds__(many_threads(NS), 1) attend_many_kernel(const 
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = bars->tmem_base;
+    // not before: a later kernel that takes tensor memory while it waits for this one
+    // (matmul_rows) would keep it from CTAs of this one that have none yet
+    pdl_trigger();
     const int8_t* codes = static_cast<const int8_t*>(a.c.codes);
 
     // 512 threads have 128 registers each; 128 scores a thread take a larger share,
