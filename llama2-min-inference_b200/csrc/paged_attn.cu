@@ -982,11 +982,13 @@ __device__ __forceinline__ uint2 codes_f16(uint32_t w) {
     return make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
 }
 
-// 4 codes to 2 x 2 bf16: the low 7 bits as the mantissa of 128, minus 128 (a
-// code of 0 to 127) or 256 (a negative one), which its sign bit makes of 128
+// 4 codes to 2 x 2 bf16, times 2^-16 (kBf16Codes undoes it): the low 7 bits as the
+// mantissa of 128, minus 128 (a code of 0 to 127) or 256 (a negative one), which its
+// sign bit makes of 128.  Any finite q of bf16 then has dots within fp32's range.
+constexpr float kBf16Codes = 65536.0f;
 __device__ __forceinline__ uint2 codes_bf16(uint32_t w) {
     auto two = [](uint32_t x) {
-        const uint32_t m = (x & 0x007F007Fu) | 0x43004300u, off = (x & 0x00800080u) | 0x43004300u;
+        const uint32_t m = (x & 0x007F007Fu) | 0x3B003B00u, off = (x & 0x00800080u) | 0x3B003B00u;
         const __nv_bfloat162 r =
             __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&m), *reinterpret_cast<const __nv_bfloat162*>(&off));
         return *reinterpret_cast<const uint32_t*>(&r);
@@ -1317,7 +1319,7 @@ __global__ void __launch_bounds__(many_threads(NS), 1) attend_many_kernel(const 
                     }
                 }
                 cp_async_wait();
-                bars->fs[i * 128 + w4 * 32 + lane] = fabsf(a.scale);
+                bars->fs[i * 128 + w4 * 32 + lane] = fabsf(a.scale) * (kBf16 ? kBf16Codes : 1.0f);
             } else {
                 // scaled and split, a few rows at a time (all their loads before the
                 // first use), 4 dims a lane

@@ -193,3 +193,19 @@ def test_attend_prompt_blind_to_later_pages(cuda, rows, ctx):
             outs.append(run_attention(cuda, q, codes, other, batch, dtype, hs, 0.125)[1:])
         for out, lse in outs[1:]:
             assert np.array_equal(out[:-8], outs[0][0][:-8]) and np.array_equal(lse[:-8], outs[0][1][:-8])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,ctx,hs", [([1], [300], 64), ([50], [120], 128), ([40, 3], [300, 50], 256)])
+@pytest.mark.parametrize("size", [1e-20, 1e20, 3e37])
+def test_attend_queries_of_any_size(cuda, dtype, rows, ctx, hs, size):
+    """Queries near the ends of fp32's range whose scores, by the scale, are ordinary."""
+    rng = np.random.default_rng(hs)
+    batch = Batch(rng, rows, ctx, 32)
+    codes, scales = random_cache(rng, batch.n_pages, 1, hs, 32)
+    q = np.clip(rng.standard_normal((batch.n_rows, 1, hs)), -5, 5) * size
+    scale = 2 / size / math.sqrt(hs)
+    qv, out, lse = run_attention(cuda, q, codes, scales, batch, dtype, hs, scale)
+    want, wlse, tol, ltol = attention(qv, codes, scales, batch, dtype, scale)
+    assert np.all(np.abs(out - want) <= tol), (np.abs(out - want) / tol).max()
+    assert np.all(np.abs(lse - wlse) <= ltol)
