@@ -316,7 +316,7 @@ def rope_table(positions: int, head_size: int, base: float = 10000.0):
     """numpy [positions, head_size / 2, 2] of (cos, sin) for kv_append."""
     import numpy as np
 
-    t = np.empty((max(positions, 0), head_size // 2, 2), np.float32)
+    t = np.empty((max(positions, 0), max(head_size // 2, 0), 2), np.float32)
     check(lib().lq_rope_table(t.ctypes.data, positions, head_size, base))
     return t
 
@@ -333,9 +333,10 @@ def paged_attention(out_ptr: int, q_ptr: int, n_heads: int, cache: PagedKV, batc
                     lse_ptr: int | None = None) -> None:
     """Causal attention of the batch's rows over the paged cache (scale: 1 / sqrt(head_size) when None)."""
     row = n_heads * cache.head_size
+    if scale is None:
+        scale = max(cache.head_size, 1) ** -0.5  # a head size below 1 is refused below
     rc = lib().paged_attention(out_ptr, row if ld_out is None else ld_out, q_ptr, row if ld_q is None else ld_q,
-                               dtype, n_heads, cache, batch,
-                               cache.head_size ** -0.5 if scale is None else scale, lse_ptr)
+                               dtype, n_heads, cache, batch, scale, lse_ptr)
     if rc != OK:
         raise LlamaQError(rc, last_error())
 
