@@ -209,3 +209,17 @@ def test_attend_queries_of_any_size(cuda, dtype, rows, ctx, hs, size):
     want, wlse, tol, ltol = attention(qv, codes, scales, batch, dtype, scale)
     assert np.all(np.abs(out - want) <= tol), (np.abs(out - want) / tol).max()
     assert np.all(np.abs(lse - wlse) <= ltol)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("hs,group,page", [(256, 1, 64), (144, 2, 16)])
+def test_attend_long_prompt_wide_heads(cuda, dtype, hs, group, page):
+    """Heads above 128 dims, prompts of several row tiles behind a context and not."""
+    rng = np.random.default_rng(hs)
+    batch = Batch(rng, [300, 170], [500, 170], page)
+    codes, scales = random_cache(rng, batch.n_pages, 1, hs, page)
+    q = rng.standard_normal((batch.n_rows, group, hs)) * 2
+    qv, out, lse = run_attention(cuda, q, codes, scales, batch, dtype, hs, hs**-0.5)
+    want, wlse, tol, ltol = attention(qv, codes, scales, batch, dtype, hs**-0.5)
+    assert np.all(np.abs(out - want) <= tol), (np.abs(out - want) / tol).max()
+    assert np.all(np.abs(lse - wlse) <= ltol)
