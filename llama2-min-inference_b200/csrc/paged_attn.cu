@@ -519,7 +519,8 @@ __global__ void __launch_bounds__(kFewThreads, few_ctas(HS, ROWS)) attend_few_ke
             if (t0 + 16 > pos) sv[1] = 0.0f;
         }
         const float svm = fmaxf(sv[0], sv[1]);
-        constexpr float kOne = 4294967040.0f;  // the largest weight: 2^32 less an ulp
+        // the largest weight, 2^32 less an ulp; its first digit is a unit of the products
+        constexpr float kOne = 4294967040.0f, kUnitOf = 16777216.0f / kOne;
         if constexpr (ROWS == 1) {
             // scores: the codes of 16 tokens are the A operand, q's digits the
             // columns 0-2 and, again, 4-6.  A lane so finds one digit pair or third
@@ -557,7 +558,7 @@ __global__ void __launch_bounds__(kFewThreads, few_ctas(HS, ROWS)) attend_few_ke
             const float p = exp2_fast(x - (top == -INFINITY ? 0.0f : top));
             l = fmaf(l, corr, p * rise);
             // the weight in fixed point; its bytes are the B operand's columns
-            float w = p, of = svm * rise * (1.0f / kOne);
+            float w = p, of = svm * rise * kUnitOf;
             if (P < kItem) {  // two pages
                 w = svm > 0.0f ? p * ((late ? sv[1] : sv[0]) / svm) : 0.0f;
                 const float most = max_redux(w);
@@ -639,7 +640,7 @@ __global__ void __launch_bounds__(kFewThreads, few_ctas(HS, ROWS)) attend_few_ke
             const float corr = exp2_fast(m - mref);  // 0 for the first tokens
             const float rise = exp2_fast(top - mref);
             m = top_new;
-            float sum = 0.0f, of = svm * rise * (1.0f / kOne);
+            float sum = 0.0f, of = svm * rise * kUnitOf;
 #pragma unroll
             for (int t = 0; t < 4; ++t)
 #pragma unroll
@@ -704,9 +705,9 @@ __global__ void __launch_bounds__(kFewThreads, few_ctas(HS, ROWS)) attend_few_ke
                     }
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        float v = fmaf(unbias(d[e]), 256.0f, unbias(d[2 + e]));
-                        v = fmaf(v, 256.0f, unbias(d3[e]));
-                        v = fmaf(v, 256.0f, unbias(d3[2 + e]));
+                        float v = fmaf(unbias(d3[2 + e]), 0.00390625f, unbias(d3[e]));
+                        v = fmaf(v, 0.00390625f, unbias(d[2 + e]));
+                        v = fmaf(v, 0.00390625f, unbias(d[e]));
                         o[t + i][e] = fmaf(v, of, o[t + i][e]);
                     }
                 }
@@ -740,8 +741,8 @@ __global__ void __launch_bounds__(kFewThreads, few_ctas(HS, ROWS)) attend_few_ke
             if constexpr (ROWS == 8) {
                 *reinterpret_cast<float2*>(mine + t * 8 + 2 * jj) = make_float2(o[t][0] + poison, o[t][1] + poison);
             } else {  // dim 8 t + lane / 4: two digits here, the others by the next lane
-                float v = fmaf(o[t][0], 256.0f, o[t][1]);
-                v = fmaf(v, 65536.0f, __shfl_down_sync(0xffffffffu, v, 1));
+                float v = fmaf(o[t][1], 0.00390625f, o[t][0]);
+                v = fmaf(__shfl_down_sync(0xffffffffu, v, 1), 1.52587890625e-5f, v);
                 if (jj == 0) mine[t * 8 + (lane >> 2)] = v + poison;
             }
         }

@@ -223,3 +223,22 @@ def test_attend_long_prompt_wide_heads(cuda, dtype, hs, group, page):
     want, wlse, tol, ltol = attention(qv, codes, scales, batch, dtype, hs**-0.5)
     assert np.all(np.abs(out - want) <= tol), (np.abs(out - want) / tol).max()
     assert np.all(np.abs(lse - wlse) <= ltol)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,ctx,group,page", [([1], [3000], 1, 64), ([1, 2], [90, 33], 4, 16), ([60], [200], 2, 32)])
+@pytest.mark.parametrize("size", [2.0**-105, 2.0**115])
+def test_attend_values_of_any_size(cuda, dtype, rows, ctx, group, page, size):
+    """Values near the ends of fp32's range keep their bits: a power of two in the
+    scales is one in the outputs."""
+    rng = np.random.default_rng(page)
+    hs = 64
+    batch = Batch(rng, rows, ctx, page)
+    codes, scales = random_cache(rng, batch.n_pages, 2, hs, page)
+    q = rng.standard_normal((batch.n_rows, 2 * group, hs)) * 2
+    far = scales.copy()
+    far[:, :, 1] *= np.float32(size)
+    qv, out, lse = run_attention(cuda, q, codes, far, batch, dtype, hs, 0.125)
+    want, wlse, tol, ltol = attention(qv, codes, scales, batch, dtype, 0.125)
+    assert np.all(np.abs(out / size - want) <= tol), (np.abs(out / size - want) / tol).max()
+    assert np.all(np.abs(lse - wlse) <= ltol)
