@@ -182,7 +182,7 @@ def generate(a, stream):
         token.copy_(out.argmax(-1))
         return out
 
-    got_logits.append(step().clone())  # not captured: the first use sets up the library's workspaces
+    got_logits.append(step().clone())  # not captured: the first step sets up what is allocated once
     got_tokens.append(token.clone())
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph, stream=stream):

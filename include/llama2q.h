@@ -202,7 +202,8 @@ int matmul_rows(void* xout, int type, int64_t ld, const QuantizedTensor* x, cons
  * [page_size / 16][head_size][16] (16 tokens of one dim together): both are
  * K-major tensor-core operands as they lie.  A token's value is code * scale.
  * scales: fp32 [n_pages][n_kv_heads][K, V].  Fresh memory needs no clearing: a
- * page's scale is set when its first token arrives. */
+ * page's scale is set when its first token arrives.  Attention takes any finite
+ * scales, however far those of a sequence's pages lie apart. */
 typedef struct PagedKV {
     void* codes;        /* device, 16-byte aligned */
     float* scales;      /* device, 8-byte aligned */
@@ -256,8 +257,9 @@ int lq_rope_table(float* table, int positions, int head_size, float base);
 
 /* Append the call's keys (rotated by their positions) and values to the cache,
  * and rotate its queries.  A page's scale is max|x|/127 over the tokens it has
- * ever held since its first one arrived (0 -> 1e-8); when new tokens raise it
- * from s to s', the codes of the earlier ones become rint(code * (s / s')).
+ * ever held since its first one arrived (a page of zeros has 1e-8, and keeps at
+ * least that); when new tokens raise it from s to s', the codes of the earlier ones
+ * become rint(code * (s / s')).
  * A NaN or an infinity makes the scale of its page and head NaN (codes zero)
  * until the page is begun again. */
 int kv_append(const PagedKV* cache, const KVBatch* batch, const KVRows* rows);
@@ -267,7 +269,9 @@ int kv_append(const PagedKV* cache, const KVBatch* batch, const KVRows* rows);
  * n_kv_heads (query head h reads kv head h / (n_heads / n_kv_heads)).  out and q
  * of `type`, head h of row r at element r * ld + h * head_size.  lse (may be
  * null): fp32 [n_rows][n_heads], log of the sum of exp(scale * q . K).  A row that
- * attends to nothing gives zeros and lse -inf. */
+ * attends to nothing gives zeros and lse -inf.  A row of q without a value of 1e-30
+ * or more may count as zeros.  Needs no call before a stream capture: a captured
+ * graph has a workspace of its own, and may be replayed on any stream. */
 int paged_attention(void* out, int64_t ld_out, const void* q, int64_t ld_q, int type, int n_heads,
                     const PagedKV* cache, const KVBatch* batch, float scale, float* lse);
 

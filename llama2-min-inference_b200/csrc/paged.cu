@@ -290,8 +290,10 @@ struct Walk {
 // L1 or L2) for the codes, in short loops by many threads: keeping the values in
 // registers between the two unrolled the code, whose instructions run once per
 // block, and was slower (69 us against 45 for 2048 fp32 tokens of 32 heads,
-// without queries).  Bound by issue slots and the loads' latency: prompts of 64 + 2
-// x 8 heads, 220 MB of bf16 rows and codes in pages of 16, take 47 us (4.7 TB/s).
+// without queries).  Prompts of 64 + 2 x 8 heads, 220 MB of bf16 rows and codes in
+// pages of 16, take 47 us (4.7 TB/s): neither DRAM (46%) nor the issue slots (54%)
+// are full, a block's chain of loads from its page's look-up to its codes is what a
+// small page costs.
 
 template <typename T, bool VEC, int MODE>
 __global__ void __launch_bounds__(kAppendThreads, 4) append_kernel(const __grid_constant__ AppendArgs a) {

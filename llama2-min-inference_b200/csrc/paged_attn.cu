@@ -234,7 +234,7 @@ __device__ __forceinline__ float unbias(int d) { return __int_as_float(d) - kBia
 // One row (a token, and a query head to each kv head): the codes are the MMA's
 // 16 rows, 16 tokens of K or 16 dims of V, and the digits its columns, so that
 // one MMA takes all digits and a lane one token's softmax.  64 sequences of the
-// case below take 78 us so, 120 us as a tile of 8 rows with seven empty.
+// case below take 77 us so, 102 us as a tile of 8 rows with seven empty.
 //
 // How long a split is follows from the contexts, which only the device knows
 // (a captured call's max_context is that of its longest replay): the least
@@ -246,11 +246,11 @@ __device__ __forceinline__ float unbias(int d) { return __int_as_float(d) - kBia
 // column 2j + e of the even tile is token 4j + 2x + e with x = j / 2, of the odd
 // tile with x = 1 - j / 2.
 //
-// Measured, 128 dims: 64 sequences of up to 1100 tokens, 40 heads, fp32 78 us (458
-// MB, 5.9 TB/s); 16 of up to 4000, 8 kv heads of 8 query heads each, 26 us (86
-// MB, 3.3 TB/s); 16 of 8192 each 53 us (5.1 TB/s); one of 2048, 32
-// heads, fp32 10.7 us.  What holds the short ones is the chain lengths, pages,
-// codes, and the two joins: 5 us with one split to a sequence, 8 us with more.
+// Measured, 128 dims: 64 sequences of up to 1100 tokens, 40 heads, fp32 77 us (458
+// MB, 5.9 TB/s); 16 of up to 4000, 8 kv heads of 8 query heads each, 26 us (86 MB,
+// 3.3 TB/s: DRAM 32% busy, issue slots 36%); 16 of 8192 each 57 us (4.7 TB/s); one
+// of 2048, 32 heads, fp32 10.6 us.  What holds the short ones is the chain lengths,
+// pages, codes, and the two joins: 5 us with one split to a sequence, 8 us with more.
 
 constexpr int kFewWarps = 4;
 constexpr int kFewThreads = 32 * kFewWarps;
@@ -924,8 +924,8 @@ cudaError_t few_launch(const AttArgs& a, dim3 grid, cudaStream_t st) {
 // more than 2^kGrow since its last one: weights are 2^kUnit at that maximum, 2^14 at
 // most, and have 11 bits, down to 2^-31 of the largest (fp32: 22, down to 2^-36).
 //
-// Measured, 1024 rows at the end of 4096 tokens, 32 heads of 128: bf16 117 us
-// (60 GFLOP, 515 TFLOP/s), fp32 161 us.  What bounds it is the conversion (93 us
+// Measured, 1024 rows at the end of 4096 tokens, 32 heads of 128: bf16 119 us
+// (60 GFLOP, 505 TFLOP/s), fp32 162 us.  What bounds it is the conversion (93 us
 // without it), then a row tile's chain from scores through softmax to the next
 // product, which two row tiles on an SM hide only in part (tensor pipe and issue
 // slots are both under half busy).  Tiles of 128 tokens with one buffer of scores
@@ -1601,9 +1601,9 @@ extern "C" int paged_attention(void* out, int64_t ld_out, const void* q, int64_t
     const int tile_rows = most_rows <= 1 ? 1 : 8;
     a.row_tiles = (int)(((most_rows < kFewRows ? most_rows : kFewRows) + tile_rows - 1) / tile_rows);
     if (a.row_tiles < 1) a.row_tiles = 1;
-    // Splits of contexts, as many as find a CTA slot each (three CTAs to an SM,
-    // one beyond 128 dims): a second round costs more than uneven contexts (16
-    // sequences of the 70B shape 27 us in one, 35 us in two).
+    // Splits of contexts, as many as find a CTA slot each (few_ctas of them to an
+    // SM): a second round costs more than uneven contexts (16 sequences of the 70B
+    // shape 26 us in one, 32 us in two).
     const int64_t x = (int64_t)cache->n_kv_heads * a.row_tiles;
     const int64_t slots = few_ctas(cache->head_size, tile_rows) * c->num_sms;
     const int64_t most_splits = (int64_t)batch->n_seqs * ((batch->max_context + 255) / 256);
